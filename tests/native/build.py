@@ -19,7 +19,7 @@ def build():
     if (not os.path.exists(exe) or os.path.getmtime(exe) < os.path.getmtime(src)
             or os.path.getmtime(exe) < os.path.getmtime(lib)):
         libdir = os.path.dirname(lib)
-        cmd = [libbuild.find_hipcc(), "--offload-arch=gfx950", "-O2", "-std=c++17", "-x", "hip", src, "-o", exe,
+        cmd = [libbuild.find_hipcc(), "--offload-arch=gfx950", "-O2", "-std=c++17"] + libbuild.NO_PACKED_FP32 + ["-x", "hip", src, "-o", exe,
                "-L" + libdir, "-luniter_hip", "-Wl,-rpath,$ORIGIN/../../../uniter_amd/csrc/build"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:

@@ -4,11 +4,12 @@
     python uniter_amd/csrc/build.py [--force] [--verbose]
 
 One object per .hip file (parallel), linked into uniter_amd/csrc/build/libuniter_hip.so.  Rebuilds only
-objects whose sources (or shared headers) are newer.  hipcc cross-compiles without a GPU.
+objects whose sources (or the headers they include) are newer.  hipcc cross-compiles without a GPU.
 """
 import argparse
 import concurrent.futures as cf
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -20,9 +21,10 @@ ROOT = os.path.dirname(os.path.dirname(HERE))
 BUILD = os.path.join(HERE, os.environ.get("UNITER_BUILD_DIR", "build"))
 LIB = os.path.join(BUILD, "libuniter_hip.so")
 SOURCES = ["capi.hip", "gemm.hip", "attention.hip", "layernorm.hip", "embed.hip", "adamw.hip", "encoder.hip", "comm.hip", "ot.hip", "pool.hip", "lmhead.hip", "head.hip"]
-HEADERS = [os.path.join(HERE, h) for h in ("common.cuh", "kernels.h", "gemm_lds.cuh", "gemm_args.cuh", "gemm8.cuh", "attention_fwd.cuh", "layernorm_fwd.cuh")] + \
-    [os.path.join(ROOT, "include", "uniter_hip.h")]
 ARCH = "gfx950"
+# No packed FP32 arithmetic (v_pk_add / mul / fma_f32) in device code: some of its forms have given wrong results now and then, with no
+# error, and -O3 forms it by itself from ordinary float code.  (The host pass does not know the feature and warns: harmless.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def find_hipcc():
@@ -39,18 +41,30 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _sources_of(path, seen=None):
+    """`path`, the files that it includes by name (recursively) and this script, whose flags they are compiled with."""
+    seen = {os.path.abspath(__file__)} if seen is None else seen
+    path = os.path.normpath(path)
+    if path not in seen:
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^\s*#\s*include\s+"([^"]+)"', f.read(), flags=re.M):
+                _sources_of(os.path.join(os.path.dirname(path), name), seen)
+    return seen
+
+
 def build(force=False, verbose=False):
     hipcc = find_hipcc()
     os.makedirs(BUILD, exist_ok=True)
     flags = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Wall", "-Wno-unused-function",
-             "-DNDEBUG"] + os.environ.get("UNITER_EXTRA_FLAGS", "").split()
+             "-DNDEBUG"] + NO_PACKED_FP32 + os.environ.get("UNITER_EXTRA_FLAGS", "").split()
     jobs = []
     objs = []
     for src in SOURCES:
         s = os.path.join(HERE, src)
         o = os.path.join(BUILD, src.replace(".hip", ".o"))
         objs.append(o)
-        if force or _stale(o, [s] + HEADERS):
+        if force or _stale(o, _sources_of(s)):
             jobs.append((s, o))
 
     def compile_one(job):

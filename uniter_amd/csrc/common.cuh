@@ -312,10 +312,10 @@ __device__ __forceinline__ float dropout_mult1(const DropoutCfg& d, uint64_t idx
 // erf(z) = 1 - (a1 t + ... + a5 t^5) exp(-z^2), t = 1/(1 + p z)  (Abramowitz-Stegun 7.1.26, |error| <= 1.5e-7,
 // far below the bf16 resolution of the stored result) with z = |x|/sqrt2, so exp(-z^2) = exp(-x^2/2) serves both.
 // Two elements at a time: the GEMM epilogues that apply it are VALU-bound on it (a 3072 x 3072 output is 5-6 us of
-// nothing but this on every SIMD), so the multiplies and fused multiply-adds are packed (v_pk_fma_f32 / v_pk_mul_f32: two
-// elements per issue slot), the reciprocal is the hardware's v_rcp_f32 (1 ulp: __frcp_rn expands to a ten-instruction
+// nothing but this on every SIMD).  The build forms no packed FP32 instructions (build.py), so a pair is two scalar
+// sequences side by side; the reciprocal is the hardware's v_rcp_f32 (1 ulp: __frcp_rn expands to a ten-instruction
 // correctly rounded division) and the exponential is one multiply + v_exp_f32.  The scalar entry points run the same
-// instruction sequence on a duplicated pair, so an element gets the same bits from every caller.
+// instruction sequence, so an element gets the same bits from every caller.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void normal_cdf_pdf2(const f32x2_t x, f32x2_t& cdf, f32x2_t& pdf) {
     // every multiply-add is spelled out (and nothing else may be contracted): the same bits wherever this is inlined
@@ -366,7 +366,7 @@ __device__ __forceinline__ float act_grad(int act, float x) {
     if (act == UH_ACT_SWISH) { const float s = __frcp_rn(1.0f + __expf(-x)); return s * (1.0f + x * (1.0f - s)); }
     return gelu_erf_grad(x);
 }
-// the same for two elements (the GEMM epilogues): GELU on the packed path, the other activations element by element
+// the same for two elements (the GEMM epilogues): GELU two elements at a time, the other activations one by one
 __device__ __forceinline__ f32x2_t act_fwd2(int act, const f32x2_t x) {
     if (act == UH_ACT_GELU) return gelu_erf2(x);
     return f32x2_t{act_fwd(act, x.x), act_fwd(act, x.y)};
