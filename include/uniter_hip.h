@@ -606,6 +606,73 @@ int uniter_attn_pool_bwd(const void* x, const void* w, const float* raw, const f
                          void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Rotary positions (no counterpart in the reference, whose positions are learned and end at max_position_embeddings,
+ * model/model.py:217-245): the pairs of the first rot_dim elements of every head are turned by position * freq[pair].
+ *   half layout   (interleaved == 0): pair i is elements i and rot_dim / 2 + i;   interleaved: elements 2 i and 2 i + 1.
+ * x, y: bf16 [B, L, heads, head_dim], head elements contiguous, the other three strides free ({batch, token, head}, in elements;
+ * 16-byte-aligned heads and rot_dim % 16 == 0 run on 16-byte accesses).  y == x with equal strides turns in place.
+ * inverse != 0 turns back by the same angles, with the same multiplier: the gradient of x from the gradient of y.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct UniterRotary {
+    int64_t B, L, heads, head_dim, rot_dim;
+    const double* freq;              /* [rot_dim / 2] device, TURNS per position (angle / 2 pi) */
+    const int64_t* positions;        /* device, token l of row b: positions[b * positions_batch_stride + l]; NULL = l */
+    int64_t positions_batch_stride;  /* 0: one row of positions for the whole batch */
+    int64_t position_offset;         /* added to every position */
+    float multiplier;                /* factor on the turned elements (1, or the attention factor of a scaled context) */
+    int32_t interleaved, inverse;
+} UniterRotary;
+int uniter_rotary(const UniterRotary* r, const void* x, const int64_t* x_strides, void* y, const int64_t* y_strides, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Differential attention (no counterpart in the reference; it stands beside the softmax attention of model/layer.py:75-101):
+ *   S_j = q_j k_j^T / sqrt(d) + mask_bias,  P_j = softmax(S_j),  j = 1, 2
+ *   o = dropout(P_1 - lambda P_2) v,  lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init
+ *   out = (1 - lambda_init) norm_weight . o / sqrt(mean(o^2) + norm_eps) per head  (norm_weight NULL: out = o)
+ * A head is 2 d columns of q, k, v and out (d = head_dim, 32 or 64): the first d of q / k belong to map 1, the rest to map 2.  With
+ * d = 32 a head is the 64 columns of a BertSelfAttention head.  Any lengths, Lq and Lk apart; rows of a head are 16-byte aligned.
+ *   dense:  q [B, Lq, ..], k / v [B, Lk, ..], strides in elements; mask_bias [B, Lk] fp32 (row stride mask_row) is added to the scores
+ *           of both maps, NULL = none.  -inf takes a key out for good (what k and v hold there is never used); a row left
+ *           without keys gives zeros and no gradient.
+ *   packed: cu_seqlens_q / _k, device int32 [B + 1]: example b owns rows cu[b] .. cu[b + 1] - 1 of q / out and k / v; Lq / Lk are then
+ *           the longest examples, total_q / total_k the rows there are, the batch strides are ignored, and rows outside every
+ *           example (or behind Lq / Lk rows of one) are neither read nor written.
+ * lambda_*: bf16, [heads, d] (lambda_per_head != 0) or [d] for all heads; norm_weight bf16 [2 d].
+ * Dropout keeps or drops elements of the difference (one draw for both maps), stream as in the header's conventions.
+ * For a backward pass the forward keeps stats [B, heads, Lq, 4] and maps [rows, heads, 2, 2 d], both fp32 (rows = B Lq, or total_q);
+ * both NULL: nothing is kept. */
+typedef struct UniterDiffAttention {
+    const void *q, *k, *v;
+    int64_t q_row, k_row, v_row;          /* row strides, multiples of 8 */
+    int64_t q_batch, k_batch, v_batch;
+    const float* mask_bias;
+    int64_t mask_row;
+    const int32_t *cu_seqlens_q, *cu_seqlens_k;
+    int64_t total_q, total_k;
+    const void *lambda_q1, *lambda_k1, *lambda_q2, *lambda_k2;
+    const void* norm_weight;
+    int64_t B, Lq, Lk, heads, head_dim;
+    float lambda_init, norm_eps, p_drop;
+    int32_t lambda_per_head;
+    uint64_t seed, offset;
+} UniterDiffAttention;
+/* Gradients: q, k, v are overwritten (strides as above); the five parameters' are added to what is there when accumulate_params != 0
+ * and overwritten otherwise; a NULL among those five is not written. */
+typedef struct UniterDiffAttentionGrads {
+    void *q, *k, *v;
+    int64_t q_row, k_row, v_row;
+    int64_t q_batch, k_batch, v_batch;
+    void *lambda_q1, *lambda_k1, *lambda_q2, *lambda_k2;
+    void* norm_weight;
+    int64_t accumulate_params;
+} UniterDiffAttentionGrads;
+int uniter_diff_attention_fwd(const UniterDiffAttention* a, void* out, int64_t out_row, int64_t out_batch, float* stats, float* maps,
+                              void* stream);
+size_t uniter_diff_attention_bwd_workspace_bytes(const UniterDiffAttention* a);
+int uniter_diff_attention_bwd(const UniterDiffAttention* a, const float* stats, const float* maps, const void* dout, int64_t dout_row,
+                              int64_t dout_batch, const UniterDiffAttentionGrads* g, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Word-region alignment loss: IPOT optimal-transport distance.
  * Replaces model/ot.py:11-85 (cost_matrix_cosine, ipot, trace) and the un-compaction scatter of
  * model/pretrain.py:166-181 — one workgroup per example instead of ~8 PyTorch launches x 50 iterations.

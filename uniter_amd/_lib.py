@@ -48,6 +48,29 @@ class UniterEncoderShape(Structure):
                 ("total_tokens", c_int64), ("cu_seqlens", c_void_p), ("hidden_act", c_int32)]
 
 
+class UniterRotary(Structure):
+    _fields_ = [("B", c_int64), ("L", c_int64), ("heads", c_int64), ("head_dim", c_int64), ("rot_dim", c_int64),
+                ("freq", c_void_p), ("positions", c_void_p), ("positions_batch_stride", c_int64), ("position_offset", c_int64),
+                ("multiplier", c_float), ("interleaved", c_int32), ("inverse", c_int32)]
+
+
+class UniterDiffAttention(Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_row", c_int64), ("k_row", c_int64), ("v_row", c_int64),
+                ("q_batch", c_int64), ("k_batch", c_int64), ("v_batch", c_int64), ("mask_bias", c_void_p), ("mask_row", c_int64),
+                ("cu_seqlens_q", c_void_p), ("cu_seqlens_k", c_void_p), ("total_q", c_int64), ("total_k", c_int64),
+                ("lambda_q1", c_void_p), ("lambda_k1", c_void_p), ("lambda_q2", c_void_p), ("lambda_k2", c_void_p),
+                ("norm_weight", c_void_p), ("B", c_int64), ("Lq", c_int64), ("Lk", c_int64), ("heads", c_int64), ("head_dim", c_int64),
+                ("lambda_init", c_float), ("norm_eps", c_float), ("p_drop", c_float), ("lambda_per_head", c_int32),
+                ("seed", c_uint64), ("offset", c_uint64)]
+
+
+class UniterDiffAttentionGrads(Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_row", c_int64), ("k_row", c_int64), ("v_row", c_int64),
+                ("q_batch", c_int64), ("k_batch", c_int64), ("v_batch", c_int64),
+                ("lambda_q1", c_void_p), ("lambda_k1", c_void_p), ("lambda_q2", c_void_p), ("lambda_k2", c_void_p),
+                ("norm_weight", c_void_p), ("accumulate_params", c_int64)]
+
+
 class UniterAdamTensor(Structure):
     _fields_ = [("param", c_void_p), ("grad", c_void_p), ("master", c_void_p), ("exp_avg", c_void_p),
                 ("exp_avg_sq", c_void_p), ("numel", c_int64), ("group", c_int32), ("param_is_bf16", c_int32)]
@@ -174,6 +197,11 @@ SIGNATURES = {
     "uniter_attn_pool_workspace_bytes": (c_size_t, [_I, _I]),
     "uniter_attn_pool_fwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, c_float, c_uint64, c_uint64, _P]),
     "uniter_attn_pool_bwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, c_size_t, _P]),
+    "uniter_rotary": (c_int, [POINTER(UniterRotary), _P, POINTER(c_int64), _P, POINTER(c_int64), _P]),
+    "uniter_diff_attention_fwd": (c_int, [POINTER(UniterDiffAttention), _P, _I, _I, _P, _P, _P]),
+    "uniter_diff_attention_bwd_workspace_bytes": (c_size_t, [POINTER(UniterDiffAttention)]),
+    "uniter_diff_attention_bwd": (c_int, [POINTER(UniterDiffAttention), _P, _P, _P, _I, _I, POINTER(UniterDiffAttentionGrads), _P,
+                                          c_size_t, _P]),
     "uniter_ot_fwd": (c_int, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, c_float, c_int32, c_int32, _P]),
     "uniter_ot_bwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "uniter_nlvr2_pair_masks": (c_int, [_P, _P, _P, _I, _I, _P]),

@@ -20,7 +20,8 @@ ROOT = os.path.dirname(os.path.dirname(HERE))
 #  a variant up through UNITER_AMD_LIB=<path to its libuniter_hip.so> / LD_LIBRARY_PATH for the native harness)
 BUILD = os.path.join(HERE, os.environ.get("UNITER_BUILD_DIR", "build"))
 LIB = os.path.join(BUILD, "libuniter_hip.so")
-SOURCES = ["capi.hip", "gemm.hip", "attention.hip", "layernorm.hip", "embed.hip", "adamw.hip", "encoder.hip", "comm.hip", "ot.hip", "pool.hip", "lmhead.hip", "head.hip"]
+SOURCES = ["capi.hip", "gemm.hip", "attention.hip", "layernorm.hip", "embed.hip", "adamw.hip", "encoder.hip", "comm.hip", "ot.hip", "pool.hip", "lmhead.hip", "head.hip", "rotary.hip",
+           "diff_attention.hip"]
 ARCH = "gfx950"
 # No packed FP32 arithmetic (v_pk_add / mul / fma_f32) in device code: some of its forms have given wrong results now and then, with no
 # error, and -O3 forms it by itself from ordinary float code.  (The host pass does not know the feature and warns: harmless.)

@@ -846,6 +846,312 @@ def dense_gelu(mod, hidden_states):
 
 
 # ----------------------------------------------------------------------------------------------------
+# rotary positions and differential attention (no counterpart in the reference: they stand beside BertSelfAttention's learned
+# positions and softmax attention, model/layer.py:75-101, model/model.py:217-245)
+# ----------------------------------------------------------------------------------------------------
+class _on_device(object):
+    """Make the device of `t` the current one for the launches inside (free when it already is)."""
+
+    def __init__(self, t):
+        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _same_device(first, name, *others):
+    for t, what in others:
+        if t is not None and t.device != first.device:
+            raise _lib.UniterHipError("%s is on %s, %s on %s" % (what, t.device, name, first.device))
+
+
+def _rows16(t):
+    """`t` with contiguous rows that start on 16 bytes (a copy when they do not)."""
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+    return t if ok and all(s % 8 == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])) else t.contiguous()
+
+
+def _rotary_launch(x, y, positions, offset, rot, inverse):
+    if x.numel() == 0:
+        return
+    B, L = (x.shape[0], x.shape[1]) if x.dim() == 4 else (1, x.shape[0])
+    r = _lib.UniterRotary()
+    r.B, r.L, r.heads, r.head_dim, r.rot_dim = B, L, x.shape[-2], x.shape[-1], rot.rotary_dim
+    turns = rot.turns(x.device)
+    r.freq, r.positions = turns.data_ptr(), ptr(positions)
+    r.positions_batch_stride = 0 if positions is None or positions.dim() == 1 else positions.stride(0)
+    r.position_offset = offset
+    r.multiplier, r.interleaved, r.inverse = rot.multiplier, int(rot.interleaved), int(inverse)
+    strides = [(ctypes.c_int64 * 3)(*(((0,) if t.dim() == 3 else ()) + tuple(t.stride()[:-1]))) for t in (x, y)]
+    with _on_device(x):
+        C.uniter_rotary(ctypes.byref(r), ptr(x), strides[0], ptr(y), strides[1], _lib.stream_ptr())
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, offset, rot):
+        y = torch.empty(x.shape, dtype=_BF16, device=x.device)
+        _rotary_launch(x, y, positions, offset, rot, False)
+        ctx.offset, ctx.rot = offset, rot
+        ctx.save_for_backward(positions)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        positions, = ctx.saved_tensors
+        dy = dy if dy.stride(-1) == 1 or dy.numel() == 0 else dy.contiguous()
+        dx = torch.empty(dy.shape, dtype=_BF16, device=dy.device)
+        _rotary_launch(dy, dx, positions, ctx.offset, ctx.rot, True)
+        return dx, None, None, None
+
+
+def rotary(x, positions, rot, offset=0, out=None):
+    """Turn the heads of x by their token positions (model/rotary.py::RotaryPositions `rot`).
+
+    x: bf16 [B, L, heads, head_dim], or [T, heads, head_dim] for rows back to back (a packed batch); any strides with contiguous heads
+    (a slice of a fused projection is read in place).  positions: integer tensor [B, L] or [L] ([T]) on x's device, or None for
+    0 .. L - 1 (of every row of the batch); `offset` is added to either.  Returns a new tensor; out=x turns x in place, out=another
+    tensor of x's shape writes there (both outside autograd only).  The gradient is turned back by the same kernel."""
+    _check_dev(x, "rotary input")
+    if x.dim() not in (3, 4) or x.shape[-1] != rot.head_dim:
+        raise _lib.UniterHipError("rotary input must be [B, L, heads, %d] or [T, heads, %d], got %s" % (rot.head_dim, rot.head_dim, tuple(x.shape)))
+    rows = tuple(x.shape[:-2])
+    if x.dim() == 3 and positions is None:
+        raise _lib.UniterHipError("rotary: rows stored back to back need their positions")
+    if positions is not None:
+        if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int64, torch.int32):
+            raise _lib.UniterHipError("rotary: positions must be an int64 or int32 tensor (or None)")
+        _same_device(x, "x", (positions, "positions"))
+        if positions.dim() == 2 and positions.shape[0] == 1 and len(rows) == 2:
+            positions = positions[0]
+        if tuple(positions.shape) not in (rows, rows[-1:]):
+            raise _lib.UniterHipError("rotary: positions must be %s or %s, got %s" % (list(rows), list(rows[-1:]), list(positions.shape)))
+        positions = positions.to(torch.int64)
+        if positions.numel() and positions.stride(-1) != 1:
+            positions = positions.contiguous()
+    if x.stride(-1) != 1 and x.numel():
+        if out is x:
+            raise _lib.UniterHipError("rotary: in place needs contiguous heads")
+        x = x.contiguous()
+    if out is None:
+        return _RotaryFn.apply(x, positions, int(offset), rot)
+    if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
+        raise _lib.UniterHipError("rotary: out= writes outside autograd; call it without gradients or let it return a new tensor")
+    _check_dev(out, "rotary output")
+    _same_device(x, "x", (out, "out"))
+    if out.shape != x.shape or (out.numel() and out.stride(-1) != 1):
+        raise _lib.UniterHipError("rotary: out must have x's shape and contiguous heads")
+    if out.numel() and out.data_ptr() != x.data_ptr() and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() \
+            and _overlap(out, x):
+        raise _lib.UniterHipError("rotary: out overlaps x without being x")
+    _rotary_launch(x, out, positions, int(offset), rot, False)
+    return out
+
+
+def _overlap(a, b):
+    """Whether the address ranges of two views of one storage meet AND their rows can (equal strides and interleaved rows that stay
+    apart — q and k blocks of one projection — do not)."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + 2 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    row = a.stride(-3)
+    if a.stride() == b.stride() and a.dim() >= 3 and row >= a.shape[-2] * a.stride(-2):
+        # same row pitch: rows of width w at offsets d apart modulo the pitch
+        w, d = a.shape[-2] * a.stride(-2), (abs(a0 - b0) // 2) % row
+        return d < w or row - d < w
+    return True
+
+
+def _diff_args(q, k, v, heads, dim, lams, lambda_init, weight, eps, mask, cu_q, cu_k, max_q, max_k, p, seed, off):
+    a = _lib.UniterDiffAttention()
+    a.q, a.k, a.v = ptr(q), ptr(k), ptr(v)
+    a.q_row, a.k_row, a.v_row = q.stride(-2), k.stride(-2), v.stride(-2)
+    if cu_q is None:
+        a.q_batch, a.k_batch, a.v_batch = q.stride(0), k.stride(0), v.stride(0)
+        a.B, a.Lq, a.Lk = q.shape[0], q.shape[1], k.shape[1]
+    else:
+        a.cu_seqlens_q, a.cu_seqlens_k = ptr(cu_q), ptr(cu_k)
+        a.total_q, a.total_k = q.shape[0], k.shape[0]
+        a.B, a.Lq, a.Lk = cu_q.numel() - 1, max_q, max_k
+    if mask is not None:
+        a.mask_bias, a.mask_row = ptr(mask), mask.stride(0)
+    a.lambda_q1, a.lambda_k1, a.lambda_q2, a.lambda_k2 = [ptr(t) for t in lams]
+    a.norm_weight = ptr(weight)
+    a.heads, a.head_dim = heads, dim
+    a.lambda_init, a.norm_eps, a.p_drop = lambda_init, eps, p
+    a.lambda_per_head = int(lams[0].dim() == 2)
+    a.seed, a.offset = seed, off
+    return a
+
+
+def _diff_forward(q, k, v, cfg, lams, weight, mask, cu_q, cu_k, keep):
+    """(out, stats, maps): one launch on the current stream; stats / maps only when a backward pass will want them."""
+    heads, dim, lambda_init, eps, max_q, max_k, p, seed, off = cfg
+    a = _diff_args(q, k, v, heads, dim, lams, lambda_init, weight, eps, mask, cu_q, cu_k, max_q, max_k, p, seed, off)
+    # rows of a packed batch that belong to no example are not written: they are zeros
+    out = (torch.empty if cu_q is None else torch.zeros)(q.shape, dtype=_BF16, device=q.device)
+    stats = maps = None
+    if keep:
+        stats = torch.empty(a.B * heads * a.Lq * 4, dtype=torch.float32, device=q.device)
+        maps = torch.empty(out.numel() * 2, dtype=torch.float32, device=q.device)
+    with _on_device(q):
+        C.uniter_diff_attention_fwd(ctypes.byref(a), ptr(out), out.stride(-2), out.stride(0) if cu_q is None else 0,
+                                    ptr(stats), ptr(maps), _lib.stream_ptr())
+    return out, stats, maps
+
+
+def _diff_backward(q, k, v, cfg, lams, weight, mask, cu_q, cu_k, stats, maps, dout, dq, dk, dv, dlams, dweight, accumulate):
+    heads, dim, lambda_init, eps, max_q, max_k, p, seed, off = cfg
+    a = _diff_args(q, k, v, heads, dim, lams, lambda_init, weight, eps, mask, cu_q, cu_k, max_q, max_k, p, seed, off)
+    g = _lib.UniterDiffAttentionGrads()
+    g.q, g.k, g.v = ptr(dq), ptr(dk), ptr(dv)
+    g.q_row, g.k_row, g.v_row = dq.stride(-2), dk.stride(-2), dv.stride(-2)
+    if cu_q is None:
+        g.q_batch, g.k_batch, g.v_batch = dq.stride(0), dk.stride(0), dv.stride(0)
+    g.lambda_q1, g.lambda_k1, g.lambda_q2, g.lambda_k2 = [ptr(t) for t in dlams]
+    g.norm_weight, g.accumulate_params = ptr(dweight), int(accumulate)
+    n = C.uniter_diff_attention_bwd_workspace_bytes(ctypes.byref(a))
+    # (from the caching allocator, not a shared scratch buffer: calls on other streams and captured graphs get memory of their own)
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
+    with _on_device(q):
+        C.uniter_diff_attention_bwd(ctypes.byref(a), ptr(stats), ptr(maps), ptr(dout), dout.stride(-2),
+                                    dout.stride(0) if cu_q is None else 0, ctypes.byref(g), ptr(ws), n, _lib.stream_ptr())
+
+
+class _DiffAttentionFn(torch.autograd.Function):
+    """fused: `q` is the whole [.., 3 H] projection (k, v None), and so is its gradient."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, mask, cu_q, cu_k, cfg, keep, weight, *lams):
+        ctx.fused = k is None
+        qs, ks, vs = q.split(q.shape[-1] // 3, dim=-1) if ctx.fused else (q, k, v)
+        out, stats, maps = _diff_forward(qs, ks, vs, cfg, lams, weight, mask, cu_q, cu_k, keep)
+        ctx.cfg = cfg
+        if keep:
+            ctx.save_for_backward(q, k, v, mask, cu_q, cu_k, weight, stats, maps, *lams)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, mask, cu_q, cu_k, weight, stats, maps = ctx.saved_tensors[:9]
+        lams = ctx.saved_tensors[9:]
+        dout = _rows16(dout)
+        new = torch.empty if cu_q is None else torch.zeros             # rows of no example have no gradient
+        dq = new(q.shape, dtype=_BF16, device=q.device)
+        if ctx.fused:
+            H = q.shape[-1] // 3
+            qs, ks, vs = q.split(H, dim=-1)
+            dqs, dks, dvs = dq.split(H, dim=-1)
+            dk = dv = None
+        else:
+            dk, dv = (new(t.shape, dtype=_BF16, device=q.device) for t in (k, v))
+            qs, ks, vs, dqs, dks, dvs = q, k, v, dq, dk, dv
+        dlams = [torch.empty_like(t) for t in lams]
+        dweight = None if weight is None else torch.empty_like(weight)
+        _diff_backward(qs, ks, vs, ctx.cfg, lams, weight, mask, cu_q, cu_k, stats, maps, dout, dqs, dks, dvs, dlams, dweight, False)
+        return (dq, dk, dv, None, None, None, None, None, dweight) + tuple(dlams)
+
+
+def _diff_check(data, widths, heads, lams, lambda_init, weight, mask, cu_q, cu_k, max_q, max_k, p_drop):
+    """Arguments common to both calls; returns (dim, mask, cu_q, cu_k, max_q, max_k, lams, weight)."""
+    q, name = data[0]
+    H = q.shape[-1] // widths
+    if heads < 1 or q.shape[-1] % widths or H % (2 * heads) or H // (2 * heads) not in (32, 64):
+        raise _lib.UniterHipError("differential attention: a head is 64 or 128 columns (two maps of 32 or 64), got %d columns for %d heads" % (H, heads))
+    dim = H // (2 * heads)
+    packed = cu_q is not None or cu_k is not None
+    for t, what in data:
+        _check_dev(t, what)
+        if t.dim() != (2 if packed else 3):
+            raise _lib.UniterHipError("%s must be %s, got %s" % (what, "[rows, columns] when cu_seqlens is given" if packed else "[B, L, columns]", tuple(t.shape)))
+    lams = tuple(lams)
+    if len(lams) != 4:
+        raise _lib.UniterHipError("lambdas are four tensors: q1, k1, q2, k2")
+    for t in lams:
+        _check_dev(t, "lambda vector")
+        if tuple(t.shape) not in ((dim,), (heads, dim)) or t.shape != lams[0].shape:
+            raise _lib.UniterHipError("lambda vectors must all be [%d] or [%d, %d], got %s" % (dim, heads, dim, tuple(t.shape)))
+    if weight is not None:
+        _check_dev(weight, "norm_weight")
+        if tuple(weight.shape) != (2 * dim,):
+            raise _lib.UniterHipError("norm_weight must be [%d], got %s" % (2 * dim, tuple(weight.shape)))
+    if not 0.0 <= p_drop < 1.0:
+        raise _lib.UniterHipError("dropout probability must be in [0, 1), got %r" % (p_drop,))
+    if packed:
+        if mask is not None:
+            raise _lib.UniterHipError("packed rows take no mask_bias: only real tokens are there")
+        cu_k = cu_q if cu_k is None else cu_k
+        max_k = max_q if max_k is None else max_k
+        if cu_q is None or max_q is None or max_k is None or max_q < 0 or max_k < 0:
+            raise _lib.UniterHipError("packed rows need cu_seqlens and max_len (and those of the keys where they differ)")
+        for c in (cu_q, cu_k):
+            _check_dev(c, "cu_seqlens", torch.int32)
+            if c.dim() != 1 or c.numel() != cu_q.numel() or c.numel() < 1:
+                raise _lib.UniterHipError("cu_seqlens must be int32 [examples + 1]")
+        cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
+    elif mask is not None:
+        _check_dev(mask, "mask_bias", torch.float32)
+        if mask.dim() == 4:                        # UniterModel's extended mask [B, 1, 1, L]
+            mask = mask.reshape(mask.shape[0], mask.shape[-1])
+        if tuple(mask.shape) != (q.shape[0], data[-1][0].shape[1]):
+            raise _lib.UniterHipError("mask_bias must be [%d, %d] (or [B, 1, 1, Lk]), got %s" % (q.shape[0], data[-1][0].shape[1], tuple(mask.shape)))
+        if mask.numel() and mask.stride(1) != 1:
+            mask = mask.contiguous()
+    _same_device(q, name, (mask, "mask_bias"), (cu_q, "cu_seqlens"), (cu_k, "cu_seqlens_k"), (weight, "norm_weight"),
+                 *[(t, what) for t, what in data[1:]], *[(t, "lambda vector") for t in lams])
+    lams = tuple(t.contiguous() for t in lams)
+    weight = None if weight is None else _rows16(weight.contiguous())
+    return dim, mask, cu_q, cu_k, max_q, max_k, lams, weight
+
+
+def _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop):
+    dim, mask, cu_q, cu_k, max_q, max_k, lams, weight = checked
+    q = _rows16(q)
+    k, v = (None, None) if k is None else (_rows16(k), _rows16(v))
+    tensors = [t for t in (q, k, v, weight) + lams if t is not None]
+    keep = torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    p = float(p_drop)
+    seed, off = _next_offsets(1) if p > 0.0 else (0, 0)
+    cfg = (heads, dim, float(lambda_init), float(eps), max_q, max_k, p, seed, off)
+    return _DiffAttentionFn.apply(q, k, v, mask, cu_q, cu_k, cfg, keep, weight, *lams)
+
+
+def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=None, mask_bias=None, cu_seqlens=None, cu_seqlens_k=None,
+                           max_len=None, max_len_k=None, eps=1e-5, p_drop=0.0):
+    """Differential attention of q over k / v: per head (softmax(q1 k1^T / sqrt(d)) - lambda softmax(q2 k2^T / sqrt(d))) v, then, with
+    norm_weight, (1 - lambda_init) * norm_weight * RMS-normalised per head.
+
+    q bf16 [B, Lq, heads * 2 d], k and v [B, Lk, heads * 2 d], d = 32 or 64; any lengths, any strides with contiguous rows.
+    lambdas: (q1, k1, q2, k2), each bf16 [heads, d] or [d]: lambda = exp(q1 . k1) - exp(q2 . k2) + lambda_init.  norm_weight: bf16 [2 d].
+    mask_bias: fp32 [B, Lk], added to the scores; -inf removes a key for good, and a row without keys is zeros.
+    Packed rows: q [T, ..], k / v [Tk, ..], cu_seqlens int32 [examples + 1] on the device and max_len (a longest example's length, host
+    int); cu_seqlens_k / max_len_k where the keys' differ.  Rows of no example come back as zeros.
+    p_drop: dropout on the difference of the maps (callers pass 0 in evaluation).  Gradients flow to q, k, v, lambdas and norm_weight."""
+    checked = _diff_check([(q, "q"), (k, "k"), (v, "v")], 1, heads, lambdas, lambda_init, norm_weight, mask_bias, cu_seqlens, cu_seqlens_k,
+                          max_len, max_len_k, p_drop)
+    if k.shape != v.shape or k.shape[-1] != q.shape[-1] or (cu_seqlens is None and k.shape[0] != q.shape[0]):
+        raise _lib.UniterHipError("differential attention: q %s, k %s and v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    return _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop)
+
+
+def differential_self_attention(qkv, heads, lambdas, lambda_init, norm_weight=None, mask_bias=None, cu_seqlens=None, max_len=None,
+                                eps=1e-5, p_drop=0.0):
+    """differential_attention on a fused projection qkv [B, L, 3 H] (or packed [T, 3 H]), H = heads * 2 d: the q | k | v layout that
+    BertSelfAttention.fused_qkv produces.  Its gradient is one [.., 3 H] tensor too."""
+    checked = _diff_check([(qkv, "qkv")], 3, heads, lambdas, lambda_init, norm_weight, mask_bias, cu_seqlens, None, max_len, None, p_drop)
+    return _diff_apply(qkv, None, None, heads, checked, lambda_init, eps, p_drop)
+
+
+# ----------------------------------------------------------------------------------------------------
 # LayerNorm (+ dropout on the output) as used by the embedding blocks
 # ----------------------------------------------------------------------------------------------------
 def _ln_fwd(z, weight, bias, eps, p, seed, off):
