@@ -666,8 +666,10 @@ typedef struct UniterDiffAttentionGrads {
     void* norm_weight;
     int64_t accumulate_params;
 } UniterDiffAttentionGrads;
+/* (workspace: for calls of few queries against many keys, whose keys are split over the chip and joined; 0 bytes otherwise) */
+size_t uniter_diff_attention_fwd_workspace_bytes(const UniterDiffAttention* a);
 int uniter_diff_attention_fwd(const UniterDiffAttention* a, void* out, int64_t out_row, int64_t out_batch, float* stats, float* maps,
-                              void* stream);
+                              void* workspace, size_t workspace_bytes, void* stream);
 size_t uniter_diff_attention_bwd_workspace_bytes(const UniterDiffAttention* a);
 int uniter_diff_attention_bwd(const UniterDiffAttention* a, const float* stats, const float* maps, const void* dout, int64_t dout_row,
                               int64_t dout_batch, const UniterDiffAttentionGrads* g, void* workspace, size_t workspace_bytes, void* stream);

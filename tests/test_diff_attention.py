@@ -573,7 +573,7 @@ def test_bad_c_arguments_are_refused():
 
     def refused(text, out=4096, row=64, stats=None, maps=None, **kw):
         a = args(**kw)
-        assert lib.uniter_diff_attention_fwd(ctypes.byref(a), out, row, 0, stats, maps, None) < 0, kw
+        assert lib.uniter_diff_attention_fwd(ctypes.byref(a), out, row, 0, stats, maps, None, 0, None) < 0, kw
         assert text in lib.uniter_hip_last_error(), (kw, lib.uniter_hip_last_error())
 
     refused(b"head_dim", head_dim=48)
@@ -591,6 +591,8 @@ def test_bad_c_arguments_are_refused():
     refused(b"null", lambda_k2=None)
     refused(b"null", out=None)
     refused(b"together", stats=4096)
+    refused(b"2^24", k_row=1 << 24)
+    refused(b"workspace", Lk=100_000)
     refused(b"too many", B=1 << 20, heads=64, Lq=1 << 12)
     a, g = args(), _lib.UniterDiffAttentionGrads()
     n = lib.uniter_diff_attention_bwd_workspace_bytes(ctypes.byref(a))
@@ -602,7 +604,7 @@ def test_bad_c_arguments_are_refused():
     assert b"workspace" in lib.uniter_hip_last_error()
     g.norm_weight = 4096
     assert lib.uniter_diff_attention_bwd(ctypes.byref(a), 4096, 4096, 4096, 64, 0, ctypes.byref(g), 4096, n, None) < 0
-    assert lib.uniter_diff_attention_fwd(ctypes.byref(args(B=0)), None, 0, 0, None, None, None) == 0
+    assert lib.uniter_diff_attention_fwd(ctypes.byref(args(B=0)), None, 0, 0, None, None, None, 0, None) == 0
 
 
 def test_cpu_tensors_are_refused():

@@ -198,7 +198,8 @@ SIGNATURES = {
     "uniter_attn_pool_fwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, c_float, c_uint64, c_uint64, _P]),
     "uniter_attn_pool_bwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, c_size_t, _P]),
     "uniter_rotary": (c_int, [POINTER(UniterRotary), _P, POINTER(c_int64), _P, POINTER(c_int64), _P]),
-    "uniter_diff_attention_fwd": (c_int, [POINTER(UniterDiffAttention), _P, _I, _I, _P, _P, _P]),
+    "uniter_diff_attention_fwd": (c_int, [POINTER(UniterDiffAttention), _P, _I, _I, _P, _P, _P, c_size_t, _P]),
+    "uniter_diff_attention_fwd_workspace_bytes": (c_size_t, [POINTER(UniterDiffAttention)]),
     "uniter_diff_attention_bwd_workspace_bytes": (c_size_t, [POINTER(UniterDiffAttention)]),
     "uniter_diff_attention_bwd": (c_int, [POINTER(UniterDiffAttention), _P, _P, _P, _I, _I, POINTER(UniterDiffAttentionGrads), _P,
                                           c_size_t, _P]),

@@ -48,6 +48,7 @@ struct DiffArgs {
     int64_t lo, bo;
     float* stats;                        // [B, heads, Lq, NSTAT] or NULL
     float* maps;                         // [row, heads, 2, W]: P_1 V and P_2 V, or NULL
+    float *psum, *pacc;                  // split forward: [split, B, heads, Lq, NSTAT] max and sum, [.., 2, W] sums not yet divided
     // backward
     const bf16_t* dout;
     int64_t ldo, bdo;
@@ -139,27 +140,75 @@ __device__ __forceinline__ Span span_of(const int32_t* cu, const int64_t total, 
 // additive mask in log2 units; the type's lowest value stays finite (a row of nothing but that is uniform over its keys)
 __device__ __forceinline__ float mask_log2(const float m) { return m == -INFINITY ? m : fmaxf(m * LOG2E, -3.4028234663852886e38f); }
 
-// copy KT rows x W columns into a tile; rows from n on, and rows whose mask is -inf (keep(r) false), become zeros: whatever stands
-// there, their weight is zero and 0 * NaN must not reach a sum
-template <int W, typename Keep>
-__device__ __forceinline__ void stage(bf16_t* tile, const bf16_t* src, const int64_t ld, const int r0, const int n, Keep&& keep) {
-    for (int e = threadIdx.x; e < KT * (W / 8); e += blockDim.x) {
-        const int r = e / (W / 8), c = e % (W / 8);
-        u32x4 v = {0u, 0u, 0u, 0u};
-        if (r0 + r < n && keep(r)) v = ldg16<false>(src + (int64_t)(r0 + r) * ld + c * 8);
-        *reinterpret_cast<u32x4*>(tile + tile_off<W>(r, c)) = v;
+// ---- tiles by direct global -> LDS transfers (global_load_lds_dwordx4: a wave instruction moves 64 x 16 bytes to a contiguous 1 KiB
+// of LDS, so the swizzle is applied to the source address).  The origin of a tile is scalar, a lane's offset inside it 32 bits (the entry
+// checks the row strides).  Rows behind the end are read from the last row there is: their weight is zero, see fix_rows.
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+}
+__device__ __forceinline__ void dma16(const uint32_t voff, const char* origin, const uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"((__attribute__((address_space(1))) const char*)origin), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <int W>
+__device__ __forceinline__ void dma_tile(const bf16_t* tile, const bf16_t* src, const int64_t ld, const int r0, const int n, const int wid,
+                                         const int nw, const int lane) {
+    constexpr int RPI = 512 / W, CPR = W / 8;                  // rows per instruction, 16-byte chunks per row
+    const char* origin = reinterpret_cast<const char*>(src + (int64_t)r0 * ld);
+    const uint32_t base = lds_addr(tile), pitch = (uint32_t)(ld * 2);
+    const int last = n - 1 - r0;
+    for (int j = wid; j < KT / RPI; j += nw) {
+        const int r = RPI * j + lane / CPR;
+        const int key = W == 64 ? (((r >> 1) & 3) << 1) : ((r & 7) << 1);
+        dma16((uint32_t)min(r, last) * pitch + (uint32_t)(((lane % CPR) ^ key) * 16), origin, base + (uint32_t)j * 1024u);
     }
 }
 
-// mask of the tile's keys (log2 units, -inf behind the end).  All threads of the workgroup call; a barrier follows.
-__device__ __forceinline__ void stage_mask(float* mb, const DiffArgs& p, const int b, const int k0, const int nk) {
-    if (threadIdx.x < KT) {
-        const int key = k0 + (int)threadIdx.x;
-        float m = -INFINITY;
-        if (key < nk) m = p.mask != nullptr ? mask_log2(p.mask[(int64_t)b * p.lmask + key]) : 0.f;
-        mb[threadIdx.x] = m;
+// The key tiles of the forward and dQ kernels: K and V of KT keys, double buffered, and the keys' mask.
+template <int W>
+struct KeyTiles {
+    bf16_t* Ks;                          // [2][KT * W]
+    bf16_t* Vs;
+    float* mb;                           // [2][KT] additive mask, log2 units
+    const bf16_t *K, *V;
+    int64_t lk, lv;
+    const float* mask;                   // this example's row, or NULL
+    int n, wid, nw, lane;
+    float m;                             // mask of key `lane` of the tile on its way
+    // of the tile that is there, the same in every wave: does any key carry a mask, which keys are out (-inf, or behind the end)
+    bool general;
+    unsigned long long out;
+
+    __device__ __forceinline__ void start(const int t) {
+        const int k0 = t * KT;
+        dma_tile<W>(Ks + (t & 1) * KT * W, K, lk, k0, n, wid, nw, lane);
+        dma_tile<W>(Vs + (t & 1) * KT * W, V, lv, k0, n, wid, nw, lane);
+        m = 0.f;
+        if (mask != nullptr) m = mask[min(k0 + lane, n - 1)];
     }
-}
+    // all waves; on return tile t is complete.  Keys that are out become zeros: whatever stands there, 0 * NaN must not reach a sum.
+    __device__ __forceinline__ void finish(const int t) {
+        dma_wait();
+        asm volatile("" : "+v"(m));                            // (the mask's own wait stays behind the transfers')
+        m = t * KT + lane < n ? mask_log2(m) : -INFINITY;
+        general = __ballot(m != 0.f) != 0;
+        out = __ballot(m == -INFINITY);
+        if (general && wid == 0) mb[(t & 1) * KT + lane] = m;
+        __syncthreads();
+        if (out != 0) {
+            for (int e = wid * 64 + lane; e < KT * (W / 8); e += nw * 64) {
+                const int r = e / (W / 8), c = e % (W / 8);
+                if ((out >> r) & 1) {
+                    const int at = (t & 1) * KT * W + tile_off<W>(r, c);
+                    *reinterpret_cast<u32x4*>(Ks + at) = u32x4{0u, 0u, 0u, 0u};
+                    *reinterpret_cast<u32x4*>(Vs + at) = u32x4{0u, 0u, 0u, 0u};
+                }
+            }
+            __syncthreads();
+        }
+    }
+};
 
 // lambda of head h (every lane gets it)
 template <int D>
@@ -185,34 +234,45 @@ __device__ __forceinline__ uint32_t keep16(const DiffArgs& p, const uint64_t row
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-template <int D, bool DROP>
-__global__ __launch_bounds__(256) void diff_fwd_kernel(const DiffArgs p, const int nqb) {
+// Rescaling of the accumulators waits until a score exceeds the reference maximum by 2^LAZY: until then the weights stay below 2^LAZY,
+// whose bf16 operands are as exact as any others, and the reference need not be the maximum.
+constexpr float LAZY = 8.f;
+
+// one workgroup: `nw` waves of 32 queries each, key tiles [t0, t1) of its split.  SPLIT: writes partial sums for diff_join_kernel.
+template <int D, bool DROP, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void diff_fwd_kernel(const DiffArgs p, const int nqb, const int nsplit) {
     constexpr int W = 2 * D, NS = D / 16, NV = W / 32;
-    __shared__ __attribute__((aligned(16))) bf16_t Ks[KT * W];
-    __shared__ __attribute__((aligned(16))) bf16_t Vs[KT * W];
-    __shared__ __attribute__((aligned(16))) float mb[KT];
+    __shared__ __attribute__((aligned(16))) bf16_t Ks[2 * KT * W];
+    __shared__ __attribute__((aligned(16))) bf16_t Vs[2 * KT * W];
+    __shared__ __attribute__((aligned(16))) float mb[2 * KT];
     const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x);
-    const int bh = bid / nqb, qb = bid - bh * nqb;
+    const int unit = SPLIT ? bid / nsplit : bid, sp = SPLIT ? bid - unit * nsplit : 0;
+    const int bh = unit / nqb, qb = unit - bh * nqb;
     const int b = bh / p.heads, h = bh - b * p.heads;
     const Span sq = span_of(p.cu_q, p.tot_q, b, p.Lq), sk = span_of(p.cu_k, p.tot_k, b, p.Lk);
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), half = lane >> 5;
     const int nw = (int)blockDim.x >> 6;
     if (qb * nw * 32 >= sq.n) return;
     const int q = (qb * nw + wid) * 32 + (lane & 31);
     const bool live = q < sq.n;
-    const bf16_t* Q = p.q + (int64_t)b * p.bq * (p.cu_q == nullptr) + sq.row * p.lq + h * W;
-    const bf16_t* K = p.k + (int64_t)b * p.bk * (p.cu_k == nullptr) + sk.row * p.lk + h * W;
-    const bf16_t* V = p.v + (int64_t)b * p.bv * (p.cu_k == nullptr) + sk.row * p.lv + h * W;
+    const int nt = (sk.n + KT - 1) / KT;
+    const int t0 = SPLIT ? (int)((int64_t)nt * sp / nsplit) : 0, t1 = SPLIT ? (int)((int64_t)nt * (sp + 1) / nsplit) : nt;
 
+    KeyTiles<W> kt;
+    kt.Ks = Ks; kt.Vs = Vs; kt.mb = mb;
+    kt.K = p.k + (int64_t)b * p.bk * (p.cu_k == nullptr) + sk.row * p.lk + h * W;
+    kt.V = p.v + (int64_t)b * p.bv * (p.cu_k == nullptr) + sk.row * p.lv + h * W;
+    kt.lk = p.lk; kt.lv = p.lv;
+    kt.mask = p.mask != nullptr ? p.mask + (int64_t)b * p.lmask : nullptr;
+    kt.n = sk.n; kt.wid = wid; kt.nw = nw; kt.lane = lane;
+    if (t0 < t1) kt.start(t0);
+
+    const bf16_t* Q = p.q + (int64_t)b * p.bq * (p.cu_q == nullptr) + (sq.row + min(q, sq.n - 1)) * p.lq + h * W + half * 8;
     bf16x8 qf[2][NS];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            u32x4 v = {0u, 0u, 0u, 0u};
-            if (live) v = ldg16<false>(Q + (int64_t)q * p.lq + j * D + s * 16 + half * 8);
-            qf[j][s] = __builtin_bit_cast(bf16x8, v);
-        }
+        for (int s = 0; s < NS; ++s) qf[j][s] = __builtin_bit_cast(bf16x8, ldg16<false>(Q + j * D + s * 16));
     float e1, e2;
     lambda_of<D>(p, h, lane, e1, e2);
     const float lam = e1 - e2 + p.lambda_init;
@@ -224,69 +284,110 @@ __global__ __launch_bounds__(256) void diff_fwd_kernel(const DiffArgs p, const i
 #pragma unroll
         for (int t = 0; t < NV; ++t) o[j][t] = zero16();
     const uint64_t drow = (uint64_t)bh * (uint64_t)p.Lq + (uint64_t)q;
+    if (t0 < t1) kt.finish(t0);
 
-    for (int k0 = 0; k0 < sk.n; k0 += KT) {
-        __syncthreads();
-        stage_mask(mb, p, b, k0, sk.n);
-        __syncthreads();
-        stage<W>(Ks, K, p.lk, k0, sk.n, [&](int r) { return mb[r] != -INFINITY; });
-        stage<W>(Vs, V, p.lv, k0, sk.n, [&](int r) { return mb[r] != -INFINITY; });
-        __syncthreads();
-#pragma unroll
-        for (int kt = 0; kt < KT / 32; ++kt) {
-            uint32_t keep = 0xffffu;
-            if constexpr (DROP) keep = keep16(p, drow, k0 + kt * 32, half);
-            f32x4 mv[4];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) mv[g] = *reinterpret_cast<const f32x4*>(mb + kt * 32 + 8 * g + 4 * half);
+    for (int t = t0; t < t1; ++t) {
+        const bool general = kt.general, none = kt.out == ~0ull;
+        if (t + 1 < t1) kt.start(t + 1);
+        const bf16_t* Kt = Ks + (t & 1) * KT * W;
+        const bf16_t* Vt = Vs + (t & 1) * KT * W;
+        const int subs = none ? 0 : min(2, (sk.n - t * KT + 31) >> 5);
+        for (int u = 0; u < subs; ++u) {
+            f32x16 s[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                f32x16 s = zero16();
+                s[j] = zero16();
 #pragma unroll
                 for (int ks = 0; ks < NS; ++ks)
-                    s = mfma32(row_frag<W>(Ks, kt * 32 + (lane & 31), (j * D + ks * 16) / 8 + half), qf[j][ks], s);
-                float mx = -INFINITY;
+                    s[j] = mfma32(row_frag<W>(Kt, u * 32 + (lane & 31), (j * D + ks * 16) / 8 + half), qf[j][ks], s[j]);
+            }
+            float se = p.sc;                                   // scores are s * se in log2 units
+            if (general) {
+                se = 1.f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[r] = __builtin_fmaf(s[r], p.sc, mv[r >> 2][r & 3]);
-                    mx = fmaxf(mx, s[r]);
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 mv = *reinterpret_cast<const f32x4*>(mb + (t & 1) * KT + u * 32 + 8 * g + 4 * half);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[j][4 * g + e] = __builtin_fmaf(s[j][4 * g + e], p.sc, mv[e]);
                 }
-                mx = fmaxf(mx, other_half(mx));
-                const float mn = fmaxf(m[j], mx);
-                const float ms = mn == -INFINITY ? 0.f : mn;                  // (a row that has met no key yet)
-                const float alpha = __builtin_amdgcn_exp2f(m[j] - ms);
-                m[j] = mn;
+            }
+            float mx[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                mx[j] = fmaxf(s[j][0], s[j][1]);
+#pragma unroll
+                for (int r = 2; r < 16; r += 2) mx[j] = fmaxf(fmaxf(mx[j], s[j][r]), s[j][r + 1]);
+                mx[j] *= se;
+            }
+            if (__any(mx[0] > m[0] + LAZY || mx[1] > m[1] + LAZY)) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float mn = fmaxf(m[j], fmaxf(mx[j], other_half(mx[j])));
+                    const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[j] - mn);
+                    m[j] = mn;
+                    l[j] *= alpha;
+#pragma unroll
+                    for (int t2 = 0; t2 < NV; ++t2) o[j][t2] *= alpha;
+                }
+            }
+            uint32_t keep = 0xffffu;
+            if constexpr (DROP) keep = keep16(p, drow, t * KT + u * 32, half);
+            bf16x8 pf[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float ms = m[j] == -INFINITY ? 0.f : m[j];               // (a row that has met no key yet)
                 float sum = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[r] = __builtin_amdgcn_exp2f(s[r] - ms);
-                    sum += s[r];
-                    if constexpr (DROP) s[r] = (keep >> r) & 1u ? s[r] : 0.f;
+                    s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], se, -ms));
+                    sum += s[j][r];
+                    if constexpr (DROP) s[j][r] = (keep >> r) & 1u ? s[j][r] : 0.f;
                 }
-                l[j] = l[j] * alpha + sum;
-#pragma unroll
-                for (int t = 0; t < NV; ++t) {
-                    o[j][t] *= alpha;
-#pragma unroll
-                    for (int kk = 0; kk < 2; ++kk)
-                        o[j][t] = mfma32(tr_frag<W>(Vs, kt * 32 + kk * 16, t * 32, lane), pack_step(s, kk), o[j][t]);
-                }
+                l[j] += sum;
+                pf[j][0] = pack_step(s[j], 0);
+                pf[j][1] = pack_step(s[j], 1);
             }
+#pragma unroll
+            for (int t2 = 0; t2 < NV; ++t2)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    const bf16x8 vf = tr_frag<W>(Vt, u * 32 + kk * 16, t2 * 32, lane);
+                    o[0][t2] = mfma32(vf, pf[0][kk], o[0][t2]);
+                    o[1][t2] = mfma32(vf, pf[1][kk], o[1][t2]);
+                }
         }
+        if (t + 1 < t1) kt.finish(t + 1);
     }
-    const float dscale = DROP ? p.drop.scale : 1.f;
-    float inv[2], ll[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         l[j] += other_half(l[j]);
-        inv[j] = l[j] > 0.f ? dscale / l[j] : (l[j] == 0.f ? 0.f : l[j]);
-        ll[j] = l[j] == 0.f ? INFINITY : __log2f(l[j]);
+        m[j] = m[j] == -INFINITY ? 0.f : m[j];
     }
+    const float dscale = DROP ? p.drop.scale : 1.f;
+    if constexpr (SPLIT) {
+        if (!live) return;
+        const int64_t at = ((int64_t)sp * p.B * p.heads + bh) * p.Lq + q;
+        if (half == 0) *reinterpret_cast<f32x4*>(p.psum + at * NSTAT) = f32x4{m[0], l[0], m[1], l[1]};
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int t = 0; t < NV; ++t) {
+                o[j][t] *= dscale;
+                float* dst = p.pacc + (at * 2 + j) * W + t * 32 + 4 * half;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4*>(dst + 8 * g) = f32x4{o[j][t][4 * g], o[j][t][4 * g + 1], o[j][t][4 * g + 2], o[j][t][4 * g + 3]};
+            }
+        return;
+    }
+    float inv[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) inv[j] = l[j] > 0.f ? dscale / l[j] : l[j];    // (0 without keys; a NaN stays one)
+    if (p.stats != nullptr && live && half == 0)
+        *reinterpret_cast<f32x4*>(p.stats + ((int64_t)bh * p.Lq + q) * NSTAT) =
+            f32x4{m[0], l[0] == 0.f ? INFINITY : __log2f(l[0]), m[1], l[1] == 0.f ? INFINITY : __log2f(l[1])};
     const int64_t row = p.cu_q != nullptr ? sq.row + q : (int64_t)b * p.Lq + q;
-    if (p.stats != nullptr && live && half == 0) {
-        const f32x4 st = {m[0] == -INFINITY ? 0.f : m[0], ll[0], m[1] == -INFINITY ? 0.f : m[1], ll[1]};
-        *reinterpret_cast<f32x4*>(p.stats + ((int64_t)bh * p.Lq + q) * NSTAT) = st;
-    }
     float ss = 0.f;
 #pragma unroll
     for (int t = 0; t < NV; ++t) {
@@ -311,11 +412,100 @@ __global__ __launch_bounds__(256) void diff_fwd_kernel(const DiffArgs p, const i
 #pragma unroll
         for (int t = 0; t < NV; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[0][t][r] *= rs * bf2f(p.w[t * 32 + acc_row(r) + 4 * half]);
+            for (int g = 0; g < 4; ++g) {
+                float w4[4];
+                unpack4(ldg8<false>(p.w + t * 32 + 8 * g + 4 * half), w4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[0][t][4 * g + e] *= rs * w4[e];
+            }
     }
     bf16_t* out = p.out + (int64_t)b * p.bo * (p.cu_q == nullptr) + (sq.row + q) * p.lo + h * W;
 #pragma unroll
     for (int t = 0; t < NV; ++t) store_block32(out + t * 32, o[0][t], half, live);
+}
+
+// Joins the splits of a row: one wave per (example, head, query), W / 8 lanes of 8 columns, the other lanes take other splits.
+template <int D>
+__global__ __launch_bounds__(256) void diff_join_kernel(const DiffArgs p, const int nsplit) {
+    constexpr int W = 2 * D, LN = W / 8, NG = 64 / LN;
+    const int lane = threadIdx.x & 63, c = (lane % LN) * 8, gi = lane / LN;
+    const int64_t rows = (int64_t)p.B * p.heads * p.Lq;
+    const int64_t r = (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    if (r >= rows) return;
+    const int64_t bh = r / p.Lq;
+    const int q = (int)(r - bh * p.Lq), b = (int)(bh / p.heads), h = (int)(bh - (int64_t)b * p.heads);
+    const Span sq = span_of(p.cu_q, p.tot_q, b, p.Lq);
+    if (q >= sq.n) return;
+    float e1, e2;
+    lambda_of<D>(p, h, lane, e1, e2);
+    const float lam = e1 - e2 + p.lambda_init;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[2][8];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[j][e] = 0.f;
+    for (int s = gi; s < nsplit; s += NG) {
+        const int64_t at = s * rows + r;
+        const f32x4 st = *reinterpret_cast<const f32x4*>(p.psum + at * NSTAT);
+        f32x4 a[2][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            a[j][0] = *reinterpret_cast<const f32x4*>(p.pacc + (at * 2 + j) * W + c);
+            a[j][1] = *reinterpret_cast<const f32x4*>(p.pacc + (at * 2 + j) * W + c + 4);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float ls = st[2 * j + 1];
+            const float mn = ls == 0.f ? m[j] : fmaxf(m[j], st[2 * j]);        // (a split without keys says nothing)
+            const float f0 = m[j] == mn ? 1.f : __builtin_amdgcn_exp2f(m[j] - mn), f1 = ls == 0.f ? 0.f : __builtin_amdgcn_exp2f(st[2 * j] - mn);
+            m[j] = mn;
+            l[j] = l[j] * f0 + ls * f1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[j][e] = o[j][e] * f0 + a[j][e >> 2][e & 3] * f1;
+        }
+    }
+#pragma unroll
+    for (int x = LN; x < 64; x <<= 1)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float m2 = __shfl_xor(m[j], x, WAVE), l2 = __shfl_xor(l[j], x, WAVE), mn = fmaxf(m[j], m2);
+            const float f0 = m[j] == mn ? 1.f : __builtin_amdgcn_exp2f(m[j] - mn), f1 = m2 == mn ? 1.f : __builtin_amdgcn_exp2f(m2 - mn);
+            m[j] = mn;
+            l[j] = l[j] * f0 + l2 * f1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[j][e] = o[j][e] * f0 + __shfl_xor(o[j][e], x, WAVE) * f1;
+        }
+    const int64_t row = p.cu_q != nullptr ? sq.row + q : (int64_t)b * p.Lq + q;
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        m[j] = m[j] == -INFINITY ? 0.f : m[j];
+        const float inv = l[j] > 0.f ? 1.f / l[j] : l[j];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[j][e] *= inv;
+        if (p.maps != nullptr && gi == 0) {
+            float* at = p.maps + ((row * p.heads + h) * 2 + j) * W + c;
+            *reinterpret_cast<f32x4*>(at) = f32x4{o[j][0], o[j][1], o[j][2], o[j][3]};
+            *reinterpret_cast<f32x4*>(at + 4) = f32x4{o[j][4], o[j][5], o[j][6], o[j][7]};
+        }
+    }
+    if (p.stats != nullptr && lane == 0)
+        *reinterpret_cast<f32x4*>(p.stats + r * NSTAT) = f32x4{m[0], l[0] == 0.f ? INFINITY : __log2f(l[0]), m[1], l[1] == 0.f ? INFINITY : __log2f(l[1])};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        o[0][e] -= lam * o[1][e];
+        ss += o[0][e] * o[0][e];
+    }
+    if (p.w != nullptr) {
+#pragma unroll
+        for (int x = 1; x < LN; x <<= 1) ss += __shfl_xor(ss, x, WAVE);
+        const float rs = rsqrtf(ss * (1.f / W) + p.eps) * (1.f - p.lambda_init);
+        float w8[8];
+        unpack8(ldg16<false>(p.w + c), w8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[0][e] *= rs * w8[e];
+    }
+    if (gi == 0) out_store16(p.out + (int64_t)b * p.bo * (p.cu_q == nullptr) + (sq.row + q) * p.lo + h * W + c, pack8(o[0]));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -459,46 +649,44 @@ __global__ __launch_bounds__(256) void diff_bwd_params_kernel(const DiffArgs p, 
 // backward, queries: dQ_j = sum_k dS_j K_j,  dS_1 = P_1 (G - D_1) / sqrt(d),  dS_2 = -lambda P_2 (G - D_2) / sqrt(d),  G = dropout(dO V^T)
 // ------------------------------------------------------------------------------------------------
 template <int D, bool DROP>
-__global__ __launch_bounds__(256) void diff_bwd_dq_kernel(const DiffArgs p, const int nqb) {
+__global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(const DiffArgs p, const int nqb) {
     constexpr int W = 2 * D, NS = D / 16, ND = D / 32;
-    __shared__ __attribute__((aligned(16))) bf16_t Ks[KT * W];
-    __shared__ __attribute__((aligned(16))) bf16_t Vs[KT * W];
-    __shared__ __attribute__((aligned(16))) float mb[KT];
+    __shared__ __attribute__((aligned(16))) bf16_t Ks[2 * KT * W];
+    __shared__ __attribute__((aligned(16))) bf16_t Vs[2 * KT * W];
+    __shared__ __attribute__((aligned(16))) float mb[2 * KT];
     const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x);
     const int bh = bid / nqb, qb = bid - bh * nqb;
     const int b = bh / p.heads, h = bh - b * p.heads;
     const Span sq = span_of(p.cu_q, p.tot_q, b, p.Lq), sk = span_of(p.cu_k, p.tot_k, b, p.Lk);
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), half = lane >> 5;
     const int nw = (int)blockDim.x >> 6;
     if (qb * nw * 32 >= sq.n) return;
     const int q = (qb * nw + wid) * 32 + (lane & 31);
     const bool live = q < sq.n;
-    const bf16_t* Q = p.q + (int64_t)b * p.bq * (p.cu_q == nullptr) + sq.row * p.lq + h * W;
-    const bf16_t* K = p.k + (int64_t)b * p.bk * (p.cu_k == nullptr) + sk.row * p.lk + h * W;
-    const bf16_t* V = p.v + (int64_t)b * p.bv * (p.cu_k == nullptr) + sk.row * p.lv + h * W;
-    const bool own = p.dctx != nullptr;
-    const bf16_t* dO = own ? p.dctx + ((p.cu_q != nullptr ? sq.row : (int64_t)b * p.Lq) * p.heads + h) * W
-                           : p.dout + (int64_t)b * p.bdo * (p.cu_q == nullptr) + sq.row * p.ldo + h * W;
-    const int64_t ldO = own ? (int64_t)p.heads * W : p.ldo;
+    const int qs = min(q, sq.n - 1);
+    const int nt = (sk.n + KT - 1) / KT;
 
+    KeyTiles<W> kt;
+    kt.Ks = Ks; kt.Vs = Vs; kt.mb = mb;
+    kt.K = p.k + (int64_t)b * p.bk * (p.cu_k == nullptr) + sk.row * p.lk + h * W;
+    kt.V = p.v + (int64_t)b * p.bv * (p.cu_k == nullptr) + sk.row * p.lv + h * W;
+    kt.lk = p.lk; kt.lv = p.lv;
+    kt.mask = p.mask != nullptr ? p.mask + (int64_t)b * p.lmask : nullptr;
+    kt.n = sk.n; kt.wid = wid; kt.nw = nw; kt.lane = lane;
+    if (nt > 0) kt.start(0);
+
+    const bf16_t* Q = p.q + (int64_t)b * p.bq * (p.cu_q == nullptr) + (sq.row + qs) * p.lq + h * W + half * 8;
+    const bf16_t* dO = p.dctx != nullptr ? p.dctx + (((p.cu_q != nullptr ? sq.row : (int64_t)b * p.Lq) + qs) * p.heads + h) * W
+                                         : p.dout + (int64_t)b * p.bdo * (p.cu_q == nullptr) + (sq.row + qs) * p.ldo + h * W;
     bf16x8 qf[2][NS], gf[W / 16];
 #pragma unroll
     for (int s = 0; s < W / 16; ++s) {
-        u32x4 v = {0u, 0u, 0u, 0u}, d = {0u, 0u, 0u, 0u};
-        if (live) {
-            v = ldg16<false>(Q + (int64_t)q * p.lq + s * 16 + half * 8);
-            d = ldg16<false>(dO + (int64_t)q * ldO + s * 16 + half * 8);
-        }
-        qf[s / NS][s % NS] = __builtin_bit_cast(bf16x8, v);
-        gf[s] = __builtin_bit_cast(bf16x8, d);
+        qf[s / NS][s % NS] = __builtin_bit_cast(bf16x8, ldg16<false>(Q + s * 16));
+        gf[s] = __builtin_bit_cast(bf16x8, ldg16<false>(dO + s * 16 + half * 8));
     }
-    float m[2] = {0.f, 0.f}, ll[2] = {INFINITY, INFINITY}, Dq[2] = {0.f, 0.f};
-    if (live) {
-        const f32x4 st = *reinterpret_cast<const f32x4*>(p.stats + ((int64_t)bh * p.Lq + q) * NSTAT);
-        m[0] = st[0]; ll[0] = st[1]; m[1] = st[2]; ll[1] = st[3];
-        Dq[0] = p.D[((int64_t)bh * p.Lq + q) * 2];
-        Dq[1] = p.D[((int64_t)bh * p.Lq + q) * 2 + 1];
-    }
+    const f32x4 st = *reinterpret_cast<const f32x4*>(p.stats + ((int64_t)bh * p.Lq + qs) * NSTAT);
+    const float m[2] = {st[0], st[2]}, ll[2] = {st[1], st[3]};
+    const float Dq[2] = {p.D[((int64_t)bh * p.Lq + qs) * 2], p.D[((int64_t)bh * p.Lq + qs) * 2 + 1]};
     float e1, e2;
     lambda_of<D>(p, h, lane, e1, e2);
     const float lam = e1 - e2 + p.lambda_init;
@@ -510,45 +698,62 @@ __global__ __launch_bounds__(256) void diff_bwd_dq_kernel(const DiffArgs p, cons
     for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int t = 0; t < ND; ++t) dq[j][t] = zero16();
+    if (nt > 0) kt.finish(0);
 
-    for (int k0 = 0; k0 < sk.n; k0 += KT) {
-        __syncthreads();
-        stage_mask(mb, p, b, k0, sk.n);
-        __syncthreads();
-        stage<W>(Ks, K, p.lk, k0, sk.n, [&](int r) { return mb[r] != -INFINITY; });
-        stage<W>(Vs, V, p.lv, k0, sk.n, [&](int r) { return mb[r] != -INFINITY; });
-        __syncthreads();
+    for (int t = 0; t < nt; ++t) {
+        const bool general = kt.general, none = kt.out == ~0ull;
+        if (t + 1 < nt) kt.start(t + 1);
+        const bf16_t* Kt = Ks + (t & 1) * KT * W;
+        const bf16_t* Vt = Vs + (t & 1) * KT * W;
+        const int subs = none ? 0 : min(2, (sk.n - t * KT + 31) >> 5);
+        for (int u = 0; u < subs; ++u) {
+            f32x16 g = zero16(), s[2];
 #pragma unroll
-        for (int kt = 0; kt < KT / 32; ++kt) {
-            f32x16 g = zero16();
+            for (int j = 0; j < 2; ++j) {
+                s[j] = zero16();
 #pragma unroll
-            for (int s = 0; s < W / 16; ++s) g = mfma32(row_frag<W>(Vs, kt * 32 + (lane & 31), 2 * s + half), gf[s], g);
+                for (int ks = 0; ks < NS; ++ks)
+                    s[j] = mfma32(row_frag<W>(Kt, u * 32 + (lane & 31), (j * D + ks * 16) / 8 + half), qf[j][ks], s[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < W / 16; ++i) g = mfma32(row_frag<W>(Vt, u * 32 + (lane & 31), 2 * i + half), gf[i], g);
+            // weights 2^(s se - c): with a mask the maximum is taken off the masked score first, as in the forward pass
+            float se = p.sc, c[2] = {m[0] + ll[0], m[1] + ll[1]};
+            if (general) {
+                se = 1.f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) c[j] = ll[j];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 mv = *reinterpret_cast<const f32x4*>(mb + (t & 1) * KT + u * 32 + 8 * i + 4 * half);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[j][4 * i + e] = __builtin_fmaf(s[j][4 * i + e], p.sc, mv[e]) - m[j];
+                }
+            }
             if constexpr (DROP) {
-                const uint32_t keep = keep16(p, drow, k0 + kt * 32, half);
+                const uint32_t keep = keep16(p, drow, t * KT + u * 32, half);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) g[r] = (keep >> r) & 1u ? g[r] * dscale : 0.f;
             }
-            f32x4 mv[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mv[i] = *reinterpret_cast<const f32x4*>(mb + kt * 32 + 8 * i + 4 * half);
+            bf16x8 df[2][2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                f32x16 s = zero16();
 #pragma unroll
-                for (int ks = 0; ks < NS; ++ks)
-                    s = mfma32(row_frag<W>(Ks, kt * 32 + (lane & 31), (j * D + ks * 16) / 8 + half), qf[j][ks], s);
+                for (int r = 0; r < 16; ++r) s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], se, -c[j])) * (g[r] - Dq[j]);
+                df[j][0] = pack_step(s[j], 0);
+                df[j][1] = pack_step(s[j], 1);
+            }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float pr = __builtin_amdgcn_exp2f((__builtin_fmaf(s[r], p.sc, mv[r >> 2][r & 3]) - m[j]) - ll[j]);
-                    s[r] = pr * (g[r] - Dq[j]);
-                }
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int t = 0; t < ND; ++t)
+                for (int t2 = 0; t2 < ND; ++t2)
 #pragma unroll
                     for (int kk = 0; kk < 2; ++kk)
-                        dq[j][t] = mfma32(tr_frag<W>(Ks, kt * 32 + kk * 16, j * D + t * 32, lane), pack_step(s, kk), dq[j][t]);
-            }
+                        dq[j][t2] = mfma32(tr_frag<W>(Kt, u * 32 + kk * 16, j * D + t2 * 32, lane), df[j][kk], dq[j][t2]);
         }
+        if (t + 1 < nt) kt.finish(t + 1);
     }
     const float z = p.sc * (1.f / LOG2E);
     bf16_t* dst = p.dq + (int64_t)b * p.bdq * (p.cu_q == nullptr) + (sq.row + q) * p.ldq + h * W;
@@ -564,42 +769,72 @@ __global__ __launch_bounds__(256) void diff_bwd_dq_kernel(const DiffArgs p, cons
 // ------------------------------------------------------------------------------------------------
 // backward, keys: dV = sum_q A dO with A = dropout(P_1 - lambda P_2);  dK_j = sum_q dS_j Q_j
 // ------------------------------------------------------------------------------------------------
+// per query of a tile: max and log2(sum) of both maps, their sums, and D of both maps
+enum { ST_M = 0, ST_LL = 2, ST_LSE = 4, ST_D = 6, ST_N = 8 };
+
 template <int D, bool DROP>
-__global__ __launch_bounds__(256) void diff_bwd_dkv_kernel(const DiffArgs p, const int nkb) {
+__global__ __launch_bounds__(256, D == 32 ? 2 : 1) void diff_bwd_dkv_kernel(const DiffArgs p, const int nkb) {
     constexpr int W = 2 * D, NS = D / 16, ND = D / 32, NV = W / 32;
-    __shared__ __attribute__((aligned(16))) bf16_t Qs[KT * W];
-    __shared__ __attribute__((aligned(16))) bf16_t Os[KT * W];
-    __shared__ __attribute__((aligned(16))) float st[6][KT];      // m1, log2 l1, m2, log2 l2, D1, D2
+    __shared__ __attribute__((aligned(16))) bf16_t Qs[2 * KT * W];
+    __shared__ __attribute__((aligned(16))) bf16_t Os[2 * KT * W];
+    __shared__ __attribute__((aligned(16))) float st[2][ST_N][KT];
     const int bid = xcd_remap((int)blockIdx.x, (int)gridDim.x);
     const int bh = bid / nkb, kb = bid - bh * nkb;
     const int b = bh / p.heads, h = bh - b * p.heads;
     const Span sq = span_of(p.cu_q, p.tot_q, b, p.Lq), sk = span_of(p.cu_k, p.tot_k, b, p.Lk);
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), half = lane >> 5;
     const int nw = (int)blockDim.x >> 6;
     if (kb * nw * 32 >= sk.n) return;
     const int kbase = (kb * nw + wid) * 32, key = kbase + (lane & 31);
     const bool live = key < sk.n;
+    const int nt = (sq.n + KT - 1) / KT;
     const bf16_t* Q = p.q + (int64_t)b * p.bq * (p.cu_q == nullptr) + sq.row * p.lq + h * W;
-    const bf16_t* K = p.k + (int64_t)b * p.bk * (p.cu_k == nullptr) + sk.row * p.lk + h * W;
-    const bf16_t* V = p.v + (int64_t)b * p.bv * (p.cu_k == nullptr) + sk.row * p.lv + h * W;
-    const bool own = p.dctx != nullptr;
-    const bf16_t* dO = own ? p.dctx + ((p.cu_q != nullptr ? sq.row : (int64_t)b * p.Lq) * p.heads + h) * W
-                           : p.dout + (int64_t)b * p.bdo * (p.cu_q == nullptr) + sq.row * p.ldo + h * W;
-    const int64_t ldO = own ? (int64_t)p.heads * W : p.ldo;
+    const bf16_t* dO = p.dctx != nullptr ? p.dctx + ((p.cu_q != nullptr ? sq.row : (int64_t)b * p.Lq) * p.heads + h) * W
+                                         : p.dout + (int64_t)b * p.bdo * (p.cu_q == nullptr) + sq.row * p.ldo + h * W;
+    const int64_t ldO = p.dctx != nullptr ? (int64_t)p.heads * W : p.ldo;
+    f32x4 s4;
+    float d0, d1;
+    auto start = [&](const int t) {
+        dma_tile<W>(Qs + (t & 1) * KT * W, Q, p.lq, t * KT, sq.n, wid, nw, lane);
+        dma_tile<W>(Os + (t & 1) * KT * W, dO, ldO, t * KT, sq.n, wid, nw, lane);
+        if (wid == 0) {
+            const int64_t at = (int64_t)bh * p.Lq + min(t * KT + lane, sq.n - 1);
+            s4 = *reinterpret_cast<const f32x4*>(p.stats + at * NSTAT);
+            d0 = p.D[at * 2];
+            d1 = p.D[at * 2 + 1];
+        }
+    };
+    auto finish = [&](const int t) {
+        dma_wait();
+        if (wid == 0) {
+            asm volatile("" : "+v"(s4), "+v"(d0), "+v"(d1));
+            const bool in = t * KT + lane < sq.n;                              // behind the last query: P = 0
+            float(*w)[KT] = st[t & 1];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                w[ST_M + j][lane] = s4[2 * j];
+                w[ST_LL + j][lane] = in ? s4[2 * j + 1] : INFINITY;
+                w[ST_LSE + j][lane] = in ? s4[2 * j] + s4[2 * j + 1] : INFINITY;
+            }
+            w[ST_D][lane] = d0;
+            w[ST_D + 1][lane] = d1;
+        }
+        __syncthreads();
+    };
+    if (nt > 0) start(0);
 
+    // keys that are out for good (-inf) and lanes behind the end: zeros and P = 0, whatever stands there
     float mk = -INFINITY;
     if (live) mk = p.mask != nullptr ? mask_log2(p.mask[(int64_t)b * p.lmask + key]) : 0.f;
-    const bool use = mk != -INFINITY;
+    const bool use = mk != -INFINITY, general = __any(mk != 0.f);
+    const bf16_t* K = p.k + (int64_t)b * p.bk * (p.cu_k == nullptr) + (sk.row + min(key, sk.n - 1)) * p.lk + h * W + half * 8;
+    const bf16_t* V = p.v + (int64_t)b * p.bv * (p.cu_k == nullptr) + (sk.row + min(key, sk.n - 1)) * p.lv + h * W + half * 8;
     bf16x8 kf[2][NS], vf[W / 16];
 #pragma unroll
     for (int s = 0; s < W / 16; ++s) {
-        u32x4 a = {0u, 0u, 0u, 0u}, c = {0u, 0u, 0u, 0u};
-        if (use) {
-            a = ldg16<false>(K + (int64_t)key * p.lk + s * 16 + half * 8);
-            c = ldg16<false>(V + (int64_t)key * p.lv + s * 16 + half * 8);
-        }
-        kf[s / NS][s % NS] = __builtin_bit_cast(bf16x8, a);
-        vf[s] = __builtin_bit_cast(bf16x8, c);
+        const u32x4 a = ldg16<false>(K + s * 16), c = ldg16<false>(V + s * 16), none = {0u, 0u, 0u, 0u};
+        kf[s / NS][s % NS] = __builtin_bit_cast(bf16x8, use ? a : none);
+        vf[s] = __builtin_bit_cast(bf16x8, use ? c : none);
     }
     float e1, e2;
     lambda_of<D>(p, h, lane, e1, e2);
@@ -613,69 +848,68 @@ __global__ __launch_bounds__(256) void diff_bwd_dkv_kernel(const DiffArgs p, con
     for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int t = 0; t < ND; ++t) dk[j][t] = zero16();
+    if (nt > 0) finish(0);
 
-    for (int q0 = 0; q0 < sq.n; q0 += KT) {
-        __syncthreads();
-        stage<W>(Qs, Q, p.lq, q0, sq.n, [](int) { return true; });
-        stage<W>(Os, dO, ldO, q0, sq.n, [](int) { return true; });
-        if (threadIdx.x < KT) {
-            const int t = (int)threadIdx.x, q = q0 + t;
-            float v[6] = {0.f, INFINITY, 0.f, INFINITY, 0.f, 0.f};           // behind the last query: P = 0
-            if (q < sq.n) {
-                const f32x4 s4 = *reinterpret_cast<const f32x4*>(p.stats + ((int64_t)bh * p.Lq + q) * NSTAT);
-                v[0] = s4[0]; v[1] = s4[1]; v[2] = s4[2]; v[3] = s4[3];
-                v[4] = p.D[((int64_t)bh * p.Lq + q) * 2];
-                v[5] = p.D[((int64_t)bh * p.Lq + q) * 2 + 1];
+    for (int t = 0; t < nt; ++t) {
+        if (t + 1 < nt) start(t + 1);
+        const bf16_t* Qt = Qs + (t & 1) * KT * W;
+        const bf16_t* Ot = Os + (t & 1) * KT * W;
+        const int subs = min(2, (sq.n - t * KT + 31) >> 5);
+        for (int u = 0; u < subs; ++u) {
+            const float* w = &st[t & 1][0][u * 32 + 4 * half];
+            f32x16 g = zero16(), s[2], a;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                s[j] = zero16();
+#pragma unroll
+                for (int ks = 0; ks < NS; ++ks)
+                    s[j] = mfma32(row_frag<W>(Qt, u * 32 + (lane & 31), (j * D + ks * 16) / 8 + half), kf[j][ks], s[j]);
             }
 #pragma unroll
-            for (int i = 0; i < 6; ++i) st[i][t] = v[i];
-        }
-        __syncthreads();
+            for (int i = 0; i < W / 16; ++i) g = mfma32(row_frag<W>(Ot, u * 32 + (lane & 31), 2 * i + half), vf[i], g);
+            float se = p.sc;
+            const float* cs = w + ST_LSE * KT;
+            if (general) {
+                se = 1.f;
+                cs = w + ST_LL * KT;
 #pragma unroll
-        for (int qt = 0; qt < KT / 32; ++qt) {
-            uint32_t keep = 0xffffu;
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 m4 = *reinterpret_cast<const f32x4*>(w + (ST_M + j) * KT + 8 * i);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[j][4 * i + e] = __builtin_fmaf(s[j][4 * i + e], p.sc, mk) - m4[e];
+                    }
+            }
+            uint32_t keep = ~0u;
             if constexpr (DROP) {
-                // the bits come out with a query per lane; the ballot of register r is key acc_row(r) + 4 (lane half) over the queries
-                const uint64_t drow = (uint64_t)bh * (uint64_t)p.Lq + (uint64_t)(q0 + qt * 32 + (lane & 31));
+                // the draws come with a query per lane; the ballot of bit r holds, for either half of the wave, one key over the queries
+                const uint64_t drow = (uint64_t)bh * (uint64_t)p.Lq + (uint64_t)(t * KT + u * 32 + (lane & 31));
                 const uint32_t mine = keep16(p, drow, kbase, half);
                 const int kl = lane & 31, reg = 4 * (kl >> 3) + (kl & 3), kh = (kl >> 2) & 1;
-                uint32_t word = 0;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const unsigned long long bal = __ballot((mine >> r) & 1u);
                     const uint32_t part = kh ? (uint32_t)(bal >> 32) : (uint32_t)bal;
-                    word = reg == r ? part : word;
+                    keep = reg == r ? part : keep;                             // bit: query of this block
                 }
-                keep = word;                                                  // bit: query of this 32-row block
+#pragma unroll
+                for (int r = 0; r < 16; ++r) g[r] = (keep >> (acc_row(r) + 4 * half)) & 1u ? g[r] * dscale : 0.f;
             }
-            f32x16 g = zero16();
 #pragma unroll
-            for (int s = 0; s < W / 16; ++s) g = mfma32(row_frag<W>(Os, qt * 32 + (lane & 31), 2 * s + half), vf[s], g);
-            f32x16 a;
-            f32x16 ds[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                f32x16 s = zero16();
-#pragma unroll
-                for (int ks = 0; ks < NS; ++ks)
-                    s = mfma32(row_frag<W>(Qs, qt * 32 + (lane & 31), (j * D + ks * 16) / 8 + half), kf[j][ks], s);
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int at = qt * 32 + 8 * i + 4 * half;
-                    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&st[2 * j][at]);
-                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(&st[2 * j + 1][at]);
-                    const f32x4 D4 = *reinterpret_cast<const f32x4*>(&st[4 + j][at]);
+                    const f32x4 c4 = *reinterpret_cast<const f32x4*>(cs + j * KT + 8 * i);
+                    const f32x4 D4 = *reinterpret_cast<const f32x4*>(w + (ST_D + j) * KT + 8 * i);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = 4 * i + e;
-                        const float pr = __builtin_amdgcn_exp2f((__builtin_fmaf(s[r], p.sc, mk) - m4[e]) - l4[e]);
-                        float gr = g[r];
-                        if constexpr (DROP) gr = (keep >> (acc_row(r) + 4 * half)) & 1u ? gr * dscale : 0.f;
-                        ds[j][r] = pr * (gr - D4[e]);
-                        a[r] = j == 0 ? pr : a[r] - lam * pr;
+                        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], se, -c4[e]));
+                        a[r] = j == 0 ? pr : __builtin_fmaf(-lam, pr, a[r]);
+                        s[j][r] = pr * (g[r] - D4[e]);
                     }
                 }
-            }
             if constexpr (DROP) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) a[r] = (keep >> (acc_row(r) + 4 * half)) & 1u ? a[r] * dscale : 0.f;
@@ -684,15 +918,16 @@ __global__ __launch_bounds__(256) void diff_bwd_dkv_kernel(const DiffArgs p, con
             for (int kk = 0; kk < 2; ++kk) {
                 const bf16x8 af = pack_step(a, kk);
 #pragma unroll
-                for (int t = 0; t < NV; ++t) dv[t] = mfma32(tr_frag<W>(Os, qt * 32 + kk * 16, t * 32, lane), af, dv[t]);
+                for (int t2 = 0; t2 < NV; ++t2) dv[t2] = mfma32(tr_frag<W>(Ot, u * 32 + kk * 16, t2 * 32, lane), af, dv[t2]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const bf16x8 df = pack_step(ds[j], kk);
+                    const bf16x8 df = pack_step(s[j], kk);
 #pragma unroll
-                    for (int t = 0; t < ND; ++t) dk[j][t] = mfma32(tr_frag<W>(Qs, qt * 32 + kk * 16, j * D + t * 32, lane), df, dk[j][t]);
+                    for (int t2 = 0; t2 < ND; ++t2) dk[j][t2] = mfma32(tr_frag<W>(Qt, u * 32 + kk * 16, j * D + t2 * 32, lane), df, dk[j][t2]);
                 }
             }
         }
+        if (t + 1 < nt) finish(t + 1);
     }
     const float z = p.sc * (1.f / LOG2E);
     bf16_t* dkp = p.dk + (int64_t)b * p.bdk * (p.cu_k == nullptr) + (sk.row + key) * p.ldk + h * W;
@@ -724,6 +959,8 @@ int check(const UniterDiffAttention* a) {
     UH_CHECK_ARG(a->p_drop >= 0.f && a->p_drop < 1.f, "dropout probability must be in [0,1)");
     UH_CHECK_ARG(a->q_row % 8 == 0 && a->k_row % 8 == 0 && a->v_row % 8 == 0 && a->q_batch % 8 == 0 && a->k_batch % 8 == 0 && a->v_batch % 8 == 0,
                  "row and batch strides must be multiples of 8 elements");
+    UH_CHECK_ARG(a->q_row >= 0 && a->k_row >= 0 && a->v_row >= 0 && a->q_row < (1 << 24) && a->k_row < (1 << 24) && a->v_row < (1 << 24),
+                 "row strides must be 0 .. 2^24 elements");
     UH_CHECK_ARG(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->norm_weight), "q, k, v and norm_weight must be 16-byte aligned");
     UH_CHECK_ARG(a->lambda_q1 && a->lambda_k1 && a->lambda_q2 && a->lambda_k2, "null pointer");
     const int64_t blocks = a->B * a->heads * ((a->Lq > a->Lk ? a->Lq : a->Lk) / 32 + 1);
@@ -775,12 +1012,38 @@ BwdSpace bwd_space(const UniterDiffAttention* a) {
     return s;
 }
 
+// Splits of the keys in the forward pass.  The time of a launch goes with the waves that share a SIMD times the tiles each goes through
+// plus about two tiles' worth of prologue and epilogue; joining costs a second launch, about four tiles.
+int splits_for(const UniterDiffAttention* a) {
+    const int nw = waves_for(a->Lq);
+    const int64_t wg = a->B * a->heads * ((a->Lq + 32 * nw - 1) / (32 * nw)), nt = (a->Lk + KT - 1) / KT;
+    int best = 1;
+    double cost = 1e30;
+    for (int ns = 1; ns <= 64 && ns <= nt && wg * ns <= 4096 + wg; ++ns) {
+        const double c = (double)((wg * ns * nw + 1023) / 1024) * (double)((nt + ns - 1) / ns + 2) + (ns > 1 ? 4 : 0);
+        if (c < cost) { cost = c; best = ns; }
+    }
+    return best;
+}
+size_t fwd_space(const UniterDiffAttention* a, int ns) {
+    return ns > 1 ? (size_t)(a->B * a->heads * a->Lq) * ns * (NSTAT + 4 * a->head_dim) * 4 : 0;
+}
+
 template <int D>
-int launch_fwd(const DiffArgs& p, hipStream_t st) {
+int launch_fwd(const DiffArgs& p, int ns, hipStream_t st) {
     const int nw = waves_for(p.Lq), nqb = (p.Lq + 32 * nw - 1) / (32 * nw);
-    const dim3 grid((unsigned)(p.B * p.heads * nqb)), block(64 * nw);
-    if (p.drop.p > 0.f) hipLaunchKernelGGL((diff_fwd_kernel<D, true>), grid, block, 0, st, p, nqb);
-    else hipLaunchKernelGGL((diff_fwd_kernel<D, false>), grid, block, 0, st, p, nqb);
+    const dim3 grid((unsigned)(p.B * p.heads * nqb * ns)), block(64 * nw);
+    const bool drop = p.drop.p > 0.f;
+    if (ns > 1) {
+        if (drop) hipLaunchKernelGGL((diff_fwd_kernel<D, true, true>), grid, block, 0, st, p, nqb, ns);
+        else hipLaunchKernelGGL((diff_fwd_kernel<D, false, true>), grid, block, 0, st, p, nqb, ns);
+        UH_LAUNCH_CHECK();
+        const int64_t rows = (int64_t)p.B * p.heads * p.Lq;
+        hipLaunchKernelGGL((diff_join_kernel<D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, ns);
+    } else {
+        if (drop) hipLaunchKernelGGL((diff_fwd_kernel<D, true, false>), grid, block, 0, st, p, nqb, ns);
+        else hipLaunchKernelGGL((diff_fwd_kernel<D, false, false>), grid, block, 0, st, p, nqb, ns);
+    }
     UH_LAUNCH_CHECK();
     return 0;
 }
@@ -816,8 +1079,12 @@ int launch_bwd(const DiffArgs& p, const BwdSpace& s, const ParamGrads& g, hipStr
 
 extern "C" {
 
+size_t uniter_diff_attention_fwd_workspace_bytes(const UniterDiffAttention* a) {
+    return check(a) || a->B == 0 || a->Lq == 0 ? 0 : fwd_space(a, splits_for(a));
+}
+
 int uniter_diff_attention_fwd(const UniterDiffAttention* a, void* out, int64_t out_row, int64_t out_batch, float* stats, float* maps,
-                              void* stream) {
+                              void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check(a)) return rc;
     if (a->B == 0 || a->Lq == 0) return 0;
     UH_CHECK_ARG(a->q && out && (a->Lk == 0 || (a->k && a->v)), "null pointer");
@@ -827,7 +1094,12 @@ int uniter_diff_attention_fwd(const UniterDiffAttention* a, void* out, int64_t o
     DiffArgs p = args_of(a);
     p.out = (bf16_t*)out; p.lo = out_row; p.bo = out_batch;
     p.stats = stats; p.maps = maps;
-    return a->head_dim == 32 ? launch_fwd<32>(p, (hipStream_t)stream) : launch_fwd<64>(p, (hipStream_t)stream);
+    const int ns = splits_for(a);
+    UH_CHECK_ARG(workspace_bytes >= fwd_space(a, ns) && (workspace != nullptr || ns == 1), "workspace too small");
+    UH_CHECK_ARG(aligned16(workspace), "workspace must be 16-byte aligned");
+    p.psum = (float*)workspace;
+    p.pacc = (float*)workspace + (size_t)(a->B * a->heads * a->Lq) * ns * NSTAT;
+    return a->head_dim == 32 ? launch_fwd<32>(p, ns, (hipStream_t)stream) : launch_fwd<64>(p, ns, (hipStream_t)stream);
 }
 
 size_t uniter_diff_attention_bwd_workspace_bytes(const UniterDiffAttention* a) { return check(a) ? 0 : bwd_space(a).bytes; }
@@ -842,6 +1114,7 @@ int uniter_diff_attention_bwd(const UniterDiffAttention* a, const float* stats, 
     UH_CHECK_ARG(a->B == 0 || a->Lk == 0 || (g->k && g->v), "null pointer");
     UH_CHECK_ARG(aligned16(stats) && aligned16(maps) && aligned16(dout) && aligned16(g->q) && aligned16(g->k) && aligned16(g->v) && aligned16(workspace),
                  "tensors must be 16-byte aligned");
+    UH_CHECK_ARG(dout_row >= 0 && dout_row < (1 << 24), "row strides must be 0 .. 2^24 elements");
     UH_CHECK_ARG((dout_row | dout_batch | g->q_row | g->k_row | g->v_row | g->q_batch | g->k_batch | g->v_batch) % 8 == 0,
                  "row and batch strides must be multiples of 8 elements");
     const BwdSpace s = bwd_space(a);

@@ -993,7 +993,7 @@ def _diff_args(q, k, v, heads, dim, lams, lambda_init, weight, eps, mask, cu_q, 
 
 
 def _diff_forward(q, k, v, cfg, lams, weight, mask, cu_q, cu_k, keep):
-    """(out, stats, maps): one launch on the current stream; stats / maps only when a backward pass will want them."""
+    """(out, stats, maps), launched on the current stream; stats / maps only when a backward pass will want them."""
     heads, dim, lambda_init, eps, max_q, max_k, p, seed, off = cfg
     a = _diff_args(q, k, v, heads, dim, lams, lambda_init, weight, eps, mask, cu_q, cu_k, max_q, max_k, p, seed, off)
     # rows of a packed batch that belong to no example are not written: they are zeros
@@ -1002,9 +1002,12 @@ def _diff_forward(q, k, v, cfg, lams, weight, mask, cu_q, cu_k, keep):
     if keep:
         stats = torch.empty(a.B * heads * a.Lq * 4, dtype=torch.float32, device=q.device)
         maps = torch.empty(out.numel() * 2, dtype=torch.float32, device=q.device)
+    n = C.uniter_diff_attention_fwd_workspace_bytes(ctypes.byref(a))
+    # (workspaces come from the caching allocator, not a shared scratch buffer: calls on other streams and captured graphs get their own)
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     with _on_device(q):
         C.uniter_diff_attention_fwd(ctypes.byref(a), ptr(out), out.stride(-2), out.stride(0) if cu_q is None else 0,
-                                    ptr(stats), ptr(maps), _lib.stream_ptr())
+                                    ptr(stats), ptr(maps), ptr(ws), n, _lib.stream_ptr())
     return out, stats, maps
 
 
@@ -1019,7 +1022,6 @@ def _diff_backward(q, k, v, cfg, lams, weight, mask, cu_q, cu_k, stats, maps, do
     g.lambda_q1, g.lambda_k1, g.lambda_q2, g.lambda_k2 = [ptr(t) for t in dlams]
     g.norm_weight, g.accumulate_params = ptr(dweight), int(accumulate)
     n = C.uniter_diff_attention_bwd_workspace_bytes(ctypes.byref(a))
-    # (from the caching allocator, not a shared scratch buffer: calls on other streams and captured graphs get memory of their own)
     ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
     with _on_device(q):
         C.uniter_diff_attention_bwd(ctypes.byref(a), ptr(stats), ptr(maps), ptr(dout), dout.stride(-2),
