@@ -151,6 +151,14 @@ __device__ __forceinline__ void dma16(const uint32_t voff, const char* origin, c
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// Values loaded before a loop are complete from here on: without it the compiler's wait for them (vmcnt, which counts the tile transfers
+// too) lands inside the loop and waits for the next tile in every round.
+template <int N>
+__device__ __forceinline__ void pin(bf16x8 (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
 template <int W>
 __device__ __forceinline__ void dma_tile(const bf16_t* tile, const bf16_t* src, const int64_t ld, const int r0, const int n, const int wid,
                                          const int nw, const int lane) {
@@ -184,17 +192,16 @@ struct KeyTiles {
         const int k0 = t * KT;
         dma_tile<W>(Ks + (t & 1) * KT * W, K, lk, k0, n, wid, nw, lane);
         dma_tile<W>(Vs + (t & 1) * KT * W, V, lv, k0, n, wid, nw, lane);
-        m = 0.f;
         if (mask != nullptr) m = mask[min(k0 + lane, n - 1)];
     }
     // all waves; on return tile t is complete.  Keys that are out become zeros: whatever stands there, 0 * NaN must not reach a sum.
     __device__ __forceinline__ void finish(const int t) {
         dma_wait();
         asm volatile("" : "+v"(m));                            // (the mask's own wait stays behind the transfers')
-        m = t * KT + lane < n ? mask_log2(m) : -INFINITY;
-        general = __ballot(m != 0.f) != 0;
-        out = __ballot(m == -INFINITY);
-        if (general && wid == 0) mb[(t & 1) * KT + lane] = m;
+        const float mm = t * KT + lane < n ? (mask != nullptr ? mask_log2(m) : 0.f) : -INFINITY;
+        general = __ballot(mm != 0.f) != 0;
+        out = __ballot(mm == -INFINITY);
+        if (general && wid == 0) mb[(t & 1) * KT + lane] = mm;
         __syncthreads();
         if (out != 0) {
             for (int e = wid * 64 + lane; e < KT * (W / 8); e += nw * 64) {
@@ -238,6 +245,119 @@ __device__ __forceinline__ uint32_t keep16(const DiffArgs& p, const uint64_t row
 // whose bf16 operands are as exact as any others, and the reference need not be the maximum.
 constexpr float LAZY = 8.f;
 
+// The running state of a wave's 32 queries, and one step over SUBS blocks of 32 keys of a staged tile.
+template <int D>
+struct FwdState {
+    bf16x8 qf[2][D / 16];
+    f32x16 o[2][D / 16];                 // [map][32 columns of V]
+    float m[2], l[2];
+};
+// With d = 32 both blocks of a tile go through one step: twice the independent work between the dependent stages (scores, maximum,
+// weights, products); with d = 64 the accumulators leave room for one.  V's fragments are on their way during the exponentials.
+template <int D, bool DROP, int SUBS>
+__device__ __forceinline__ void fwd_step(FwdState<D>& f, const DiffArgs& p, const bf16_t* Kt, const bf16_t* Vt, const float* mb, const int u0,
+                                         const int key0, const bool general, const uint64_t drow, const int lane) {
+    constexpr int W = 2 * D, NS = D / 16, NV = W / 32;
+    const int half = lane >> 5;
+    f32x16 s[SUBS][2];
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s[u][j] = zero16();
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks)
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                s[u][j] = mfma32(row_frag<W>(Kt, (u0 + u) * 32 + (lane & 31), (j * D + ks * 16) / 8 + half), f.qf[j][ks], s[u][j]);
+    constexpr int AHEAD = D == 32 ? 2 : 0;                                   // column blocks of V whose fragments are read before the weights are ready
+    bf16x8 vf[SUBS][NV][2];
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+        for (int t = 0; t < AHEAD; ++t)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) vf[u][t][kk] = tr_frag<W>(Vt, (u0 + u) * 32 + kk * 16, t * 32, lane);
+    float se = p.sc;                                           // scores are s * se in log2 units
+    if (general) {
+        se = 1.f;
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 mv = *reinterpret_cast<const f32x4*>(mb + (u0 + u) * 32 + 8 * g + 4 * half);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[u][j][4 * g + e] = __builtin_fmaf(s[u][j][4 * g + e], p.sc, mv[e]);
+            }
+    }
+    float mx[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        float part[2 * SUBS];
+#pragma unroll
+        for (int i = 0; i < 2 * SUBS; ++i) {
+            const f32x16& v = s[i >> 1][j];
+            const int r0 = 8 * (i & 1);
+            part[i] = fmaxf(fmaxf(v[r0], v[r0 + 1]), v[r0 + 2]);
+            part[i] = fmaxf(fmaxf(part[i], v[r0 + 3]), v[r0 + 4]);
+            part[i] = fmaxf(fmaxf(part[i], v[r0 + 5]), fmaxf(v[r0 + 6], v[r0 + 7]));
+        }
+        mx[j] = fmaxf(part[0], part[1]);
+        if constexpr (SUBS == 2) mx[j] = fmaxf(mx[j], fmaxf(part[2], part[3]));
+        mx[j] *= se;
+    }
+    if (__any(mx[0] > f.m[0] + LAZY || mx[1] > f.m[1] + LAZY)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float mn = fmaxf(f.m[j], fmaxf(mx[j], other_half(mx[j])));
+            const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(f.m[j] - mn);
+            f.m[j] = mn;
+            f.l[j] *= alpha;
+#pragma unroll
+            for (int t = 0; t < NV; ++t) f.o[j][t] *= alpha;
+        }
+    }
+    const float ms[2] = {f.m[0] == -INFINITY ? 0.f : f.m[0], f.m[1] == -INFINITY ? 0.f : f.m[1]};      // (a row that has met no key yet)
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+        uint32_t keep = 0xffffu;
+        if constexpr (DROP) keep = keep16(p, drow, key0 + (u0 + u) * 32, half);
+        bf16x8 pf[2][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[u][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j][r], se, -ms[j]));
+                sum[r & 1] += s[u][j][r];
+                if constexpr (DROP) s[u][j][r] = (keep >> r) & 1u ? s[u][j][r] : 0.f;
+            }
+            f.l[j] += sum[0] + sum[1];
+            pf[j][0] = pack_step(s[u][j], 0);
+            pf[j][1] = pack_step(s[u][j], 1);
+        }
+#pragma unroll
+        for (int t = 0; t < NV; ++t) {
+            if (AHEAD > 0 && t + AHEAD < NV) {
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) vf[u][t + AHEAD][kk] = tr_frag<W>(Vt, (u0 + u) * 32 + kk * 16, (t + AHEAD) * 32, lane);
+            }
+            if (AHEAD == 0) {
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) vf[u][t][kk] = tr_frag<W>(Vt, (u0 + u) * 32 + kk * 16, t * 32, lane);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                f.o[0][t] = mfma32(vf[u][t][kk], pf[0][kk], f.o[0][t]);
+                f.o[1][t] = mfma32(vf[u][t][kk], pf[1][kk], f.o[1][t]);
+            }
+        }
+    }
+}
+
 // one workgroup: `nw` waves of 32 queries each, key tiles [t0, t1) of its split.  SPLIT: writes partial sums for diff_join_kernel.
 template <int D, bool DROP, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(const DiffArgs p, const int nqb, const int nsplit) {
@@ -264,102 +384,41 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(const DiffArgs p, cons
     kt.V = p.v + (int64_t)b * p.bv * (p.cu_k == nullptr) + sk.row * p.lv + h * W;
     kt.lk = p.lk; kt.lv = p.lv;
     kt.mask = p.mask != nullptr ? p.mask + (int64_t)b * p.lmask : nullptr;
-    kt.n = sk.n; kt.wid = wid; kt.nw = nw; kt.lane = lane;
+    kt.n = sk.n; kt.wid = wid; kt.nw = nw; kt.lane = lane; kt.m = 0.f;
     if (t0 < t1) kt.start(t0);
 
     const bf16_t* Q = p.q + (int64_t)b * p.bq * (p.cu_q == nullptr) + (sq.row + min(q, sq.n - 1)) * p.lq + h * W + half * 8;
-    bf16x8 qf[2][NS];
+    FwdState<D> f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) qf[j][s] = __builtin_bit_cast(bf16x8, ldg16<false>(Q + j * D + s * 16));
+        for (int s = 0; s < NS; ++s) f.qf[j][s] = __builtin_bit_cast(bf16x8, ldg16<false>(Q + j * D + s * 16));
+        f.m[j] = -INFINITY;
+        f.l[j] = 0.f;
+#pragma unroll
+        for (int t = 0; t < NV; ++t) f.o[j][t] = zero16();
+    }
     float e1, e2;
     lambda_of<D>(p, h, lane, e1, e2);
     const float lam = e1 - e2 + p.lambda_init;
-
-    f32x16 o[2][NV];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int t = 0; t < NV; ++t) o[j][t] = zero16();
     const uint64_t drow = (uint64_t)bh * (uint64_t)p.Lq + (uint64_t)q;
+    pin(f.qf[0]);
+    pin(f.qf[1]);
     if (t0 < t1) kt.finish(t0);
 
     for (int t = t0; t < t1; ++t) {
-        const bool general = kt.general, none = kt.out == ~0ull;
+        const bool general = kt.general;
+        const int subs = kt.out == ~0ull ? 0 : min(2, (sk.n - t * KT + 31) >> 5);
         if (t + 1 < t1) kt.start(t + 1);
         const bf16_t* Kt = Ks + (t & 1) * KT * W;
         const bf16_t* Vt = Vs + (t & 1) * KT * W;
-        const int subs = none ? 0 : min(2, (sk.n - t * KT + 31) >> 5);
-        for (int u = 0; u < subs; ++u) {
-            f32x16 s[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                s[j] = zero16();
-#pragma unroll
-                for (int ks = 0; ks < NS; ++ks)
-                    s[j] = mfma32(row_frag<W>(Kt, u * 32 + (lane & 31), (j * D + ks * 16) / 8 + half), qf[j][ks], s[j]);
-            }
-            float se = p.sc;                                   // scores are s * se in log2 units
-            if (general) {
-                se = 1.f;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 mv = *reinterpret_cast<const f32x4*>(mb + (t & 1) * KT + u * 32 + 8 * g + 4 * half);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[j][4 * g + e] = __builtin_fmaf(s[j][4 * g + e], p.sc, mv[e]);
-                }
-            }
-            float mx[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                mx[j] = fmaxf(s[j][0], s[j][1]);
-#pragma unroll
-                for (int r = 2; r < 16; r += 2) mx[j] = fmaxf(fmaxf(mx[j], s[j][r]), s[j][r + 1]);
-                mx[j] *= se;
-            }
-            if (__any(mx[0] > m[0] + LAZY || mx[1] > m[1] + LAZY)) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float mn = fmaxf(m[j], fmaxf(mx[j], other_half(mx[j])));
-                    const float alpha = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[j] - mn);
-                    m[j] = mn;
-                    l[j] *= alpha;
-#pragma unroll
-                    for (int t2 = 0; t2 < NV; ++t2) o[j][t2] *= alpha;
-                }
-            }
-            uint32_t keep = 0xffffu;
-            if constexpr (DROP) keep = keep16(p, drow, t * KT + u * 32, half);
-            bf16x8 pf[2][2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float ms = m[j] == -INFINITY ? 0.f : m[j];               // (a row that has met no key yet)
-                float sum = 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], se, -ms));
-                    sum += s[j][r];
-                    if constexpr (DROP) s[j][r] = (keep >> r) & 1u ? s[j][r] : 0.f;
-                }
-                l[j] += sum;
-                pf[j][0] = pack_step(s[j], 0);
-                pf[j][1] = pack_step(s[j], 1);
-            }
-#pragma unroll
-            for (int t2 = 0; t2 < NV; ++t2)
-#pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    const bf16x8 vf = tr_frag<W>(Vt, u * 32 + kk * 16, t2 * 32, lane);
-                    o[0][t2] = mfma32(vf, pf[0][kk], o[0][t2]);
-                    o[1][t2] = mfma32(vf, pf[1][kk], o[1][t2]);
-                }
-        }
+        const float* mt = mb + (t & 1) * KT;
+        for (int u = 0; u < subs; ++u) fwd_step<D, DROP, 1>(f, p, Kt, Vt, mt, u, t * KT, general, drow, lane);
         if (t + 1 < t1) kt.finish(t + 1);
     }
+    f32x16(&o)[2][NV] = f.o;
+    float(&m)[2] = f.m;
+    float(&l)[2] = f.l;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         l[j] += other_half(l[j]);
@@ -672,7 +731,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(const DiffArgs p, c
     kt.V = p.v + (int64_t)b * p.bv * (p.cu_k == nullptr) + sk.row * p.lv + h * W;
     kt.lk = p.lk; kt.lv = p.lv;
     kt.mask = p.mask != nullptr ? p.mask + (int64_t)b * p.lmask : nullptr;
-    kt.n = sk.n; kt.wid = wid; kt.nw = nw; kt.lane = lane;
+    kt.n = sk.n; kt.wid = wid; kt.nw = nw; kt.lane = lane; kt.m = 0.f;
     if (nt > 0) kt.start(0);
 
     const bf16_t* Q = p.q + (int64_t)b * p.bq * (p.cu_q == nullptr) + (sq.row + qs) * p.lq + h * W + half * 8;
@@ -686,7 +745,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(const DiffArgs p, c
     }
     const f32x4 st = *reinterpret_cast<const f32x4*>(p.stats + ((int64_t)bh * p.Lq + qs) * NSTAT);
     const float m[2] = {st[0], st[2]}, ll[2] = {st[1], st[3]};
-    const float Dq[2] = {p.D[((int64_t)bh * p.Lq + qs) * 2], p.D[((int64_t)bh * p.Lq + qs) * 2 + 1]};
+    float Dq[2] = {p.D[((int64_t)bh * p.Lq + qs) * 2], p.D[((int64_t)bh * p.Lq + qs) * 2 + 1]};
     float e1, e2;
     lambda_of<D>(p, h, lane, e1, e2);
     const float lam = e1 - e2 + p.lambda_init;
@@ -698,6 +757,11 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(const DiffArgs p, c
     for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int t = 0; t < ND; ++t) dq[j][t] = zero16();
+    pin(qf[0]);
+    pin(qf[1]);
+    pin(gf);
+    float c_lse[2] = {m[0] + ll[0], m[1] + ll[1]};
+    asm volatile("" : "+v"(c_lse[0]), "+v"(c_lse[1]), "+v"(Dq[0]), "+v"(Dq[1]));
     if (nt > 0) kt.finish(0);
 
     for (int t = 0; t < nt; ++t) {
@@ -717,8 +781,15 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(const DiffArgs p, c
             }
 #pragma unroll
             for (int i = 0; i < W / 16; ++i) g = mfma32(row_frag<W>(Vt, u * 32 + (lane & 31), 2 * i + half), gf[i], g);
+            bf16x8 kf[2][ND][2];                               // on their way during the exponentials
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int t2 = 0; t2 < ND; ++t2)
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk) kf[j][t2][kk] = tr_frag<W>(Kt, u * 32 + kk * 16, j * D + t2 * 32, lane);
             // weights 2^(s se - c): with a mask the maximum is taken off the masked score first, as in the forward pass
-            float se = p.sc, c[2] = {m[0] + ll[0], m[1] + ll[1]};
+            float se = p.sc, c[2] = {c_lse[0], c_lse[1]};
             if (general) {
                 se = 1.f;
 #pragma unroll
@@ -751,7 +822,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(const DiffArgs p, c
                 for (int t2 = 0; t2 < ND; ++t2)
 #pragma unroll
                     for (int kk = 0; kk < 2; ++kk)
-                        dq[j][t2] = mfma32(tr_frag<W>(Kt, u * 32 + kk * 16, j * D + t2 * 32, lane), df[j][kk], dq[j][t2]);
+                        dq[j][t2] = mfma32(kf[j][t2][kk], df[j][kk], dq[j][t2]);
         }
         if (t + 1 < nt) kt.finish(t + 1);
     }
@@ -848,6 +919,9 @@ __global__ __launch_bounds__(256, D == 32 ? 2 : 1) void diff_bwd_dkv_kernel(cons
     for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int t = 0; t < ND; ++t) dk[j][t] = zero16();
+    pin(kf[0]);
+    pin(kf[1]);
+    pin(vf);
     if (nt > 0) finish(0);
 
     for (int t = 0; t < nt; ++t) {
@@ -867,6 +941,16 @@ __global__ __launch_bounds__(256, D == 32 ? 2 : 1) void diff_bwd_dkv_kernel(cons
             }
 #pragma unroll
             for (int i = 0; i < W / 16; ++i) g = mfma32(row_frag<W>(Ot, u * 32 + (lane & 31), 2 * i + half), vf[i], g);
+            bf16x8 ot[NV][2], qt[2][ND][2];                    // on their way during the exponentials
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+                for (int t2 = 0; t2 < NV; ++t2) ot[t2][kk] = tr_frag<W>(Ot, u * 32 + kk * 16, t2 * 32, lane);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int t2 = 0; t2 < ND; ++t2) qt[j][t2][kk] = tr_frag<W>(Qt, u * 32 + kk * 16, j * D + t2 * 32, lane);
+            }
             float se = p.sc;
             const float* cs = w + ST_LSE * KT;
             if (general) {
@@ -918,12 +1002,12 @@ __global__ __launch_bounds__(256, D == 32 ? 2 : 1) void diff_bwd_dkv_kernel(cons
             for (int kk = 0; kk < 2; ++kk) {
                 const bf16x8 af = pack_step(a, kk);
 #pragma unroll
-                for (int t2 = 0; t2 < NV; ++t2) dv[t2] = mfma32(tr_frag<W>(Ot, u * 32 + kk * 16, t2 * 32, lane), af, dv[t2]);
+                for (int t2 = 0; t2 < NV; ++t2) dv[t2] = mfma32(ot[t2][kk], af, dv[t2]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const bf16x8 df = pack_step(s[j], kk);
 #pragma unroll
-                    for (int t2 = 0; t2 < ND; ++t2) dk[j][t2] = mfma32(tr_frag<W>(Qt, u * 32 + kk * 16, j * D + t2 * 32, lane), df, dk[j][t2]);
+                    for (int t2 = 0; t2 < ND; ++t2) dk[j][t2] = mfma32(qt[j][t2][kk], df, dk[j][t2]);
                 }
             }
         }
@@ -1013,14 +1097,16 @@ BwdSpace bwd_space(const UniterDiffAttention* a) {
 }
 
 // Splits of the keys in the forward pass.  The time of a launch goes with the waves that share a SIMD times the tiles each goes through
-// plus about two tiles' worth of prologue and epilogue; joining costs a second launch, about four tiles.
+// (about 1 us with d = 32, 1.5 with d = 64) plus about two tiles' worth of prologue and epilogue; joining costs a second launch (3 us) and
+// the partial sums' way to memory and back.
 int splits_for(const UniterDiffAttention* a) {
     const int nw = waves_for(a->Lq);
     const int64_t wg = a->B * a->heads * ((a->Lq + 32 * nw - 1) / (32 * nw)), nt = (a->Lk + KT - 1) / KT;
+    const double tile = a->head_dim == 32 ? 1.0 : 1.5, part = (double)(a->B * a->heads * a->Lq) * (16.0 * a->head_dim + 16.0) * 2e-6 / 2.5;
     int best = 1;
     double cost = 1e30;
     for (int ns = 1; ns <= 64 && ns <= nt && wg * ns <= 4096 + wg; ++ns) {
-        const double c = (double)((wg * ns * nw + 1023) / 1024) * (double)((nt + ns - 1) / ns + 2) + (ns > 1 ? 4 : 0);
+        const double c = tile * (double)((wg * ns * nw + 1023) / 1024) * (double)((nt + ns - 1) / ns + 2) + (ns > 1 ? 3.0 + ns * part : 0.0);
         if (c < cost) { cost = c; best = ns; }
     }
     return best;

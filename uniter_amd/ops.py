@@ -849,47 +849,51 @@ def dense_gelu(mod, hidden_states):
 # rotary positions and differential attention (no counterpart in the reference: they stand beside BertSelfAttention's learned
 # positions and softmax attention, model/layer.py:75-101, model/model.py:217-245)
 # ----------------------------------------------------------------------------------------------------
-class _on_device(object):
-    """Make the device of `t` the current one for the launches inside (free when it already is)."""
-
-    def __init__(self, t):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_I3 = ctypes.c_int64 * 3
 
 
-def _same_device(first, name, *others):
+def _launch_on(t, fn, *args):
+    """fn(*args, stream) on t's device (the current one or not) and that device's current stream."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        fn(*args, _lib.stream_ptr())
+    else:
+        with torch.cuda.device(t.device):
+            fn(*args, _lib.stream_ptr())
+
+
+def _check_same_device(first, name, others):
+    dev = first.get_device()
     for t, what in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             raise _lib.UniterHipError("%s is on %s, %s on %s" % (what, t.device, name, first.device))
 
 
 def _rows16(t):
     """`t` with contiguous rows that start on 16 bytes (a copy when they do not)."""
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-    return t if ok and all(s % 8 == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])) else t.contiguous()
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0:
+        for s, n in zip(st[:-1], t.shape):
+            if s % 8 != 0 and n != 1:
+                break
+        else:
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _rotary_launch(x, y, positions, offset, rot, inverse):
     if x.numel() == 0:
         return
-    B, L = (x.shape[0], x.shape[1]) if x.dim() == 4 else (1, x.shape[0])
-    r = _lib.UniterRotary()
-    r.B, r.L, r.heads, r.head_dim, r.rot_dim = B, L, x.shape[-2], x.shape[-1], rot.rotary_dim
-    turns = rot.turns(x.device)
-    r.freq, r.positions = turns.data_ptr(), ptr(positions)
-    r.positions_batch_stride = 0 if positions is None or positions.dim() == 1 else positions.stride(0)
-    r.position_offset = offset
-    r.multiplier, r.interleaved, r.inverse = rot.multiplier, int(rot.interleaved), int(inverse)
-    strides = [(ctypes.c_int64 * 3)(*(((0,) if t.dim() == 3 else ()) + tuple(t.stride()[:-1]))) for t in (x, y)]
-    with _on_device(x):
-        C.uniter_rotary(ctypes.byref(r), ptr(x), strides[0], ptr(y), strides[1], _lib.stream_ptr())
+    shape, sx, sy = x.shape, x.stride(), y.stride()
+    if len(shape) == 4:
+        B, L, heads, dim = shape
+        sx, sy = _I3(sx[0], sx[1], sx[2]), _I3(sy[0], sy[1], sy[2])
+    else:
+        B, (L, heads, dim) = 1, shape
+        sx, sy = _I3(0, sx[0], sx[1]), _I3(0, sy[0], sy[1])
+    pos, pos_b = (None, 0) if positions is None else (positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0)
+    r = _lib.UniterRotary(B, L, heads, dim, rot.rotary_dim, rot.turns(x.device).data_ptr(), pos, pos_b, offset, rot.multiplier,
+                          rot.interleaved, inverse)
+    _launch_on(x, C.uniter_rotary, ctypes.byref(r), x.data_ptr(), sx, y.data_ptr(), sy)
 
 
 class _RotaryFn(torch.autograd.Function):
@@ -919,37 +923,42 @@ def rotary(x, positions, rot, offset=0, out=None):
     0 .. L - 1 (of every row of the batch); `offset` is added to either.  Returns a new tensor; out=x turns x in place, out=another
     tensor of x's shape writes there (both outside autograd only).  The gradient is turned back by the same kernel."""
     _check_dev(x, "rotary input")
-    if x.dim() not in (3, 4) or x.shape[-1] != rot.head_dim:
+    nd = x.dim()
+    if nd not in (3, 4) or x.shape[-1] != rot.head_dim:
         raise _lib.UniterHipError("rotary input must be [B, L, heads, %d] or [T, heads, %d], got %s" % (rot.head_dim, rot.head_dim, tuple(x.shape)))
-    rows = tuple(x.shape[:-2])
-    if x.dim() == 3 and positions is None:
-        raise _lib.UniterHipError("rotary: rows stored back to back need their positions")
-    if positions is not None:
+    if positions is None:
+        if nd == 3:
+            raise _lib.UniterHipError("rotary: rows stored back to back need their positions")
+    else:
         if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int64, torch.int32):
             raise _lib.UniterHipError("rotary: positions must be an int64 or int32 tensor (or None)")
-        _same_device(x, "x", (positions, "positions"))
-        if positions.dim() == 2 and positions.shape[0] == 1 and len(rows) == 2:
+        _check_same_device(x, "x", ((positions, "positions"),))
+        if nd == 4 and positions.dim() == 2 and positions.shape[0] == 1:
             positions = positions[0]
-        if tuple(positions.shape) not in (rows, rows[-1:]):
-            raise _lib.UniterHipError("rotary: positions must be %s or %s, got %s" % (list(rows), list(rows[-1:]), list(positions.shape)))
-        positions = positions.to(torch.int64)
-        if positions.numel() and positions.stride(-1) != 1:
+        if positions.shape != x.shape[:-2] and positions.shape != x.shape[-3:-2]:
+            raise _lib.UniterHipError("rotary: positions must be %s or %s, got %s" % (list(x.shape[:-2]), list(x.shape[-3:-2]), list(positions.shape)))
+        if positions.dtype != torch.int64:
+            positions = positions.to(torch.int64)
+        if positions.stride(-1) != 1:
             positions = positions.contiguous()
-    if x.stride(-1) != 1 and x.numel():
+    if x.stride(-1) != 1:
         if out is x:
             raise _lib.UniterHipError("rotary: in place needs contiguous heads")
         x = x.contiguous()
     if out is None:
-        return _RotaryFn.apply(x, positions, int(offset), rot)
-    if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
-        raise _lib.UniterHipError("rotary: out= writes outside autograd; call it without gradients or let it return a new tensor")
-    _check_dev(out, "rotary output")
-    _same_device(x, "x", (out, "out"))
-    if out.shape != x.shape or (out.numel() and out.stride(-1) != 1):
-        raise _lib.UniterHipError("rotary: out must have x's shape and contiguous heads")
-    if out.numel() and out.data_ptr() != x.data_ptr() and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() \
-            and _overlap(out, x):
-        raise _lib.UniterHipError("rotary: out overlaps x without being x")
+        if x.requires_grad and torch.is_grad_enabled():
+            return _RotaryFn.apply(x, positions, int(offset), rot)
+        out = torch.empty(x.shape, dtype=_BF16, device=x.device)
+    else:
+        if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
+            raise _lib.UniterHipError("rotary: out= writes outside autograd; call it without gradients or let it return a new tensor")
+        _check_dev(out, "rotary output")
+        _check_same_device(x, "x", ((out, "out"),))
+        if out.shape != x.shape or out.stride(-1) != 1:
+            raise _lib.UniterHipError("rotary: out must have x's shape and contiguous heads")
+        if out.numel() and (out.data_ptr() != x.data_ptr() or out.stride() != x.stride()) \
+                and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() and _overlap(out, x):
+            raise _lib.UniterHipError("rotary: out overlaps x without being x")
     _rotary_launch(x, out, positions, int(offset), rot, False)
     return out
 
@@ -970,122 +979,118 @@ def _overlap(a, b):
     return True
 
 
-def _diff_args(q, k, v, heads, dim, lams, lambda_init, weight, eps, mask, cu_q, cu_k, max_q, max_k, p, seed, off):
-    a = _lib.UniterDiffAttention()
-    a.q, a.k, a.v = ptr(q), ptr(k), ptr(v)
-    a.q_row, a.k_row, a.v_row = q.stride(-2), k.stride(-2), v.stride(-2)
-    if cu_q is None:
-        a.q_batch, a.k_batch, a.v_batch = q.stride(0), k.stride(0), v.stride(0)
-        a.B, a.Lq, a.Lk = q.shape[0], q.shape[1], k.shape[1]
-    else:
-        a.cu_seqlens_q, a.cu_seqlens_k = ptr(cu_q), ptr(cu_k)
-        a.total_q, a.total_k = q.shape[0], k.shape[0]
-        a.B, a.Lq, a.Lk = cu_q.numel() - 1, max_q, max_k
-    if mask is not None:
-        a.mask_bias, a.mask_row = ptr(mask), mask.stride(0)
-    a.lambda_q1, a.lambda_k1, a.lambda_q2, a.lambda_k2 = [ptr(t) for t in lams]
-    a.norm_weight = ptr(weight)
-    a.heads, a.head_dim = heads, dim
-    a.lambda_init, a.norm_eps, a.p_drop = lambda_init, eps, p
-    a.lambda_per_head = int(lams[0].dim() == 2)
-    a.seed, a.offset = seed, off
-    return a
+def _qkv_of(t, k, v):
+    """(pointers, row strides, batch strides) of q, k, v: three tensors, or the thirds of one projection's rows (k, v None)."""
+    b = t.stride(0)
+    if k is None:
+        row, third = t.stride(-2), t.shape[-1] // 3 * 2
+        p = t.data_ptr()
+        return (p, p + third, p + 2 * third), (row, row, row), (b, b, b)
+    return ((t.data_ptr(), k.data_ptr(), v.data_ptr()), (t.stride(-2), k.stride(-2), v.stride(-2)), (b, k.stride(0), v.stride(0)))
 
 
-def _diff_forward(q, k, v, cfg, lams, weight, mask, cu_q, cu_k, keep):
-    """(out, stats, maps), launched on the current stream; stats / maps only when a backward pass will want them."""
+def _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams):
     heads, dim, lambda_init, eps, max_q, max_k, p, seed, off = cfg
-    a = _diff_args(q, k, v, heads, dim, lams, lambda_init, weight, eps, mask, cu_q, cu_k, max_q, max_k, p, seed, off)
+    ptrs, rows, batches = _qkv_of(q, k, v)
+    if cu_q is None:
+        Lq = q.shape[1]
+        packed = (None, None, 0, 0)
+        B, Lk = q.shape[0], Lq if k is None else k.shape[1]
+    else:
+        packed = (cu_q.data_ptr(), cu_k.data_ptr(), q.shape[0], q.shape[0] if k is None else k.shape[0])
+        B, Lq, Lk = cu_q.shape[0] - 1, max_q, max_k
+    return _lib.UniterDiffAttention(*ptrs, *rows, *batches, ptr(mask), 0 if mask is None else mask.stride(0), *packed,
+                                    lams[0].data_ptr(), lams[1].data_ptr(), lams[2].data_ptr(), lams[3].data_ptr(), ptr(weight),
+                                    B, Lq, Lk, heads, dim, lambda_init, eps, p, lams[0].dim() == 2, seed, off)
+
+
+def _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, keep):
+    """(out, stats, maps), launched on the current stream; stats / maps only when a backward pass will want them."""
+    a = _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams)
+    H = a.heads * 2 * a.head_dim
     # rows of a packed batch that belong to no example are not written: they are zeros
-    out = (torch.empty if cu_q is None else torch.zeros)(q.shape, dtype=_BF16, device=q.device)
-    stats = maps = None
+    out = (torch.empty if cu_q is None else torch.zeros)((*q.shape[:-1], H), dtype=_BF16, device=q.device)
+    stats = maps = ws = None
     if keep:
-        stats = torch.empty(a.B * heads * a.Lq * 4, dtype=torch.float32, device=q.device)
+        stats = torch.empty(a.B * a.heads * a.Lq * 4, dtype=torch.float32, device=q.device)
         maps = torch.empty(out.numel() * 2, dtype=torch.float32, device=q.device)
-    n = C.uniter_diff_attention_fwd_workspace_bytes(ctypes.byref(a))
-    # (workspaces come from the caching allocator, not a shared scratch buffer: calls on other streams and captured graphs get their own)
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    with _on_device(q):
-        C.uniter_diff_attention_fwd(ctypes.byref(a), ptr(out), out.stride(-2), out.stride(0) if cu_q is None else 0,
-                                    ptr(stats), ptr(maps), ptr(ws), n, _lib.stream_ptr())
+    ref = ctypes.byref(a)
+    n = C.uniter_diff_attention_fwd_workspace_bytes(ref)
+    if n:
+        # (workspaces come from the caching allocator, not a shared scratch buffer: other streams and captured graphs get their own)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+    _launch_on(q, C.uniter_diff_attention_fwd, ref, out.data_ptr(), H, out.stride(0), ptr(stats), ptr(maps), ptr(ws), n)
     return out, stats, maps
 
 
-def _diff_backward(q, k, v, cfg, lams, weight, mask, cu_q, cu_k, stats, maps, dout, dq, dk, dv, dlams, dweight, accumulate):
-    heads, dim, lambda_init, eps, max_q, max_k, p, seed, off = cfg
-    a = _diff_args(q, k, v, heads, dim, lams, lambda_init, weight, eps, mask, cu_q, cu_k, max_q, max_k, p, seed, off)
-    g = _lib.UniterDiffAttentionGrads()
-    g.q, g.k, g.v = ptr(dq), ptr(dk), ptr(dv)
-    g.q_row, g.k_row, g.v_row = dq.stride(-2), dk.stride(-2), dv.stride(-2)
-    if cu_q is None:
-        g.q_batch, g.k_batch, g.v_batch = dq.stride(0), dk.stride(0), dv.stride(0)
-    g.lambda_q1, g.lambda_k1, g.lambda_q2, g.lambda_k2 = [ptr(t) for t in dlams]
-    g.norm_weight, g.accumulate_params = ptr(dweight), int(accumulate)
-    n = C.uniter_diff_attention_bwd_workspace_bytes(ctypes.byref(a))
+def _diff_backward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, stats, maps, dout, dq, dk, dv, dlams, dweight, accumulate):
+    """dq / dk / dv: tensors like q / k / v (one [.., 3 H] tensor and None, None for a fused projection)."""
+    a = _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams)
+    ptrs, rows, batches = _qkv_of(dq, dk, dv)
+    g = _lib.UniterDiffAttentionGrads(*ptrs, *rows, *batches, ptr(dlams[0]), ptr(dlams[1]), ptr(dlams[2]), ptr(dlams[3]), ptr(dweight),
+                                      accumulate)
+    ref = ctypes.byref(a)
+    n = C.uniter_diff_attention_bwd_workspace_bytes(ref)
     ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
-    with _on_device(q):
-        C.uniter_diff_attention_bwd(ctypes.byref(a), ptr(stats), ptr(maps), ptr(dout), dout.stride(-2),
-                                    dout.stride(0) if cu_q is None else 0, ctypes.byref(g), ptr(ws), n, _lib.stream_ptr())
+    _launch_on(q, C.uniter_diff_attention_bwd, ref, ptr(stats), ptr(maps), dout.data_ptr(), dout.stride(-2), dout.stride(0),
+               ctypes.byref(g), ws.data_ptr(), n)
 
 
 class _DiffAttentionFn(torch.autograd.Function):
     """fused: `q` is the whole [.., 3 H] projection (k, v None), and so is its gradient."""
 
     @staticmethod
-    def forward(ctx, q, k, v, mask, cu_q, cu_k, cfg, keep, weight, *lams):
-        ctx.fused = k is None
-        qs, ks, vs = q.split(q.shape[-1] // 3, dim=-1) if ctx.fused else (q, k, v)
-        out, stats, maps = _diff_forward(qs, ks, vs, cfg, lams, weight, mask, cu_q, cu_k, keep)
+    def forward(ctx, q, k, v, mask, cu_q, cu_k, cfg, weight, *lams):
+        out, stats, maps = _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, True)
         ctx.cfg = cfg
-        if keep:
-            ctx.save_for_backward(q, k, v, mask, cu_q, cu_k, weight, stats, maps, *lams)
+        ctx.save_for_backward(q, k, v, mask, cu_q, cu_k, weight, stats, maps, *lams)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, mask, cu_q, cu_k, weight, stats, maps = ctx.saved_tensors[:9]
-        lams = ctx.saved_tensors[9:]
+        q, k, v, mask, cu_q, cu_k, weight, stats, maps, *lams = ctx.saved_tensors
         dout = _rows16(dout)
         new = torch.empty if cu_q is None else torch.zeros             # rows of no example have no gradient
         dq = new(q.shape, dtype=_BF16, device=q.device)
-        if ctx.fused:
-            H = q.shape[-1] // 3
-            qs, ks, vs = q.split(H, dim=-1)
-            dqs, dks, dvs = dq.split(H, dim=-1)
-            dk = dv = None
-        else:
-            dk, dv = (new(t.shape, dtype=_BF16, device=q.device) for t in (k, v))
-            qs, ks, vs, dqs, dks, dvs = q, k, v, dq, dk, dv
-        dlams = [torch.empty_like(t) for t in lams]
+        dk = dv = None
+        if k is not None:
+            dk, dv = new(k.shape, dtype=_BF16, device=q.device), new(v.shape, dtype=_BF16, device=q.device)
+        dlams = torch.empty((4, *lams[0].shape), dtype=_BF16, device=q.device).unbind(0)
         dweight = None if weight is None else torch.empty_like(weight)
-        _diff_backward(qs, ks, vs, ctx.cfg, lams, weight, mask, cu_q, cu_k, stats, maps, dout, dqs, dks, dvs, dlams, dweight, False)
-        return (dq, dk, dv, None, None, None, None, None, dweight) + tuple(dlams)
+        _diff_backward(q, k, v, mask, cu_q, cu_k, ctx.cfg, weight, lams, stats, maps, dout, dq, dk, dv, dlams, dweight, False)
+        return (dq, dk, dv, None, None, None, None, dweight, *dlams)
 
 
-def _diff_check(data, widths, heads, lams, lambda_init, weight, mask, cu_q, cu_k, max_q, max_k, p_drop):
-    """Arguments common to both calls; returns (dim, mask, cu_q, cu_k, max_q, max_k, lams, weight)."""
-    q, name = data[0]
-    H = q.shape[-1] // widths
-    if heads < 1 or q.shape[-1] % widths or H % (2 * heads) or H // (2 * heads) not in (32, 64):
+def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, p_drop):
+    """What both calls ask of their arguments (k, v None: q is a fused projection); (dim, mask, cu_q, cu_k, max_q, max_k, lams, weight)."""
+    fused = k is None
+    H, odd = divmod(q.shape[-1], 3) if fused else (q.shape[-1], 0)
+    dim = H // (2 * heads) if heads > 0 else 0
+    if odd or dim not in (32, 64) or H != heads * 2 * dim:
         raise _lib.UniterHipError("differential attention: a head is 64 or 128 columns (two maps of 32 or 64), got %d columns for %d heads" % (H, heads))
-    dim = H // (2 * heads)
     packed = cu_q is not None or cu_k is not None
-    for t, what in data:
+    for t, what in ((q, "qkv"),) if fused else ((q, "q"), (k, "k"), (v, "v")):
         _check_dev(t, what)
         if t.dim() != (2 if packed else 3):
             raise _lib.UniterHipError("%s must be %s, got %s" % (what, "[rows, columns] when cu_seqlens is given" if packed else "[B, L, columns]", tuple(t.shape)))
-    lams = tuple(lams)
+    Bk = q if fused else k
+    if not fused and (k.shape != v.shape or k.shape[-1] != H or (not packed and k.shape[0] != q.shape[0])):
+        raise _lib.UniterHipError("differential attention: q %s, k %s and v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if len(lams) != 4:
         raise _lib.UniterHipError("lambdas are four tensors: q1, k1, q2, k2")
+    shape = lams[0].shape
+    if shape != (heads, dim) and shape != (dim,):
+        raise _lib.UniterHipError("lambda vectors must be [%d] or [%d, %d], got %s" % (dim, heads, dim, tuple(shape)))
     for t in lams:
         _check_dev(t, "lambda vector")
-        if tuple(t.shape) not in ((dim,), (heads, dim)) or t.shape != lams[0].shape:
-            raise _lib.UniterHipError("lambda vectors must all be [%d] or [%d, %d], got %s" % (dim, heads, dim, tuple(t.shape)))
+        if t.shape != shape:
+            raise _lib.UniterHipError("lambda vectors must have one shape, got %s and %s" % (tuple(shape), tuple(t.shape)))
     if weight is not None:
         _check_dev(weight, "norm_weight")
-        if tuple(weight.shape) != (2 * dim,):
+        if weight.shape != (2 * dim,):
             raise _lib.UniterHipError("norm_weight must be [%d], got %s" % (2 * dim, tuple(weight.shape)))
+        weight = _rows16(weight)
     if not 0.0 <= p_drop < 1.0:
         raise _lib.UniterHipError("dropout probability must be in [0, 1), got %r" % (p_drop,))
     if packed:
@@ -1104,27 +1109,27 @@ def _diff_check(data, widths, heads, lams, lambda_init, weight, mask, cu_q, cu_k
         _check_dev(mask, "mask_bias", torch.float32)
         if mask.dim() == 4:                        # UniterModel's extended mask [B, 1, 1, L]
             mask = mask.reshape(mask.shape[0], mask.shape[-1])
-        if tuple(mask.shape) != (q.shape[0], data[-1][0].shape[1]):
-            raise _lib.UniterHipError("mask_bias must be [%d, %d] (or [B, 1, 1, Lk]), got %s" % (q.shape[0], data[-1][0].shape[1], tuple(mask.shape)))
-        if mask.numel() and mask.stride(1) != 1:
+        if mask.shape != (q.shape[0], Bk.shape[1]):
+            raise _lib.UniterHipError("mask_bias must be [%d, %d] (or [B, 1, 1, Lk]), got %s" % (q.shape[0], Bk.shape[1], tuple(mask.shape)))
+        if mask.stride(1) != 1:
             mask = mask.contiguous()
-    _same_device(q, name, (mask, "mask_bias"), (cu_q, "cu_seqlens"), (cu_k, "cu_seqlens_k"), (weight, "norm_weight"),
-                 *[(t, what) for t, what in data[1:]], *[(t, "lambda vector") for t in lams])
-    lams = tuple(t.contiguous() for t in lams)
-    weight = None if weight is None else _rows16(weight.contiguous())
-    return dim, mask, cu_q, cu_k, max_q, max_k, lams, weight
+    dev = q.get_device()
+    for t in (k, v, mask, cu_q, cu_k, weight, *lams):
+        if t is not None and t.get_device() != dev:
+            raise _lib.UniterHipError("differential attention: all tensors must be on %s, one is on %s" % (q.device, t.device))
+    return dim, mask, cu_q, cu_k, max_q, max_k, [t.contiguous() for t in lams], weight
 
 
 def _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop):
     dim, mask, cu_q, cu_k, max_q, max_k, lams, weight = checked
     q = _rows16(q)
-    k, v = (None, None) if k is None else (_rows16(k), _rows16(v))
-    tensors = [t for t in (q, k, v, weight) + lams if t is not None]
-    keep = torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
-    p = float(p_drop)
-    seed, off = _next_offsets(1) if p > 0.0 else (0, 0)
-    cfg = (heads, dim, float(lambda_init), float(eps), max_q, max_k, p, seed, off)
-    return _DiffAttentionFn.apply(q, k, v, mask, cu_q, cu_k, cfg, keep, weight, *lams)
+    if k is not None:
+        k, v = _rows16(k), _rows16(v)
+    seed, off = _next_offsets(1) if p_drop > 0.0 else (0, 0)
+    cfg = (heads, dim, lambda_init, eps, max_q, max_k, p_drop, seed, off)
+    if torch.is_grad_enabled() and any([t.requires_grad for t in (q, k, v, weight, *lams) if t is not None]):
+        return _DiffAttentionFn.apply(q, k, v, mask, cu_q, cu_k, cfg, weight, *lams)
+    return _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, False)[0]
 
 
 def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=None, mask_bias=None, cu_seqlens=None, cu_seqlens_k=None,
@@ -1138,10 +1143,7 @@ def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=Non
     Packed rows: q [T, ..], k / v [Tk, ..], cu_seqlens int32 [examples + 1] on the device and max_len (a longest example's length, host
     int); cu_seqlens_k / max_len_k where the keys' differ.  Rows of no example come back as zeros.
     p_drop: dropout on the difference of the maps (callers pass 0 in evaluation).  Gradients flow to q, k, v, lambdas and norm_weight."""
-    checked = _diff_check([(q, "q"), (k, "k"), (v, "v")], 1, heads, lambdas, lambda_init, norm_weight, mask_bias, cu_seqlens, cu_seqlens_k,
-                          max_len, max_len_k, p_drop)
-    if k.shape != v.shape or k.shape[-1] != q.shape[-1] or (cu_seqlens is None and k.shape[0] != q.shape[0]):
-        raise _lib.UniterHipError("differential attention: q %s, k %s and v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    checked = _diff_check(q, k, v, heads, lambdas, norm_weight, mask_bias, cu_seqlens, cu_seqlens_k, max_len, max_len_k, p_drop)
     return _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop)
 
 
@@ -1149,7 +1151,7 @@ def differential_self_attention(qkv, heads, lambdas, lambda_init, norm_weight=No
                                 eps=1e-5, p_drop=0.0):
     """differential_attention on a fused projection qkv [B, L, 3 H] (or packed [T, 3 H]), H = heads * 2 d: the q | k | v layout that
     BertSelfAttention.fused_qkv produces.  Its gradient is one [.., 3 H] tensor too."""
-    checked = _diff_check([(qkv, "qkv")], 3, heads, lambdas, lambda_init, norm_weight, mask_bias, cu_seqlens, None, max_len, None, p_drop)
+    checked = _diff_check(qkv, None, None, heads, lambdas, norm_weight, mask_bias, cu_seqlens, None, max_len, None, p_drop)
     return _diff_apply(qkv, None, None, heads, checked, lambda_init, eps, p_drop)
 
 
