@@ -15,6 +15,7 @@ from torch import nn
 
 from .. import ops
 from .._lib import UniterHipError
+from .rotary import RotaryPositions
 
 # The reference aliases apex FusedLayerNorm as BertLayerNorm (model/layer.py:25); the parameter holder here
 # is torch's LayerNorm (same `weight` / `bias` names, same math for the head-side uses).
@@ -150,6 +151,51 @@ class BertSelfAttention(nn.Module):
         return ops.self_attention(self, hidden_states, attention_mask)
 
 
+class HeadRMSNorm(nn.Module):
+    """Weight of differential attention's per-head normalisation (applied inside the attention kernel)."""
+
+    def __init__(self, width, eps=1e-5):
+        super(HeadRMSNorm, self).__init__()
+        self.weight = nn.Parameter(torch.ones(width))
+        self.eps = eps
+
+
+class BertDifferentialSelfAttention(BertSelfAttention):
+    """Differential self-attention in the place of BertSelfAttention: the same query / key / value projections (fused storage, arena,
+    checkpoint names), per head the difference of two softmax maps with a learned weight, normalised per head.
+
+    config.attention_type = "differential" builds it.  A head's hidden_size / num_attention_heads columns are 64 or 128: two maps of 32
+    or 64.  config.rotary, if set, is a dict of RotaryPositions' arguments (rotary_dim, base, interleaved, scaling): queries and keys
+    are then turned by their position in the sequence, which has no largest one.  Lengths are not limited to 512.  `depth` is the layer's
+    index: lambda starts at 0.8 - 0.6 exp(-0.3 depth)."""
+
+    def __init__(self, config, depth=0):
+        super(BertDifferentialSelfAttention, self).__init__(config)
+        if self.attention_head_size not in (64, 128):
+            raise UniterHipError("differential attention needs heads of 64 or 128 columns, got %d" % self.attention_head_size)
+        self.map_size = self.attention_head_size // 2
+        for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
+            setattr(self, name, nn.Parameter(torch.randn(self.num_attention_heads, self.map_size) * 0.1))
+        self.LayerNorm = HeadRMSNorm(self.attention_head_size)        # (the name keeps its weight out of the weight decay)
+        rotary = getattr(config, "rotary", None)
+        self.rotary = None if rotary is None else RotaryPositions(self.map_size, **rotary)
+        self.set_depth(depth)
+
+    def set_depth(self, depth):
+        self.lambda_init = 0.8 - 0.6 * math.exp(-0.3 * depth)
+
+    def lambdas(self):
+        return (self.lambda_q1, self.lambda_k1, self.lambda_q2, self.lambda_k2)
+
+    def forward(self, hidden_states, attention_mask=None, positions=None, cu_seqlens=None, max_len=None):
+        """hidden_states [B, L, H] with the additive mask [B, 1, 1, L] or [B, L] (None: no key is masked), or packed rows [T, H] with
+        cu_seqlens (int32 [examples + 1], device) and max_len.  positions: as ops.rotary takes them (default: 0 .. in every sequence)."""
+        return ops.bert_differential_self_attention(self, hidden_states, attention_mask, positions, cu_seqlens, max_len)
+
+
+ATTENTION_TYPES = {"softmax": BertSelfAttention, "differential": BertDifferentialSelfAttention}
+
+
 class BertSelfOutput(nn.Module):
     """Parameter holder of the attention output projection + LayerNorm (model/layer.py:104-115)."""
 
@@ -167,7 +213,12 @@ class BertSelfOutput(nn.Module):
 class BertAttention(nn.Module):
     def __init__(self, config):
         super(BertAttention, self).__init__()
-        self.self = BertSelfAttention(config)
+        kind = getattr(config, "attention_type", "softmax")
+        if kind not in ATTENTION_TYPES:
+            raise UniterHipError("attention_type must be one of %s, got %r" % (sorted(ATTENTION_TYPES), kind))
+        if kind == "softmax" and getattr(config, "rotary", None) is not None:
+            raise UniterHipError("rotary positions go with attention_type = 'differential' (softmax layers run the fused stack, which has learned positions)")
+        self.self = ATTENTION_TYPES[kind](config)
         self.output = BertSelfOutput(config)
 
     def forward(self, input_tensor, attention_mask):
@@ -208,10 +259,32 @@ def layer_dropouts(layer):
     return float(layer.output.dropout.p), float(layer.attention.self.dropout.p)
 
 
+def is_differential(layer):
+    return isinstance(layer.attention.self, BertDifferentialSelfAttention)
+
+
+def run_differential(layers, hidden_states, attention_mask=None, positions=None, cu_seqlens=None, max_len=None, output_all=False, hook=None):
+    """The layers of a differential encoder, one after the other: the fused stack runs softmax attention, so here every block is its own
+    autograd node (attention, output projection + LayerNorm, intermediate, output).  Gradients are complete on the compute stream when
+    backward() returns.  A reducer that counts on the fused stack's per-layer calls would wait for them in vain and is refused
+    (GradientReducer reduces such an encoder in finish())."""
+    if hook is not None and not isinstance(hook, ops.DeferWgradJoin):
+        raise UniterHipError("a per-layer gradient hook needs the fused stack (attention_type = 'softmax')")
+    outs, x = [], hidden_states
+    for lay in layers:
+        a = lay.attention.self(x, attention_mask, positions, cu_seqlens, max_len)
+        a = lay.attention.output(a, x)
+        x = lay.output(lay.intermediate(a), a)
+        outs.append(x)
+    return tuple(outs) if output_all else x
+
+
 def run_layers(layers, hidden_states, attention_mask, output_all=False, hook=None):
     """Shared entry of BertLayer.forward / UniterEncoder.forward."""
     layers = list(layers)
     first = layers[0]
+    if is_differential(first):
+        return run_differential(layers, hidden_states, ops.key_mask(attention_mask, hidden_states), output_all=output_all, hook=hook)
     cfg = dict(first._enc_cfg)
     p_h, p_a = layer_dropouts(first)
     for lay in layers[1:]:
@@ -231,6 +304,9 @@ def run_layers_packed(layers, hidden_states, cu_seqlens, n_examples, max_len, ou
     """Padding-free variant: hidden_states [T, H] holds only real tokens (see ops.encoder_forward_packed)."""
     layers = list(layers)
     first = layers[0]
+    if is_differential(first):
+        positions = ops.packed_positions(cu_seqlens, hidden_states.shape[0]) if first.attention.self.rotary is not None else None
+        return run_differential(layers, hidden_states, None, positions, cu_seqlens, max_len, output_all=output_all, hook=hook)
     cfg = dict(first._enc_cfg)
     p_h, p_a = layer_dropouts(first)
     for lay in layers[1:]:

@@ -20,7 +20,7 @@ import torch
 from torch import nn
 
 from .. import ops
-from .layer import run_layers_packed, BertLayer, BertLayerNorm, BertPooler, run_layers
+from .layer import run_layers_packed, BertLayer, BertLayerNorm, BertPooler, is_differential, run_layers
 
 logger = logging.getLogger(__name__)
 
@@ -220,6 +220,9 @@ class UniterEncoder(nn.Module):
         super().__init__()
         layer = BertLayer(config)
         self.layer = nn.ModuleList([copy.deepcopy(layer) for _ in range(config.num_hidden_layers)])
+        for depth, lay in enumerate(self.layer):
+            if is_differential(lay):
+                lay.attention.self.set_depth(depth)
         # optional callable(layer_index) fired during backward when a layer's gradients have been enqueued
         # (utils.distributed.GradientReducer uses it to overlap the allreduce with the rest of backward)
         self.grad_ready_hook = None

@@ -1155,6 +1155,108 @@ def differential_self_attention(qkv, heads, lambdas, lambda_init, norm_weight=No
     return _diff_apply(qkv, None, None, heads, checked, lambda_init, eps, p_drop)
 
 
+def key_mask(attention_mask, hidden_states):
+    """The additive key mask of dense hidden_states [B, L, H] as fp32 [B, L] (None stays None)."""
+    if attention_mask is None:
+        return None
+    B, L = hidden_states.shape[0], hidden_states.shape[1]
+    if attention_mask.numel() != B * L:
+        raise _lib.UniterHipError("attention_mask must have B*L elements (got %d for B=%d L=%d)" % (attention_mask.numel(), B, L))
+    return attention_mask.float().reshape(B, L)
+
+
+def packed_positions(cu_seqlens, total):
+    """int64 [total]: the position of every row inside its sequence (rows stored back to back; no synchronisation)."""
+    cu = cu_seqlens.to(torch.int64)
+    return torch.arange(total, device=cu.device) - torch.repeat_interleave(cu[:-1], cu.diff(), output_size=total)
+
+
+class _BertDiffAttentionFn(torch.autograd.Function):
+    """BertDifferentialSelfAttention.forward: fused [3H, H] projection, q | k turned in place, differential attention."""
+
+    @staticmethod
+    def forward(ctx, x, mask, positions, cu, max_len, att, p, keep, *anchor):
+        H = x.shape[-1]
+        T = x.numel() // H
+        xc = x.contiguous()
+        wqkv, bqkv = att.fused_qkv()
+        qkv = torch.empty((*x.shape[:-1], 3 * H), dtype=_BF16, device=x.device)
+        C.uniter_gemm_bias_fwd(ptr(xc), ptr(wqkv), ptr(bqkv), ptr(qkv), T, 3 * H, H, _lib.stream_ptr())
+        if att.rotary is not None:
+            qk = qkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
+            _rotary_launch(qk, qk, positions, 0, att.rotary, False)
+        seed, off = _next_offsets(1) if p > 0.0 else (0, 0)
+        cfg = (att.num_attention_heads, att.map_size, att.lambda_init, att.LayerNorm.eps, max_len, max_len, p, seed, off)
+        lams = [t.detach() for t in att.lambdas()]
+        out, stats, maps = _diff_forward(qkv, None, None, mask, cu, cu, cfg, att.LayerNorm.weight, lams, keep)
+        ctx.att, ctx.cfg = att, cfg
+        if keep:
+            ctx.save_for_backward(xc, qkv, mask, positions, cu, stats, maps, out)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        xc, qkv, mask, positions, cu, stats, maps, out = ctx.saved_tensors
+        att = ctx.att
+        H = xc.shape[-1]
+        T = xc.numel() // H
+        st = _lib.stream_ptr()
+        dqkv = (torch.empty if cu is None else torch.zeros)(qkv.shape, dtype=_BF16, device=qkv.device)
+        dl = [ensure_grad(t) if t.requires_grad else None for t in att.lambdas()]
+        w = att.LayerNorm.weight
+        dw = ensure_grad(w) if w.requires_grad else None
+        _diff_backward(qkv, None, None, mask, cu, cu, ctx.cfg, w, att.lambdas(), stats, maps, _rows16(dout), dqkv, None, None, dl, dw, True)
+        if att.rotary is not None:
+            dqk = dqkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
+            _rotary_launch(dqk, dqk, positions, 0, att.rotary, True)
+        wqkv, _ = att.fused_qkv()
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = torch.empty_like(xc)
+            C.uniter_gemm_dgrad(ptr(dqkv), ptr(wqkv), None, ptr(dx), T, 3 * H, H, st)
+        if any(m.weight.requires_grad for m in (att.query, att.key, att.value)):
+            gw, gb = att.fused_qkv_grad()
+            _wgrad_into(dqkv, xc, gw, gb, T, 3 * H, H)
+        return (dx,) + (None,) * (len(ctx.needs_input_grad) - 1)
+
+
+def bert_differential_self_attention(att, hidden_states, attention_mask=None, positions=None, cu_seqlens=None, max_len=None):
+    """model/layer.py::BertDifferentialSelfAttention.forward.  Parameter gradients are accumulated into `.grad`."""
+    _check_dev(hidden_states, "hidden_states")
+    packed = cu_seqlens is not None
+    if hidden_states.dim() != (2 if packed else 3) or hidden_states.shape[-1] != att.all_head_size:
+        raise _lib.UniterHipError("hidden_states must be %s, got %s" % ("[T, %d] with cu_seqlens" % att.all_head_size if packed else
+                                                                      "[B, L, %d]" % att.all_head_size, tuple(hidden_states.shape)))
+    if hidden_states.get_device() != torch._C._cuda_getDevice():
+        raise _lib.UniterHipError("hidden_states is on %s, which is not the current device" % (hidden_states.device,))
+    lin = (att.query, att.key, att.value)
+    prm = [m.weight for m in lin] + [m.bias for m in lin] + list(att.lambdas()) + [att.LayerNorm.weight]
+    _check_mod(prm, "attention parameter")
+    params_ready(*prm)
+    if packed:
+        _check_dev(cu_seqlens, "cu_seqlens", torch.int32)
+        if attention_mask is not None or max_len is None or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise _lib.UniterHipError("packed rows take cu_seqlens [examples + 1], max_len and no attention_mask")
+        cu_seqlens = cu_seqlens.contiguous()
+        if att.rotary is not None and positions is None:
+            positions = packed_positions(cu_seqlens, hidden_states.shape[0])
+    mask = key_mask(attention_mask, hidden_states)
+    if positions is not None:
+        rows = hidden_states.shape[:-1]
+        if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int64, torch.int32) or positions.device != hidden_states.device \
+                or (positions.shape != rows and positions.shape != rows[-1:]):
+            raise _lib.UniterHipError("positions must be an integer tensor %s or %s on %s" % (list(rows), list(rows[-1:]), hidden_states.device))
+        positions = positions.to(torch.int64).contiguous()
+    for t, what in ((mask, "attention_mask"), (cu_seqlens, "cu_seqlens")):
+        if t is not None and t.device != hidden_states.device:
+            raise _lib.UniterHipError("%s is on %s, hidden_states on %s" % (what, t.device, hidden_states.device))
+    track = torch.is_grad_enabled()
+    p = float(att.dropout.p) if (att.training and track) else 0.0
+    keep = track and (hidden_states.requires_grad or any(q.requires_grad for q in prm))
+    return _BertDiffAttentionFn.apply(hidden_states, mask, positions, cu_seqlens, max_len, att, p, keep, *_anchor(prm))
+
+
 # ----------------------------------------------------------------------------------------------------
 # LayerNorm (+ dropout on the output) as used by the embedding blocks
 # ----------------------------------------------------------------------------------------------------

@@ -41,7 +41,7 @@ def _ordered_parameters(model):
             for attr in ("weight", "bias"):
                 for lin in ("query", "key", "value"):
                     add("%s%s.%s" % (prefix, lin, attr), getattr(getattr(mod, lin), attr))
-            return
+            # (what else an attention module owns follows below: lambda vectors, a per-head norm)
         for n, p in mod._parameters.items():
             add(prefix + n, p)
         for n, child in mod._modules.items():

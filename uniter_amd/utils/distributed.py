@@ -253,6 +253,10 @@ class GradientReducer(object):
     def __init__(self, arena, encoder=None, layers_per_bucket=3, word_embeddings=None, word_ids_cap=None, single_launch=None):
         self.arena = arena
         self.word_compact = False             # tests: segment sums on the gathered rows even for a small vocabulary
+        if encoder is not None:
+            from ..model.layer import is_differential
+            if any(is_differential(lay) for lay in encoder.layer):
+                encoder = None                # layers run one by one, without the fused stack's per-layer calls: all is reduced in finish()
         self.word_ids_cap = word_ids_cap      # most word ids (batch x padded text length) any rank hands to finish(); None: agreed per step
         self.encoder = encoder
         self.buckets = []          # (lo, hi) element ranges
