@@ -131,6 +131,22 @@ def test_positions_forms_offsets_and_far_positions():
     close(ops.rotary(x, p1 - 12000, rot), turned(x, (p1 - 12000).expand(3, 11), rot), x, rot)       # before the origin
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("B,L,heads,dim,n", [(1, 3, 37, 64, 32), (2, 2, 9, 512, 512), (1, 2, 7, 384, 256), (1, 5, 11, 200, 16), (1, 2, 3, 520, 64)])
+def test_more_heads_than_a_wave_holds(B, L, heads, dim, n, interleaved):
+    rot = RotaryPositions(dim, rotary_dim=n, interleaved=interleaved)
+    g = torch.Generator().manual_seed(dim)
+    x = torch.randn(B, L, heads, dim, generator=g).to(BF16).cuda()
+    pos = torch.randint(0, 5000, (B, L), generator=g).cuda()
+    y = ops.rotary(x, pos, rot)
+    close(y, turned(x, pos, rot), x, rot)
+    guard = torch.full((B, L + 1, heads, dim + 8), 7.0, dtype=BF16, device="cuda")
+    view = guard[:, :L, :, :dim].copy_(x)
+    assert torch.equal(ops.rotary(view, pos, rot, out=view), y)                      # in place, between rows that stay as they were
+    assert (guard[:, L] == 7).all() and (guard[..., dim:] == 7).all()
+
+
 def turned_exact(x, pos, rot):
     """As turned(), with the angle reduced in whole-number arithmetic: far positions lose nothing."""
     from fractions import Fraction

@@ -8,10 +8,11 @@
 // in 32 bits position 131071 would already be off by 0.008 of a radian — with the product's own rounding error added back, so that no
 // position up to 2^53 loses anything; only the fraction goes to the 32-bit hardware sine and cosine, whose unit is the turn.
 //
-// What bounds it: HBM (4 bytes per element, ~1 flop).  One wave takes one token: lane = (head, chunk of 8 pairs), so a wave's loads
-// cover whole rows, and a lane's eight sines and cosines are formed once and serve every head it comes to (nj = chunks per head divides
-// the lanes into 64 / nj heads at a time).  No table is read: 8 angles per lane and token are ~60 vector instructions against the 128 to
-// 512 bytes that the lane moves.
+// What bounds it: HBM (4 bytes per element, ~1 flop).  One wave takes one token.  No table is read: a wave forms each pair's sine and
+// cosine once (half a dozen 64-bit instructions per pair) and hands them round through LDS.  Measured: 32749 tokens of 24 heads of 64, half
+// of each turned, 38.8 us (5.2 TB/s, a plain copy of that size takes 35 - 39); with a lane holding both halves of 8 pairs (32-byte
+// pieces of a row per load, each angle formed by every head's lanes) it was 52.7 us.  2848 tokens of 32 heads: 6 us, of which 3.5 are the
+// launch.  One token: 2 us in the kernel.
 #include "common.cuh"
 #include "kernels.h"
 #include "../../include/uniter_hip.h"
@@ -40,65 +41,80 @@ __device__ __forceinline__ void rot_angle(const RotArgs& p, const double pos, co
 
 // the token of this wave; false behind the last one
 __device__ __forceinline__ bool rot_row(const RotArgs& p, int64_t& xo, int64_t& yo, double& pos) {
-    const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= p.rows) return false;
-    const int64_t b = row / p.L, l = row - b * p.L;
+    const int64_t b = p.rows >> 32 ? row / p.L : (uint32_t)row / p.L, l = row - b * p.L;      // (the 64-bit division is ten times as long)
     xo = b * p.xb + l * p.xl;
     yo = b * p.yb + l * p.yl;
     pos = (double)(p.pos != nullptr ? p.pos[b * p.pos_b + l] + p.pos_offset : l + p.pos_offset);
     return true;
 }
 
-// 16-byte accesses: every head starts on 16 bytes and the turned part is whole chunks of 8 pairs
+// 16-byte accesses: every head starts on 16 bytes and the turned part is whole chunks of 8 pairs.  A lane takes one chunk of 8 elements of
+// a head, 64 / (dim / 8) heads side by side, so that loads and stores run over whole rows.  The half layout's partners sit in the lane
+// rot / 16 further on and come over a lane shuffle.
 template <bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
+    constexpr int N = 4;                                // heads in flight per lane
     int64_t xo, yo;
     double pos;
     if (!rot_row(p, xo, yo, pos)) return;
     const int lane = threadIdx.x & 63;
     const bf16_t* x = p.x + xo;
     bf16_t* y = p.y + yo;
-    const int nj = p.rot >> 4, hs = 64 / nj;            // chunks of 8 pairs per head; heads per pass
-    const int j = lane % nj, h0 = lane / nj;
-    const int oa = INTER ? 16 * j : 8 * j, ob = INTER ? 16 * j + 8 : p.rot / 2 + 8 * j;
-    if (h0 < hs && h0 < p.heads) {
-        u32x4 a = ldg16<false>(x + h0 * p.xh + oa), b = ldg16<false>(x + h0 * p.xh + ob);
-        float c[8], s[8];
+    const int nj = p.rot >> 4, nc = p.dim >> 3, hs = 64 / nc;      // chunks of the turned halves and of a head; heads per pass
+    const int h0 = lane / nc, ch = lane - h0 * nc;
+    const bool turned = ch < 2 * nj, mine = h0 < hs && (turned || p.copy);
+    x += ch * 8;
+    y += ch * 8;
+    u32x4 in[N] = {};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) rot_angle(p, pos, 8 * j + e, c[e], s[e]);
-        for (int h = h0; h < p.heads; h += hs) {
-            const u32x4 a0 = a, b0 = b;
-            if (h + hs < p.heads) {                     // the next head's loads leave before this one's arithmetic
-                a = ldg16<false>(x + (h + hs) * p.xh + oa);
-                b = ldg16<false>(x + (h + hs) * p.xh + ob);
-            }
-            float u[8], v[8], fu[8], fv[8];
-            unpack8(a0, u);
-            unpack8(b0, v);
-            if constexpr (INTER) {                      // pairs sit side by side: four in each piece
+    for (int i = 0; i < N; ++i)
+        if (const int h = h0 + i * hs; mine && h < p.heads) in[i] = ldg16<false>(x + h * p.xh);
+    // every pair's cosine and sine once per token, passed round through the wave's own piece of LDS (no other wave touches it)
+    extern __shared__ __attribute__((aligned(16))) float rot_lds[];
+    float* const cs = rot_lds + (threadIdx.x >> 6) * p.rot;
+    const int np = p.rot >> 1;
+    for (int i = lane; i < np; i += 64) rot_angle(p, pos, i, cs[i], cs[np + i]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    constexpr int W = INTER ? 4 : 8;                    // pairs that this lane's chunk has a part in
+    const int pair = turned ? (INTER ? 4 * ch : 8 * (ch < nj ? ch : ch - nj)) : 0;
+    const float sgn = !INTER && ch < nj ? -1.f : 1.f;
+    const int mate = lane + (ch < nj ? nj : -nj);
+    float c[W], s[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        c[e] = turned ? cs[pair + e] : 1.f;
+        s[e] = turned ? cs[np + pair + e] * sgn : 0.f;
+    }
+    for (int base = 0; base < p.heads; base += N * hs) {           // (the same for every lane: all take part in the shuffles)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (base + i * hs >= p.heads) break;
+            const int h = base + h0 + i * hs;
+            const bool live = mine && h < p.heads;
+            const u32x4 v = in[i];
+            if (const int n = h + N * hs; mine && n < p.heads) in[i] = ldg16<false>(x + n * p.xh);
+            float u[8], f[8];
+            unpack8(v, u);
+            if constexpr (INTER) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    fu[2 * e] = u[2 * e] * c[e] - u[2 * e + 1] * s[e];
-                    fu[2 * e + 1] = u[2 * e + 1] * c[e] + u[2 * e] * s[e];
-                    fv[2 * e] = v[2 * e] * c[4 + e] - v[2 * e + 1] * s[4 + e];
-                    fv[2 * e + 1] = v[2 * e + 1] * c[4 + e] + v[2 * e] * s[4 + e];
+                    f[2 * e] = u[2 * e] * c[e] - u[2 * e + 1] * s[e];
+                    f[2 * e + 1] = u[2 * e + 1] * c[e] + u[2 * e] * s[e];
                 }
             } else {
+                u32x4 o;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    fu[e] = u[e] * c[e] - v[e] * s[e];
-                    fv[e] = v[e] * c[e] + u[e] * s[e];
-                }
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_amdgcn_ds_bpermute(mate << 2, v[e]);
+                float w[8];
+                unpack8(o, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = u[e] * c[e] + w[e] * s[e];
             }
-            out_store16(y + h * p.yh + oa, pack8(fu));
-            out_store16(y + h * p.yh + ob, pack8(fv));
-        }
-    }
-    if (p.copy) {
-        const int nr = (p.dim - p.rot) >> 3;            // chunks of 8 elements per head that are not turned
-        for (int e = lane; e < p.heads * nr; e += 64) {
-            const int h = e / nr, c = e - h * nr;
-            out_store16(y + h * p.yh + p.rot + c * 8, ldg16<false>(x + h * p.xh + p.rot + c * 8));
+            // plain stores: 2 microseconds of 53 faster than non-temporal ones for 32749 tokens of 24 heads
+            if (live) *(gmem_u32x4*)(y + h * p.yh) = turned ? pack8(f) : v;
         }
     }
 }
@@ -165,12 +181,13 @@ extern "C" int uniter_rotary(const UniterRotary* r, const void* x, const int64_t
     UH_CHECK_ARG(same || x != y, "in place needs y's strides to be x's");
     p.copy = !same && p.dim > p.rot;
     const int64_t all = p.xb | p.xl | p.xh | p.yb | p.yl | p.yh | (p.copy ? p.dim : 0);
-    const bool wide = p.rot % 16 == 0 && all % 8 == 0 && (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
+    const bool wide = p.dim % 8 == 0 && p.dim <= 512 && p.rot % 16 == 0 && all % 8 == 0 && (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
     const hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)blocks), block(rows < 4 ? 64 * (unsigned)rows : 256);
+    const unsigned lds = (block.x >> 6) * (unsigned)p.rot * sizeof(float);      // at most 4 * 512 * 4 bytes
     if (wide) {
-        if (r->interleaved) hipLaunchKernelGGL(rotary_kernel<true>, grid, block, 0, st, p);
-        else hipLaunchKernelGGL(rotary_kernel<false>, grid, block, 0, st, p);
+        if (r->interleaved) hipLaunchKernelGGL(rotary_kernel<true>, grid, block, lds, st, p);
+        else hipLaunchKernelGGL(rotary_kernel<false>, grid, block, lds, st, p);
     } else {
         if (r->interleaved) hipLaunchKernelGGL(rotary_any_kernel<true>, grid, block, 0, st, p);
         else hipLaunchKernelGGL(rotary_any_kernel<false>, grid, block, 0, st, p);

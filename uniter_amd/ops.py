@@ -1191,13 +1191,13 @@ class _BertDiffAttentionFn(torch.autograd.Function):
         out, stats, maps = _diff_forward(qkv, None, None, mask, cu, cu, cfg, att.LayerNorm.weight, lams, keep)
         ctx.att, ctx.cfg = att, cfg
         if keep:
-            ctx.save_for_backward(xc, qkv, mask, positions, cu, stats, maps, out)
+            ctx.save_for_backward(xc, qkv, mask, positions, cu, stats, maps)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        xc, qkv, mask, positions, cu, stats, maps, out = ctx.saved_tensors
+        xc, qkv, mask, positions, cu, stats, maps = ctx.saved_tensors
         att = ctx.att
         H = xc.shape[-1]
         T = xc.numel() // H
