@@ -62,6 +62,9 @@ def test_cpu_tensors_and_bad_c_arguments_are_refused():
     r.head_dim, r.B = 64, 0
     assert lib.uniter_rotary(ctypes.byref(r), None, s, None, s, None) == 0           # nothing to do
     r.B, r.freq = 1, 8
+    r.L = 1 << 27
+    assert lib.uniter_rotary(ctypes.byref(r), 64, s, 64, s, None) < 0 and b"too many" in lib.uniter_hip_last_error()
+    r.L = 1
     t = (ctypes.c_int64 * 3)(64, 64, 128)
     assert lib.uniter_rotary(ctypes.byref(r), 64, s, 64, t, None) < 0 and b"in place" in lib.uniter_hip_last_error()
 
@@ -195,7 +198,8 @@ def test_refusals():
                 lambda: ops.rotary(x[0], None, rot), lambda: ops.rotary(x, torch.zeros(4, dtype=torch.int64, device="cuda"), rot),
                 lambda: ops.rotary(x, torch.zeros(3, device="cuda"), rot), lambda: ops.rotary(x, torch.zeros(3, dtype=torch.int64), rot),
                 lambda: ops.rotary(x.clone().requires_grad_(True), None, rot, out=x), lambda: ops.rotary(x, None, rot, out=x[:1]),
-                lambda: ops.rotary(x[:, :2], None, rot, out=x[:, 1:])):
+                lambda: ops.rotary(x[:, :2], None, rot, out=x[:, 1:]), lambda: ops.rotary(x, None, rot, out=x[:1].expand(2, 3, 4, 64)),
+                lambda: ops.rotary(x[:, :1].expand(2, 3, 4, 64), None, rot, out=x[:, :1].expand(2, 3, 4, 64))):
         with pytest.raises(_lib.UniterHipError):
             bad()
 

@@ -162,7 +162,7 @@ extern "C" int uniter_rotary(const UniterRotary* r, const void* x, const int64_t
     UH_CHECK_ARG(r->B <= ((int64_t)1 << 40) / r->L, "too many tokens");
     const int64_t rows = r->B * r->L;
     const int64_t blocks = (rows + 3) / 4;
-    UH_CHECK_ARG(blocks < ((int64_t)1 << 31), "too many tokens for one launch");
+    UH_CHECK_ARG(blocks < ((int64_t)1 << 24), "too many tokens for one launch");           // (a launch has fewer than 2^32 threads)
     RotArgs p;
     p.x = (const bf16_t*)x;
     p.y = (bf16_t*)y;
