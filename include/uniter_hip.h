@@ -640,7 +640,7 @@ int uniter_rotary(const UniterRotary* r, const void* x, const int64_t* x_strides
  * lambda_*: bf16, [heads, d] (lambda_per_head != 0) or [d] for all heads; norm_weight bf16 [2 d].
  * Dropout keeps or drops elements of the difference (one draw for both maps), stream as in the header's conventions.
  * For a backward pass the forward keeps stats [B, heads, Lq, 4] and maps [rows, heads, 2, 2 d], both fp32 (rows = B Lq, or total_q);
- * both NULL: nothing is kept. */
+ * both NULL: nothing is kept.  Where there are no query rows (or no key rows) at all, their pointers may be NULL. */
 typedef struct UniterDiffAttention {
     const void *q, *k, *v;
     int64_t q_row, k_row, v_row;          /* row strides, multiples of 8 */
@@ -652,7 +652,7 @@ typedef struct UniterDiffAttention {
     const void *lambda_q1, *lambda_k1, *lambda_q2, *lambda_k2;
     const void* norm_weight;
     int64_t B, Lq, Lk, heads, head_dim;
-    float lambda_init, norm_eps, p_drop;
+    float lambda_init, norm_eps, p_drop;  /* norm_eps > 0 */
     int32_t lambda_per_head;
     uint64_t seed, offset;
 } UniterDiffAttention;

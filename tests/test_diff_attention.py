@@ -291,6 +291,40 @@ def test_empty_sizes():
 
 
 @pytest.mark.gpu
+def test_packed_batches_without_rows():
+    """A batch of empty examples, and examples without keys, whose tensors have no memory at all."""
+    lams, w = params(torch.Generator().manual_seed(1), 2, 32)
+    none, cu0 = torch.empty(0, 128, dtype=BF16, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 4, 9], dtype=torch.int32, device="cuda")
+    x = torch.randn(9, 128).to(BF16).cuda()
+    for q, k, cq, ck in ((none, none, cu0, cu0), (x, none, cu, cu0), (none, x, cu0, cu)):
+        out, grads = run_all(q, k, k, 2, lams, 0.5, w, q, cu_seqlens=cq, cu_seqlens_k=ck, max_len=5, max_len_k=5)
+        assert out.shape == q.shape and not out.any()
+        assert all(not t.any() for t in grads.values()) and grads["k"].shape == k.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,Lq,Lk", [(32, 1, 5000), (64, 130, 700), (32, 300, 300)])
+def test_no_key_left_among_many(dim, Lq, Lk):
+    """Example 0 has no key at all, example 1 its very last one only, example 2 its first: many tiles (and splits) with nothing in them."""
+    g = torch.Generator().manual_seed(Lk)
+    H = 2 * 2 * dim
+    q, k, v, dy = (torch.randn(3, n, H, generator=g).to(BF16).cuda() for n in (Lq, Lk, Lk, Lq))
+    k[0], v[0] = math.nan, math.inf                                        # never used
+    bias = torch.full((3, Lk), -math.inf).cuda()
+    bias[1, -1], bias[2, 0] = 0.0, 0.0
+    lams, w = params(g, 2, dim)
+    out, grads = run_all(q, k, v, 2, lams, 0.5, w, dy, mask_bias=bias)
+    want = whole(q, k.nan_to_num(0.0), v.nan_to_num(0.0, 0.0), 2, lams, 0.5, w, 1e-5, bias.cpu(), dy=dy)
+    assert not out[0].any() and not grads["q"][0].any() and not grads["k"][0].any() and not grads["v"][0].any()
+    for n in ("out", "q", "k", "v"):
+        value, bound = want[n]
+        got = (out if n == "out" else grads[n]).cpu().double()
+        over = (got - value).abs() - bound - U * value.abs() - 1e-30
+        assert (over <= 0).all(), (n, float(over.max()))
+
+
+@pytest.mark.gpu
 def test_strides_and_alignment():
     g = torch.Generator().manual_seed(9)
     heads, dim, B, L = 2, 32, 2, 45
@@ -607,6 +641,30 @@ def test_bad_c_arguments_are_refused():
     assert lib.uniter_diff_attention_fwd(ctypes.byref(args(B=0)), None, 0, 0, None, None, None, 0, None) == 0
 
 
+def test_bad_c_arguments_of_empty_calls_are_refused():
+    """Key rows without query rows: dK and dV are written (zeros), so k, v and their gradients have to be there."""
+    import ctypes
+    lib = _lib.load()
+    a, g = _lib.UniterDiffAttention(), _lib.UniterDiffAttentionGrads()
+    a.lambda_q1 = a.lambda_k1 = a.lambda_q2 = a.lambda_k2 = 4096
+    a.B = a.heads = a.Lk = 1
+    a.head_dim, a.k_row, a.v_row, g.k_row, g.v_row, g.k, g.v = 32, 64, 64, 64, 64, 4096, 4096
+
+    def bwd():
+        n = lib.uniter_diff_attention_bwd_workspace_bytes(ctypes.byref(a))
+        return lib.uniter_diff_attention_bwd(ctypes.byref(a), None, None, None, 0, 0, ctypes.byref(g), 4096, n, None), lib.uniter_hip_last_error()
+
+    assert bwd()[0] < 0 and b"null" in bwd()[1]                            # k and v missing
+    a.k = a.v = 4096
+    g.v = None
+    assert bwd()[0] < 0 and b"null" in bwd()[1]
+    a.Lq, a.q, a.q_row, a.norm_weight = 1, 4096, 64, 4096                  # an eps of 0 with a norm: a row of zeros would be 0 / 0
+    assert lib.uniter_diff_attention_fwd(ctypes.byref(a), 4096, 64, 0, None, None, None, 0, None) < 0
+    assert b"norm_eps" in lib.uniter_hip_last_error()
+    a.norm_weight, a.cu_seqlens_q, a.cu_seqlens_k, a.q, a.k = None, 4096, 4096, None, None
+    assert lib.uniter_diff_attention_fwd(ctypes.byref(a), None, 64, 0, None, None, None, 0, None) == 0        # no rows at all
+
+
 def test_cpu_tensors_are_refused():
     t, l = torch.zeros(1, 2, 64, dtype=BF16), torch.zeros(1, 32, dtype=BF16)
     with pytest.raises(_lib.UniterHipError, match="CUDA"):
@@ -632,6 +690,8 @@ def test_refusals():
                 lambda: f(q, k.cpu(), k, 2, lam, 0.5), lambda: ops.differential_self_attention(q, 2, lam, 0.5)):
         with pytest.raises(_lib.UniterHipError):
             bad()
+    with pytest.raises(_lib.UniterHipError, match="eps"):
+        f(q, k, k, 2, lam, 0.5, norm_weight=w, eps=0.0)
     x = q.clone().requires_grad_(True)
     first, = torch.autograd.grad(f(x, k, k, 2, lam, 0.5), x, q, create_graph=True)
     with pytest.raises(RuntimeError):                                       # no second derivative

@@ -429,6 +429,7 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const Di
     pin(f.qf[1]);
 
     if (t0 < t1) kt.finish(t0);
+    else dma_wait();                     // (a first tile whose keys are all out is on its way to LDS all the same)
     for (int t = t0; t < t1; ++t) {
         const bool general = kt.mk.general;
         const int subs = idle || kt.mk.out == ~0ull ? 0 : min(2, (sk.n - t * KT + 31) >> 5);
@@ -807,6 +808,7 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
     float c_lse[2] = {m[0] + ll[0], m[1] + ll[1]};
     asm volatile("" : "+v"(c_lse[0]), "+v"(c_lse[1]), "+v"(Dq[0]), "+v"(Dq[1]));
     if (nt > 0) kt.finish(0);
+    else dma_wait();
 
     for (int t = 0; t < nt; ++t) {
         const bool general = kt.mk.general, none = kt.mk.out == ~0ull;
@@ -1111,6 +1113,7 @@ int check(const UniterDiffAttention* a) {
     UH_CHECK_ARG(a->cu_seqlens_q == nullptr || a->mask_bias == nullptr, "packed rows take no mask");
     UH_CHECK_ARG(a->total_q >= 0 && a->total_k >= 0, "bad row count");
     UH_CHECK_ARG(a->p_drop >= 0.f && a->p_drop < 1.f, "dropout probability must be in [0,1)");
+    UH_CHECK_ARG(a->norm_weight == nullptr || a->norm_eps > 0.f, "norm_eps must be positive");
     UH_CHECK_ARG(a->q_row % 8 == 0 && a->k_row % 8 == 0 && a->v_row % 8 == 0 && a->q_batch % 8 == 0 && a->k_batch % 8 == 0 && a->v_batch % 8 == 0,
                  "row and batch strides must be multiples of 8 elements");
     UH_CHECK_ARG(a->q_row >= 0 && a->k_row >= 0 && a->v_row >= 0 && a->q_row < (1 << 24) && a->k_row < (1 << 24) && a->v_row < (1 << 24),
@@ -1118,9 +1121,13 @@ int check(const UniterDiffAttention* a) {
     UH_CHECK_ARG(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->norm_weight), "q, k, v and norm_weight must be 16-byte aligned");
     UH_CHECK_ARG(a->lambda_q1 && a->lambda_k1 && a->lambda_q2 && a->lambda_k2, "null pointer");
     const int64_t blocks = a->B * a->heads * ((a->Lq > a->Lk ? a->Lq : a->Lk) / 32 + 1);
-    UH_CHECK_ARG(blocks < ((int64_t)1 << 31), "too many tokens for one launch");
+    UH_CHECK_ARG(blocks < ((int64_t)1 << 25), "too many tokens for one launch");           // (a launch has fewer than 2^32 threads)
     return 0;
 }
+
+// whether there are query / key rows at all
+bool has_queries(const UniterDiffAttention* a) { return a->B > 0 && a->Lq > 0 && (a->cu_seqlens_q == nullptr || a->total_q > 0); }
+bool has_keys(const UniterDiffAttention* a) { return a->B > 0 && a->Lk > 0 && (a->cu_seqlens_k == nullptr || a->total_k > 0); }
 
 DiffArgs args_of(const UniterDiffAttention* a) {
     DiffArgs p{};
@@ -1263,14 +1270,14 @@ int launch_bwd(const DiffArgs& p, const BwdSpace& s, const ParamGrads& g, hipStr
 extern "C" {
 
 size_t uniter_diff_attention_fwd_workspace_bytes(const UniterDiffAttention* a) {
-    return check(a) || a->B == 0 || a->Lq == 0 ? 0 : fwd_space(a, splits_for(a));
+    return check(a) || !has_queries(a) ? 0 : fwd_space(a, splits_for(a));
 }
 
 int uniter_diff_attention_fwd(const UniterDiffAttention* a, void* out, int64_t out_row, int64_t out_batch, float* stats, float* maps,
                               void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check(a)) return rc;
-    if (a->B == 0 || a->Lq == 0) return 0;
-    UH_CHECK_ARG(a->q && out && (a->Lk == 0 || (a->k && a->v)), "null pointer");
+    if (!has_queries(a)) return 0;
+    UH_CHECK_ARG(a->q && out && (!has_keys(a) || (a->k && a->v)), "null pointer");
     UH_CHECK_ARG(aligned16(out) && aligned16(stats) && aligned16(maps), "out, stats and maps must be 16-byte aligned");
     UH_CHECK_ARG(out_row % 8 == 0 && out_batch % 8 == 0, "row and batch strides must be multiples of 8 elements");
     UH_CHECK_ARG((stats == nullptr) == (maps == nullptr), "stats and maps are kept together, or neither");
@@ -1292,9 +1299,8 @@ int uniter_diff_attention_bwd(const UniterDiffAttention* a, const float* stats, 
     if (const int rc = check(a)) return rc;
     UH_CHECK_ARG(g != nullptr, "null pointer");
     UH_CHECK_ARG((a->norm_weight != nullptr) || g->norm_weight == nullptr, "a gradient of norm_weight needs norm_weight");
-    const bool any = a->B > 0 && a->Lq > 0;
-    UH_CHECK_ARG(!any || (a->q && stats && maps && dout && g->q && (a->Lk == 0 || (a->k && a->v))), "null pointer");
-    UH_CHECK_ARG(a->B == 0 || a->Lk == 0 || (g->k && g->v), "null pointer");
+    UH_CHECK_ARG(!has_queries(a) || (a->q && stats && maps && dout && g->q), "null pointer");
+    UH_CHECK_ARG(!has_keys(a) || (a->k && a->v && g->k && g->v), "null pointer");
     UH_CHECK_ARG(aligned16(stats) && aligned16(maps) && aligned16(dout) && aligned16(g->q) && aligned16(g->k) && aligned16(g->v) && aligned16(workspace),
                  "tensors must be 16-byte aligned");
     UH_CHECK_ARG(dout_row >= 0 && dout_row < (1 << 24), "row strides must be 0 .. 2^24 elements");

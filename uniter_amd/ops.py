@@ -956,6 +956,8 @@ def rotary(x, positions, rot, offset=0, out=None):
         _check_same_device(x, "x", ((out, "out"),))
         if out.shape != x.shape or out.stride(-1) != 1:
             raise _lib.UniterHipError("rotary: out must have x's shape and contiguous heads")
+        if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+            raise _lib.UniterHipError("rotary: out must not be a broadcast view")
         if out.numel() and (out.data_ptr() != x.data_ptr() or out.stride() != x.stride()) \
                 and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() and _overlap(out, x):
             raise _lib.UniterHipError("rotary: out overlaps x without being x")
@@ -1062,7 +1064,7 @@ class _DiffAttentionFn(torch.autograd.Function):
         return (dq, dk, dv, None, None, None, None, dweight, *dlams)
 
 
-def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, p_drop):
+def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, eps, p_drop):
     """What both calls ask of their arguments (k, v None: q is a fused projection); (dim, mask, cu_q, cu_k, max_q, max_k, lams, weight)."""
     fused = k is None
     H, odd = divmod(q.shape[-1], 3) if fused else (q.shape[-1], 0)
@@ -1091,6 +1093,8 @@ def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, p_
         if weight.shape != (2 * dim,):
             raise _lib.UniterHipError("norm_weight must be [%d], got %s" % (2 * dim, tuple(weight.shape)))
         weight = _rows16(weight)
+        if not eps > 0.0:
+            raise _lib.UniterHipError("eps must be positive, got %r" % (eps,))
     if not 0.0 <= p_drop < 1.0:
         raise _lib.UniterHipError("dropout probability must be in [0, 1), got %r" % (p_drop,))
     if packed:
@@ -1142,8 +1146,10 @@ def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=Non
     mask_bias: fp32 [B, Lk], added to the scores; -inf removes a key for good, and a row without keys is zeros.
     Packed rows: q [T, ..], k / v [Tk, ..], cu_seqlens int32 [examples + 1] on the device and max_len (a longest example's length, host
     int); cu_seqlens_k / max_len_k where the keys' differ.  Rows of no example come back as zeros.
-    p_drop: dropout on the difference of the maps (callers pass 0 in evaluation).  Gradients flow to q, k, v, lambdas and norm_weight."""
-    checked = _diff_check(q, k, v, heads, lambdas, norm_weight, mask_bias, cu_seqlens, cu_seqlens_k, max_len, max_len_k, p_drop)
+    p_drop: dropout on the difference of the maps (callers pass 0 in evaluation).  Gradients flow to q, k, v, lambdas and norm_weight.
+    Both passes can be captured into a graph; as with any operator, release eager autograd graphs of the same leaves before capturing a
+    backward pass."""
+    checked = _diff_check(q, k, v, heads, lambdas, norm_weight, mask_bias, cu_seqlens, cu_seqlens_k, max_len, max_len_k, eps, p_drop)
     return _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop)
 
 
@@ -1151,7 +1157,7 @@ def differential_self_attention(qkv, heads, lambdas, lambda_init, norm_weight=No
                                 eps=1e-5, p_drop=0.0):
     """differential_attention on a fused projection qkv [B, L, 3 H] (or packed [T, 3 H]), H = heads * 2 d: the q | k | v layout that
     BertSelfAttention.fused_qkv produces.  Its gradient is one [.., 3 H] tensor too."""
-    checked = _diff_check(qkv, None, None, heads, lambdas, norm_weight, mask_bias, cu_seqlens, None, max_len, None, p_drop)
+    checked = _diff_check(qkv, None, None, heads, lambdas, norm_weight, mask_bias, cu_seqlens, None, max_len, None, eps, p_drop)
     return _diff_apply(qkv, None, None, heads, checked, lambda_init, eps, p_drop)
 
 
@@ -1221,6 +1227,19 @@ class _BertDiffAttentionFn(torch.autograd.Function):
         return (dx,) + (None,) * (len(ctx.needs_input_grad) - 1)
 
 
+def tune_layer_gemms(cfg_like, hidden_states, training):
+    """Tile choices for the GEMMs of layers that run one by one, as encoder_forward makes them for its own: the shape's, or for packed
+    rows and lengths beyond the softmax stack's the next power of two's."""
+    rows = hidden_states.numel() // hidden_states.shape[-1]
+    if rows == 0:
+        return
+    if hidden_states.dim() == 3 and hidden_states.shape[1] <= 512:
+        B, L = hidden_states.shape[0], hidden_states.shape[1]
+    else:
+        B, L = max((1 << max(rows - 1, 1).bit_length()) // 64, 1), 64
+    _maybe_autotune(_shape(dict(cfg_like, heads=cfg_like["H"] // 64, p_hidden=0.0, p_attn=0.0), B, L, training), training)
+
+
 def bert_differential_self_attention(att, hidden_states, attention_mask=None, positions=None, cu_seqlens=None, max_len=None):
     """model/layer.py::BertDifferentialSelfAttention.forward.  Parameter gradients are accumulated into `.grad`."""
     _check_dev(hidden_states, "hidden_states")
@@ -1242,6 +1261,8 @@ def bert_differential_self_attention(att, hidden_states, attention_mask=None, po
         if att.rotary is not None and positions is None:
             positions = packed_positions(cu_seqlens, hidden_states.shape[0])
     mask = key_mask(attention_mask, hidden_states)
+    if positions is not None and att.rotary is None:
+        raise _lib.UniterHipError("positions are given, but this attention has no rotary positions (config.rotary)")
     if positions is not None:
         rows = hidden_states.shape[:-1]
         if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int64, torch.int32) or positions.device != hidden_states.device \
