@@ -175,14 +175,18 @@ class BertDifferentialSelfAttention(BertSelfAttention):
             raise UniterHipError("differential attention needs heads of 64 or 128 columns, got %d" % self.attention_head_size)
         self.map_size = self.attention_head_size // 2
         for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
-            setattr(self, name, nn.Parameter(torch.randn(self.num_attention_heads, self.map_size) * 0.1))
+            setattr(self, name, nn.Parameter(torch.empty(self.num_attention_heads, self.map_size)))
         self.LayerNorm = HeadRMSNorm(self.attention_head_size)        # (the name keeps its weight out of the weight decay)
         rotary = getattr(config, "rotary", None)
         self.rotary = None if rotary is None else RotaryPositions(self.map_size, **rotary)
-        self.set_depth(depth)
+        self.reset_lambda(depth)
 
-    def set_depth(self, depth):
+    def reset_lambda(self, depth):
+        """A layer of index `depth` before training: its lambda_init, and lambda vectors drawn from N(0, 0.1)."""
         self.lambda_init = 0.8 - 0.6 * math.exp(-0.3 * depth)
+        with torch.no_grad():
+            for t in self.lambdas():
+                t.normal_(0.0, 0.1)
 
     def lambdas(self):
         return (self.lambda_q1, self.lambda_k1, self.lambda_q2, self.lambda_k2)
@@ -270,6 +274,7 @@ def run_differential(layers, hidden_states, attention_mask=None, positions=None,
     (GradientReducer reduces such an encoder in finish())."""
     if hook is not None and not isinstance(hook, ops.DeferWgradJoin):
         raise UniterHipError("a per-layer gradient hook needs the fused stack (attention_type = 'softmax')")
+    ops.tune_layer_gemms(layers[0]._enc_cfg, hidden_states, layers[0].training)
     outs, x = [], hidden_states
     for lay in layers:
         a = lay.attention.self(x, attention_mask, positions, cu_seqlens, max_len)

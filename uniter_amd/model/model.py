@@ -222,7 +222,7 @@ class UniterEncoder(nn.Module):
         self.layer = nn.ModuleList([copy.deepcopy(layer) for _ in range(config.num_hidden_layers)])
         for depth, lay in enumerate(self.layer):
             if is_differential(lay):
-                lay.attention.self.set_depth(depth)
+                lay.attention.self.reset_lambda(depth)
         # optional callable(layer_index) fired during backward when a layer's gradients have been enqueued
         # (utils.distributed.GradientReducer uses it to overlap the allreduce with the rest of backward)
         self.grad_ready_hook = None
