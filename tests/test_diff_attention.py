@@ -687,7 +687,10 @@ def test_refusals():
                 lambda: f(q[0], k[0], k[0], 2, lam, 0.5, cu_seqlens=cu.long(), max_len=3), lambda: f(q[0], k[0], k[0], 2, lam, 0.5),
                 lambda: f(q[0], k[0], k[0], 2, lam, 0.5, cu_seqlens_k=cu, max_len=3),
                 lambda: f(q[0], k[0], k[0], 2, lam, 0.5, cu_seqlens=cu, max_len=3, mask_bias=torch.zeros(1, 3, device="cuda")),
-                lambda: f(q, k.cpu(), k, 2, lam, 0.5), lambda: ops.differential_self_attention(q, 2, lam, 0.5)):
+                lambda: f(q, k.cpu(), k, 2, lam, 0.5), lambda: f(q, k, None, 2, lam, 0.5), lambda: f(q, None, None, 2, lam, 0.5),
+                lambda: f(q, k, k, 2, (l, l, l, l.cpu()), 0.5), lambda: f(q, k, k, 2, lam, 0.5, norm_weight=w.float()),
+                lambda: f(q, k, k, 2, lam, 0.5, mask_bias=torch.zeros(2, 4)),
+                lambda: f(q, k, k, 2, lam, 0.5, mask_bias=torch.zeros(2, 1, 3, 4, device="cuda")), lambda: ops.differential_self_attention(q, 2, lam, 0.5)):
         with pytest.raises(_lib.UniterHipError):
             bad()
     with pytest.raises(_lib.UniterHipError, match="eps"):

@@ -899,7 +899,7 @@ def _rotary_launch(x, y, positions, offset, rot, inverse):
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, offset, rot):
-        y = torch.empty(x.shape, dtype=_BF16, device=x.device)
+        y = x.new_empty(x.shape)
         _rotary_launch(x, y, positions, offset, rot, False)
         ctx.offset, ctx.rot = offset, rot
         ctx.save_for_backward(positions)
@@ -910,7 +910,7 @@ class _RotaryFn(torch.autograd.Function):
     def backward(ctx, dy):
         positions, = ctx.saved_tensors
         dy = dy if dy.stride(-1) == 1 or dy.numel() == 0 else dy.contiguous()
-        dx = torch.empty(dy.shape, dtype=_BF16, device=dy.device)
+        dx = dy.new_empty(dy.shape)
         _rotary_launch(dy, dx, positions, ctx.offset, ctx.rot, True)
         return dx, None, None, None
 
@@ -948,7 +948,7 @@ def rotary(x, positions, rot, offset=0, out=None):
     if out is None:
         if x.requires_grad and torch.is_grad_enabled():
             return _RotaryFn.apply(x, positions, int(offset), rot)
-        out = torch.empty(x.shape, dtype=_BF16, device=x.device)
+        out = x.new_empty(x.shape)
     else:
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise _lib.UniterHipError("rotary: out= writes outside autograd; call it without gradients or let it return a new tensor")
@@ -1007,25 +1007,28 @@ def _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams):
 
 
 def _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, keep):
-    """(out, stats, maps), launched on the current stream; stats / maps only when a backward pass will want them."""
+    """(out, saved), launched on the current stream; saved (fp32: both maps' outputs, then the rows' statistics) only when a backward pass
+    will want it."""
     a = _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams)
     H = a.heads * 2 * a.head_dim
     # rows of a packed batch that belong to no example are not written: they are zeros
-    out = (torch.empty if cu_q is None else torch.zeros)((*q.shape[:-1], H), dtype=_BF16, device=q.device)
-    stats = maps = ws = None
+    out = (q.new_empty if cu_q is None else q.new_zeros)((*q.shape[:-1], H))
+    saved = maps = stats = ws = None
     if keep:
-        stats = torch.empty(a.B * a.heads * a.Lq * 4, dtype=torch.float32, device=q.device)
-        maps = torch.empty(out.numel() * 2, dtype=torch.float32, device=q.device)
+        n = out.numel() * 2
+        saved = q.new_empty(n + a.B * a.heads * a.Lq * 4, dtype=torch.float32)
+        maps = saved.data_ptr()
+        stats = maps + 4 * n
     ref = ctypes.byref(a)
     n = C.uniter_diff_attention_fwd_workspace_bytes(ref)
     if n:
         # (workspaces come from the caching allocator, not a shared scratch buffer: other streams and captured graphs get their own)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-    _launch_on(q, C.uniter_diff_attention_fwd, ref, out.data_ptr(), H, out.stride(0), ptr(stats), ptr(maps), ptr(ws), n)
-    return out, stats, maps
+        ws = q.new_empty(n, dtype=torch.uint8)
+    _launch_on(q, C.uniter_diff_attention_fwd, ref, out.data_ptr(), H, out.stride(0), stats, maps, ptr(ws), n)
+    return out, saved
 
 
-def _diff_backward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, stats, maps, dout, dq, dk, dv, dlams, dweight, accumulate):
+def _diff_backward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, saved, dout, dq, dk, dv, dlams, dweight, accumulate):
     """dq / dk / dv: tensors like q / k / v (one [.., 3 H] tensor and None, None for a fused projection)."""
     a = _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams)
     ptrs, rows, batches = _qkv_of(dq, dk, dv)
@@ -1033,8 +1036,9 @@ def _diff_backward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, stats, maps, do
                                       accumulate)
     ref = ctypes.byref(a)
     n = C.uniter_diff_attention_bwd_workspace_bytes(ref)
-    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
-    _launch_on(q, C.uniter_diff_attention_bwd, ref, ptr(stats), ptr(maps), dout.data_ptr(), dout.stride(-2), dout.stride(0),
+    ws = q.new_empty(max(n, 16), dtype=torch.uint8)
+    maps = saved.data_ptr()
+    _launch_on(q, C.uniter_diff_attention_bwd, ref, maps + 8 * dout.numel(), maps, dout.data_ptr(), dout.stride(-2), dout.stride(0),
                ctypes.byref(g), ws.data_ptr(), n)
 
 
@@ -1043,24 +1047,24 @@ class _DiffAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, mask, cu_q, cu_k, cfg, weight, *lams):
-        out, stats, maps = _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, True)
+        out, saved = _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, True)
         ctx.cfg = cfg
-        ctx.save_for_backward(q, k, v, mask, cu_q, cu_k, weight, stats, maps, *lams)
+        ctx.save_for_backward(q, k, v, mask, cu_q, cu_k, weight, saved, *lams)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, mask, cu_q, cu_k, weight, stats, maps, *lams = ctx.saved_tensors
+        q, k, v, mask, cu_q, cu_k, weight, saved, *lams = ctx.saved_tensors
         dout = _rows16(dout)
-        new = torch.empty if cu_q is None else torch.zeros             # rows of no example have no gradient
-        dq = new(q.shape, dtype=_BF16, device=q.device)
+        new = q.new_empty if cu_q is None else q.new_zeros             # rows of no example have no gradient
+        dq = new(q.shape)
         dk = dv = None
         if k is not None:
-            dk, dv = new(k.shape, dtype=_BF16, device=q.device), new(v.shape, dtype=_BF16, device=q.device)
-        dlams = torch.empty((4, *lams[0].shape), dtype=_BF16, device=q.device).unbind(0)
+            dk, dv = new(k.shape), new(v.shape)
+        dlams = q.new_empty((4, *lams[0].shape)).unbind(0)
         dweight = None if weight is None else torch.empty_like(weight)
-        _diff_backward(q, k, v, mask, cu_q, cu_k, ctx.cfg, weight, lams, stats, maps, dout, dq, dk, dv, dlams, dweight, False)
+        _diff_backward(q, k, v, mask, cu_q, cu_k, ctx.cfg, weight, lams, saved, dout, dq, dk, dv, dlams, dweight, False)
         return (dq, dk, dv, None, None, None, None, dweight, *dlams)
 
 
@@ -1072,10 +1076,21 @@ def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, ep
     if odd or dim not in (32, 64) or H != heads * 2 * dim:
         raise _lib.UniterHipError("differential attention: a head is 64 or 128 columns (two maps of 32 or 64), got %d columns for %d heads" % (H, heads))
     packed = cu_q is not None or cu_k is not None
-    for t, what in ((q, "qkv"),) if fused else ((q, "q"), (k, "k"), (v, "v")):
-        _check_dev(t, what)
-        if t.dim() != (2 if packed else 3):
-            raise _lib.UniterHipError("%s must be %s, got %s" % (what, "[rows, columns] when cu_seqlens is given" if packed else "[B, L, columns]", tuple(t.shape)))
+    nd = 2 if packed else 3
+    _check_dev(q, "qkv" if fused else "q")
+    dev = q.get_device()
+
+    def bf16_here(t, what):
+        if not isinstance(t, torch.Tensor) or t.dtype is not _BF16 or t.get_device() != dev:
+            _check_dev(t, what)
+            _check_same_device(q, "qkv" if fused else "q", ((t, what),))
+
+    if q.dim() != nd or not fused and (k.dim() != nd or v.dim() != nd):
+        raise _lib.UniterHipError("%s must be %s, got %s" % ("qkv" if fused else "q, k and v", "[rows, columns] when cu_seqlens is given" if packed else
+                                                             "[B, L, columns]", [tuple(t.shape) for t in (q, k, v) if t is not None]))
+    if not fused:
+        bf16_here(k, "k")
+        bf16_here(v, "v")
     Bk = q if fused else k
     if not fused and (k.shape != v.shape or k.shape[-1] != H or (not packed and k.shape[0] != q.shape[0])):
         raise _lib.UniterHipError("differential attention: q %s, k %s and v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
@@ -1085,11 +1100,11 @@ def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, ep
     if shape != (heads, dim) and shape != (dim,):
         raise _lib.UniterHipError("lambda vectors must be [%d] or [%d, %d], got %s" % (dim, heads, dim, tuple(shape)))
     for t in lams:
-        _check_dev(t, "lambda vector")
+        bf16_here(t, "lambda vector")
         if t.shape != shape:
             raise _lib.UniterHipError("lambda vectors must have one shape, got %s and %s" % (tuple(shape), tuple(t.shape)))
     if weight is not None:
-        _check_dev(weight, "norm_weight")
+        bf16_here(weight, "norm_weight")
         if weight.shape != (2 * dim,):
             raise _lib.UniterHipError("norm_weight must be [%d], got %s" % (2 * dim, tuple(weight.shape)))
         weight = _rows16(weight)
@@ -1111,16 +1126,13 @@ def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, ep
         cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
     elif mask is not None:
         _check_dev(mask, "mask_bias", torch.float32)
-        if mask.dim() == 4:                        # UniterModel's extended mask [B, 1, 1, L]
-            mask = mask.reshape(mask.shape[0], mask.shape[-1])
+        if mask.dim() == 4 and mask.shape[1] == mask.shape[2] == 1:        # UniterModel's extended mask [B, 1, 1, L]
+            mask = mask[:, 0, 0]
         if mask.shape != (q.shape[0], Bk.shape[1]):
             raise _lib.UniterHipError("mask_bias must be [%d, %d] (or [B, 1, 1, Lk]), got %s" % (q.shape[0], Bk.shape[1], tuple(mask.shape)))
         if mask.stride(1) != 1:
             mask = mask.contiguous()
-    dev = q.get_device()
-    for t in (k, v, mask, cu_q, cu_k, weight, *lams):
-        if t is not None and t.get_device() != dev:
-            raise _lib.UniterHipError("differential attention: all tensors must be on %s, one is on %s" % (q.device, t.device))
+    _check_same_device(q, "qkv" if fused else "q", ((mask, "mask_bias"), (cu_q, "cu_seqlens"), (cu_k, "cu_seqlens_k")))
     return dim, mask, cu_q, cu_k, max_q, max_k, [t.contiguous() for t in lams], weight
 
 
@@ -1149,6 +1161,8 @@ def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=Non
     p_drop: dropout on the difference of the maps (callers pass 0 in evaluation).  Gradients flow to q, k, v, lambdas and norm_weight.
     Both passes can be captured into a graph; as with any operator, release eager autograd graphs of the same leaves before capturing a
     backward pass."""
+    if not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor):
+        raise _lib.UniterHipError("differential attention needs k and v (differential_self_attention takes a fused projection)")
     checked = _diff_check(q, k, v, heads, lambdas, norm_weight, mask_bias, cu_seqlens, cu_seqlens_k, max_len, max_len_k, eps, p_drop)
     return _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop)
 
@@ -1194,25 +1208,25 @@ class _BertDiffAttentionFn(torch.autograd.Function):
         seed, off = _next_offsets(1) if p > 0.0 else (0, 0)
         cfg = (att.num_attention_heads, att.map_size, att.lambda_init, att.LayerNorm.eps, max_len, max_len, p, seed, off)
         lams = [t.detach() for t in att.lambdas()]
-        out, stats, maps = _diff_forward(qkv, None, None, mask, cu, cu, cfg, att.LayerNorm.weight, lams, keep)
+        out, saved = _diff_forward(qkv, None, None, mask, cu, cu, cfg, att.LayerNorm.weight, lams, keep)
         ctx.att, ctx.cfg = att, cfg
         if keep:
-            ctx.save_for_backward(xc, qkv, mask, positions, cu, stats, maps)
+            ctx.save_for_backward(xc, qkv, mask, positions, cu, saved)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        xc, qkv, mask, positions, cu, stats, maps = ctx.saved_tensors
+        xc, qkv, mask, positions, cu, saved = ctx.saved_tensors
         att = ctx.att
         H = xc.shape[-1]
         T = xc.numel() // H
         st = _lib.stream_ptr()
-        dqkv = (torch.empty if cu is None else torch.zeros)(qkv.shape, dtype=_BF16, device=qkv.device)
+        dqkv = (qkv.new_empty if cu is None else qkv.new_zeros)(qkv.shape)
         dl = [ensure_grad(t) if t.requires_grad else None for t in att.lambdas()]
         w = att.LayerNorm.weight
         dw = ensure_grad(w) if w.requires_grad else None
-        _diff_backward(qkv, None, None, mask, cu, cu, ctx.cfg, w, att.lambdas(), stats, maps, _rows16(dout), dqkv, None, None, dl, dw, True)
+        _diff_backward(qkv, None, None, mask, cu, cu, ctx.cfg, w, att.lambdas(), saved, _rows16(dout), dqkv, None, None, dl, dw, True)
         if att.rotary is not None:
             dqk = dqkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
             _rotary_launch(dqk, dqk, positions, 0, att.rotary, True)
