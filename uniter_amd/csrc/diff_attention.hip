@@ -102,6 +102,8 @@ __device__ __forceinline__ bf16x8 pack_step(const f32x16& s, const int kk) {
     for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(s[8 * kk + 2 * i], s[8 * kk + 2 * i + 1]);
     return __builtin_bit_cast(bf16x8, w);
 }
+// the larger one, or a NaN (one instruction for two of them: v_maximum3; fmaxf would quieten its operands first)
+__device__ __forceinline__ float max2(const float a, const float b) { return __builtin_elementwise_maximum(a, b); }
 // the value of lane ^ 32
 __device__ __forceinline__ float other_half(const float x) { return __shfl_xor(x, 32, WAVE); }
 // row (or column) of an accumulator register: 8 (r / 4) + 4 half + r % 4
@@ -145,8 +147,10 @@ __device__ __forceinline__ Span span_of(const int32_t* cu, const int64_t total, 
     return s;
 }
 
-// additive mask in log2 units; the type's lowest value stays finite (a row of nothing but that is uniform over its keys)
-__device__ __forceinline__ float mask_log2(const float m) { return m == -INFINITY ? m : fmaxf(m * LOG2E, -3.4028234663852886e38f); }
+// additive mask in log2 units; the type's lowest value stays finite and above NONE, the reference of a row without keys yet (a row of
+// nothing but lowest values is uniform over its keys)
+constexpr float NONE = -3.4028234663852886e38f;
+__device__ __forceinline__ float mask_log2(const float m) { return m == -INFINITY ? m : fmaxf(m * LOG2E, -3e38f); }
 
 // ---- tiles by direct global -> LDS transfers (global_load_lds_dwordx4: a wave instruction moves 64 x 16 bytes to a contiguous 1 KiB
 // of LDS, so the swizzle is applied to the source address).  The origin of a tile is scalar, a lane's offset inside it 32 bits (the entry
@@ -293,7 +297,7 @@ template <int D>
 struct FwdState {
     bf16x8 qf[2][D / 16];
     f32x16 o[2][D / 16];                 // [map][32 columns of V]
-    float m[2], l[2];
+    float m[2], l[2];                    // reference (NONE: no key yet) and sum of the weights
     float se;                            // scores are s * se in log2 units (1 once a mask has been added)
 };
 
@@ -340,15 +344,15 @@ __device__ __forceinline__ void fwd_arrive(FwdState<D>& f, f32x16 (&s)[2], const
     float mx[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        mx[j] = fmaxf(s[j][0], s[j][1]);
+        mx[j] = max2(s[j][0], s[j][1]);
 #pragma unroll
-        for (int r = 2; r < 16; r += 2) mx[j] = fmaxf(fmaxf(mx[j], s[j][r]), s[j][r + 1]);
+        for (int r = 2; r < 16; r += 2) mx[j] = max2(max2(mx[j], s[j][r]), s[j][r + 1]);
         mx[j] *= f.se;
     }
     if (__any(mx[0] > f.m[0] + LAZY || mx[1] > f.m[1] + LAZY)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float top = fmaxf(mx[j], other_half(mx[j]));
+            const float top = max2(mx[j], other_half(mx[j]));
             const bool move = top > f.m[j] + LAZY;
             const float alpha = move ? __builtin_amdgcn_exp2f(f.m[j] - top) : 1.f;
             f.m[j] = move ? top : f.m[j];
@@ -359,14 +363,14 @@ __device__ __forceinline__ void fwd_arrive(FwdState<D>& f, f32x16 (&s)[2], const
     }
 }
 template <int D, bool DROP>
-__device__ __forceinline__ void fwd_weights(FwdState<D>& f, f32x16 (&s)[2], bf16x8 (&pf)[2][2], const float (&ms)[2], const uint32_t keep) {
+__device__ __forceinline__ void fwd_weights(FwdState<D>& f, f32x16 (&s)[2], bf16x8 (&pf)[2][2], const uint32_t keep) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        float sum[2] = {0.f, 0.f};
+        float sum[2];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], f.se, -ms[j]));
-            sum[r & 1] += s[j][r];
+            s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], f.se, -f.m[j]));
+            sum[r & 1] = r < 2 ? s[j][r] : sum[r & 1] + s[j][r];
             if constexpr (DROP) s[j][r] = (keep >> r) & 1u ? s[j][r] : 0.f;
         }
         f.l[j] += sum[0] + sum[1];
@@ -415,7 +419,7 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const Di
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) f.qf[j][s] = __builtin_bit_cast(bf16x8, ldg16<false>(Q + j * D + s * 16));
-        f.m[j] = -INFINITY;
+        f.m[j] = NONE;
         f.l[j] = 0.f;
 #pragma unroll
         for (int t = 0; t < NV; ++t) f.o[j][t] = zero16();
@@ -441,8 +445,7 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const Di
             fwd_arrive<D>(f, s, p, kt.Mb(t), general, u, lane);
             uint32_t keep = 0xffffu;
             if constexpr (DROP) keep = keep16(p, drow, t * KT + u * 32, half);
-            const float ms[2] = {f.m[0] == -INFINITY ? 0.f : f.m[0], f.m[1] == -INFINITY ? 0.f : f.m[1]};
-            fwd_weights<D, DROP>(f, s, pf, ms, keep);
+            fwd_weights<D, DROP>(f, s, pf, keep);
             fwd_products<D>(f, pf, kt.Vb(t), u, lane);
         }
         if (t + 1 < t1) kt.finish(t + 1);
@@ -453,7 +456,7 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const Di
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         l[j] += other_half(l[j]);
-        m[j] = m[j] == -INFINITY ? 0.f : m[j];
+        m[j] = m[j] == NONE ? 0.f : m[j];
     }
     const float dscale = DROP ? p.drop.scale : 1.f;
     if constexpr (SPLIT) {
@@ -807,6 +810,16 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
     pin(gf);
     float c_lse[2] = {m[0] + ll[0], m[1] + ll[1]};
     asm volatile("" : "+v"(c_lse[0]), "+v"(c_lse[1]), "+v"(Dq[0]), "+v"(Dq[1]));
+    // d = 32, no dropout: the products start from -D_1 held in 16 registers and give G - D_1 at once; map 2 takes D_2 - D_1 off it (24 sequences
+    // to 509: 79.4 us against 80.5; with d = 64 the registers are short: 16 x 178 16.6 against 16.2)
+    constexpr bool HELD = D == 32 && !DROP;
+    f32x16 nD;
+    if constexpr (HELD) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) nD[r] = -Dq[0];
+        asm volatile("" : "+v"(nD));                           // (registers, not 16 moves in every block)
+        Dq[1] -= Dq[0];
+    }
     if (nt > 0) kt.finish(0);
     else dma_wait();
 
@@ -816,7 +829,7 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
         const bf16_t *Kt = kt.Kb(t), *Vt = kt.Vb(t);
         const int subs = none || idle ? 0 : min(2, (sk.n - t * KT + 31) >> 5);
         for (int u = 0; u < subs; ++u) {
-            f32x16 g = zero16(), s[2];
+            f32x16 g = HELD ? nD : zero16(), s[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 s[j] = zero16();
@@ -850,7 +863,7 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], se, -c[j])) * (g[r] - Dq[j]);
+                for (int r = 0; r < 16; ++r) s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], se, -c[j])) * (HELD && j == 0 ? g[r] : g[r] - Dq[j]);
                 df[j][0] = pack_step(s[j], 0);
                 df[j][1] = pack_step(s[j], 1);
             }
@@ -879,7 +892,7 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
 // backward, keys: dV = sum_q A dO with A = dropout(P_1 - lambda P_2);  dK_j = sum_q dS_j Q_j
 // ------------------------------------------------------------------------------------------------
 // per query of a tile: max and log2(sum) of both maps, their sums, and D of both maps
-enum { ST_M = 0, ST_LL = 2, ST_LSE = 4, ST_D = 6, ST_N = 8 };
+enum { ST_M = 0, ST_LL = 2, ST_LSE = 4, ST_D = 6, ST_N = 8 };            // (without dropout ST_D holds -D_1 and D_2 - D_1)
 
 template <int D, bool DROP>
 __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, const int bid, char* smem) {
@@ -932,8 +945,8 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
                 w[ST_LL + j][lane] = in ? s4[2 * j + 1] : INFINITY;
                 w[ST_LSE + j][lane] = in ? s4[2 * j] + s4[2 * j + 1] : INFINITY;
             }
-            w[ST_D][lane] = d0;
-            w[ST_D + 1][lane] = d1;
+            w[ST_D][lane] = DROP ? d0 : -d0;
+            w[ST_D + 1][lane] = DROP ? d1 : d1 - d0;
         }
         __syncthreads();
     };
@@ -977,6 +990,13 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
         for (int u = 0; u < subs; ++u) {
             const float* w = &st[t & 1][0][u * 32 + 4 * half];
             f32x16 g = zero16(), s[2], a;
+            if constexpr (!DROP)                               // the products give G - D_1 at once; map 2 takes D_2 - D_1 off it
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 D4 = *reinterpret_cast<const f32x4*>(w + ST_D * KT + 8 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) g[4 * i + e] = D4[e];
+                }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 s[j] = zero16();
@@ -1026,7 +1046,7 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
                         const int r = 4 * i + e;
                         const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], se, -c4[e]));
                         a[r] = j == 0 ? pr : __builtin_fmaf(-lam, pr, a[r]);
-                        s[j][r] = pr * (g[r] - D4[e]);
+                        s[j][r] = pr * (!DROP && j == 0 ? g[r] : g[r] - D4[e]);
                     }
                 }
             if constexpr (DROP) {
