@@ -217,6 +217,50 @@ def test_encoder_against_plain_layers(heads, hidden, rotary, L):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.0, 0.2])
+def test_one_node_per_layer_does_what_the_blocks_do(p):
+    """The blocks on their own round two residual sums more, and gelu's derivative once more: three roundings among the 20 of a layer's
+    backward pass, well under its tolerance of 5e-2 to the formula.  Dropout draws are the same."""
+    cfg = config(2, 128, 2, ROTARY, p=p)
+    one = encoder(cfg).cuda().train()
+    two = copy.deepcopy(one)
+    for l in two.layer:                          # a frozen bias: block by block
+        l.output.dense.bias.requires_grad_(False)
+    g = torch.Generator().manual_seed(2)
+    x, dy = (torch.randn(2, 40, 128, generator=g).to(BF16).cuda() for _ in range(2))
+    got = []
+    for e in (one, two):
+        ops.manual_seed(5)
+        xg = x.clone().requires_grad_(True)
+        y = e(xg, torch.zeros(2, 40).cuda())[-1]
+        y.backward(dy)
+        got.append((y.detach(), xg.grad))
+    assert torch.equal(got[0][0], got[1][0])
+    assert rel_l2(got[1][1], got[0][1]) < 2e-2
+    for (n, q), (_, r) in zip(one.named_parameters(), two.named_parameters()):
+        if r.requires_grad and not n.endswith("key.bias"):
+            assert cosine(q.grad, r.grad) > 0.995, n
+        elif not r.requires_grad:
+            assert r.grad is None and q.grad.any(), n
+
+
+@pytest.mark.gpu
+def test_frozen_encoders_and_what_the_blocks_refuse():
+    x = torch.randn(2, 9, 64).to(BF16).cuda()
+    for kw in (dict(intermediate_size=96), dict(hidden_act="relu")):
+        with pytest.raises(_lib.UniterHipError):
+            encoder(config(1, 64, 1, **kw)).cuda().train()(x, torch.zeros(2, 9).cuda())
+    e = encoder(config(1, 64, 2)).cuda().train()
+    for q in e.parameters():
+        q.requires_grad_(False)
+    xg = x.clone().requires_grad_(True)
+    e(xg, torch.zeros(2, 9).cuda())[-1].backward(x)
+    assert xg.grad.any() and all(q.grad is None for q in e.parameters())
+    y = e(x, torch.zeros(2, 9).cuda())[-1]
+    assert not y.requires_grad
+
+
+@pytest.mark.gpu
 def test_packed_rows_give_what_padded_rows_give():
     cfg = config(2, 128, 2, ROTARY)
     e = encoder(cfg).cuda().eval()

@@ -268,18 +268,15 @@ def is_differential(layer):
 
 
 def run_differential(layers, hidden_states, attention_mask=None, positions=None, cu_seqlens=None, max_len=None, output_all=False, hook=None):
-    """The layers of a differential encoder, one after the other: the fused stack runs softmax attention, so here every block is its own
-    autograd node (attention, output projection + LayerNorm, intermediate, output).  Gradients are complete on the compute stream when
-    backward() returns.  A reducer that counts on the fused stack's per-layer calls would wait for them in vain and is refused
-    (GradientReducer reduces such an encoder in finish())."""
+    """The layers of a differential encoder, one autograd node each: the fused stack runs softmax attention.  Gradients are complete on the
+    compute stream when backward() returns.  A reducer that counts on the fused stack's per-layer calls would wait for them in vain and is
+    refused (GradientReducer reduces such an encoder in finish())."""
     if hook is not None and not isinstance(hook, ops.DeferWgradJoin):
         raise UniterHipError("a per-layer gradient hook needs the fused stack (attention_type = 'softmax')")
     ops.tune_layer_gemms(layers[0]._enc_cfg, hidden_states, layers[0].training)
     outs, x = [], hidden_states
     for lay in layers:
-        a = lay.attention.self(x, attention_mask, positions, cu_seqlens, max_len)
-        a = lay.attention.output(a, x)
-        x = lay.output(lay.intermediate(a), a)
+        x = ops.bert_differential_layer(lay, x, attention_mask, positions, cu_seqlens, max_len)
         outs.append(x)
     return tuple(outs) if output_all else x
 

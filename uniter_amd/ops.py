@@ -1191,25 +1191,43 @@ def packed_positions(cu_seqlens, total):
     return torch.arange(total, device=cu.device) - torch.repeat_interleave(cu[:-1], cu.diff(), output_size=total)
 
 
+def _bert_diff_forward(xc, mask, positions, cu, max_len, att, p, keep):
+    """Fused [3H, H] projection, q | k turned in place, differential attention: (out, qkv, saved, cfg)."""
+    H = xc.shape[-1]
+    wqkv, bqkv = att.fused_qkv()
+    qkv = xc.new_empty((*xc.shape[:-1], 3 * H))
+    C.uniter_gemm_bias_fwd(ptr(xc), ptr(wqkv), ptr(bqkv), ptr(qkv), xc.numel() // H, 3 * H, H, _lib.stream_ptr())
+    if att.rotary is not None:
+        qk = qkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
+        _rotary_launch(qk, qk, positions, 0, att.rotary, False)
+    seed, off = _next_offsets(1) if p > 0.0 else (0, 0)
+    cfg = (att.num_attention_heads, att.map_size, att.lambda_init, att.LayerNorm.eps, max_len, max_len, p, seed, off)
+    out, saved = _diff_forward(qkv, None, None, mask, cu, cu, cfg, att.LayerNorm.weight, att.lambdas(), keep)
+    return out, qkv, saved, cfg
+
+
+def _bert_diff_backward(qkv, mask, positions, cu, cfg, att, saved, dout):
+    """Gradient of the projection's output; those of lambda and of the per-head norm are accumulated into `.grad`."""
+    H = qkv.shape[-1] // 3
+    dqkv = (qkv.new_empty if cu is None else qkv.new_zeros)(qkv.shape)
+    dl = [ensure_grad(t) if t.requires_grad else None for t in att.lambdas()]
+    w = att.LayerNorm.weight
+    dw = ensure_grad(w) if w.requires_grad else None
+    _diff_backward(qkv, None, None, mask, cu, cu, cfg, w, att.lambdas(), saved, _rows16(dout), dqkv, None, None, dl, dw, True)
+    if att.rotary is not None:
+        dqk = dqkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
+        _rotary_launch(dqk, dqk, positions, 0, att.rotary, True)
+    return dqkv
+
+
 class _BertDiffAttentionFn(torch.autograd.Function):
-    """BertDifferentialSelfAttention.forward: fused [3H, H] projection, q | k turned in place, differential attention."""
+    """BertDifferentialSelfAttention.forward."""
 
     @staticmethod
     def forward(ctx, x, mask, positions, cu, max_len, att, p, keep, *anchor):
-        H = x.shape[-1]
-        T = x.numel() // H
         xc = x.contiguous()
-        wqkv, bqkv = att.fused_qkv()
-        qkv = torch.empty((*x.shape[:-1], 3 * H), dtype=_BF16, device=x.device)
-        C.uniter_gemm_bias_fwd(ptr(xc), ptr(wqkv), ptr(bqkv), ptr(qkv), T, 3 * H, H, _lib.stream_ptr())
-        if att.rotary is not None:
-            qk = qkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
-            _rotary_launch(qk, qk, positions, 0, att.rotary, False)
-        seed, off = _next_offsets(1) if p > 0.0 else (0, 0)
-        cfg = (att.num_attention_heads, att.map_size, att.lambda_init, att.LayerNorm.eps, max_len, max_len, p, seed, off)
-        lams = [t.detach() for t in att.lambdas()]
-        out, saved = _diff_forward(qkv, None, None, mask, cu, cu, cfg, att.LayerNorm.weight, lams, keep)
-        ctx.att, ctx.cfg = att, cfg
+        out, qkv, saved, ctx.cfg = _bert_diff_forward(xc, mask, positions, cu, max_len, att, p, keep)
+        ctx.att = att
         if keep:
             ctx.save_for_backward(xc, qkv, mask, positions, cu, saved)
         return out
@@ -1221,23 +1239,78 @@ class _BertDiffAttentionFn(torch.autograd.Function):
         att = ctx.att
         H = xc.shape[-1]
         T = xc.numel() // H
-        st = _lib.stream_ptr()
-        dqkv = (qkv.new_empty if cu is None else qkv.new_zeros)(qkv.shape)
-        dl = [ensure_grad(t) if t.requires_grad else None for t in att.lambdas()]
-        w = att.LayerNorm.weight
-        dw = ensure_grad(w) if w.requires_grad else None
-        _diff_backward(qkv, None, None, mask, cu, cu, ctx.cfg, w, att.lambdas(), saved, _rows16(dout), dqkv, None, None, dl, dw, True)
-        if att.rotary is not None:
-            dqk = dqkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
-            _rotary_launch(dqk, dqk, positions, 0, att.rotary, True)
-        wqkv, _ = att.fused_qkv()
+        dqkv = _bert_diff_backward(qkv, mask, positions, cu, ctx.cfg, att, saved, dout)
         dx = None
         if ctx.needs_input_grad[0]:
             dx = torch.empty_like(xc)
-            C.uniter_gemm_dgrad(ptr(dqkv), ptr(wqkv), None, ptr(dx), T, 3 * H, H, st)
+            C.uniter_gemm_dgrad(ptr(dqkv), ptr(att.fused_qkv()[0]), None, ptr(dx), T, 3 * H, H, _lib.stream_ptr())
         if any(m.weight.requires_grad for m in (att.query, att.key, att.value)):
             gw, gb = att.fused_qkv_grad()
             _wgrad_into(dqkv, xc, gw, gb, T, 3 * H, H)
+        return (dx,) + (None,) * (len(ctx.needs_input_grad) - 1)
+
+
+class _BertDiffLayerFn(torch.autograd.Function):
+    """A whole BertLayer with differential attention and erf GELU: the kernels of its blocks as one node, the residual sums in the
+    data-gradient GEMMs' epilogues and the four weight gradients in one launch."""
+
+    @staticmethod
+    def forward(ctx, x, mask, positions, cu, max_len, layer, ps, keep, *anchor):
+        att, ao, im, out = layer.attention.self, layer.attention.output, layer.intermediate, layer.output
+        H, I = x.shape[-1], im.dense.weight.shape[0]
+        st = _lib.stream_ptr()
+        xc = x.contiguous()
+        T = xc.numel() // H
+        c, qkv, saved, cfg = _bert_diff_forward(xc, mask, positions, cu, max_len, att, ps[0], keep)
+        r1 = _next_offsets(1) if ps[1] > 0.0 else (0, 0)
+        z1 = xc.new_empty((T, H))
+        C.uniter_gemm_bias_dropout_residual_fwd(ptr(c), ptr(ao.dense.weight), ptr(ao.dense.bias), ptr(xc), ptr(z1), T, H, H, ps[1], *r1, st)
+        h, m1, s1 = _ln_fwd(z1, ao.LayerNorm.weight, ao.LayerNorm.bias, 1e-12, 0.0, 0, 0)
+        u, g = xc.new_empty((T, I)), xc.new_empty((T, I))
+        C.uniter_gemm_bias_gelu_fwd(ptr(h), ptr(im.dense.weight), ptr(im.dense.bias), ptr(u), ptr(g), T, I, H, st)
+        r2 = _next_offsets(1) if ps[2] > 0.0 else (0, 0)
+        z2 = xc.new_empty((T, H))
+        C.uniter_gemm_bias_dropout_residual_fwd(ptr(g), ptr(out.dense.weight), ptr(out.dense.bias), ptr(h), ptr(z2), T, H, I, ps[2], *r2, st)
+        y, m2, s2 = _ln_fwd(z2, out.LayerNorm.weight, out.LayerNorm.bias, 1e-12, 0.0, 0, 0)
+        if keep:
+            ctx.layer, ctx.cfg, ctx.ps, ctx.r1, ctx.r2 = layer, cfg, ps, r1, r2
+            ctx.save_for_backward(xc, qkv, mask, positions, cu, saved, c, z1, m1, s1, h, u, g, z2, m2, s2)
+        return y.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xc, qkv, mask, positions, cu, saved, c, z1, m1, s1, h, u, g, z2, m2, s2 = ctx.saved_tensors
+        layer = ctx.layer
+        att, ao, im, out = layer.attention.self, layer.attention.output, layer.intermediate, layer.output
+        T, H = z1.shape
+        I = u.shape[1]
+        st = _lib.stream_ptr()
+
+        def norm(dy, z, mean, rstd, mod, p, seed, off):
+            dz, dd = torch.empty_like(z), torch.empty_like(z)                  # to the residual as it is, to the dense branch through dropout
+            wsb = C.uniter_layernorm_bwd_workspace_bytes(T, H)
+            ws = _scratch(("ln", z.device.index), wsb, z.device)
+            ln = mod.LayerNorm
+            C.uniter_layernorm_bwd(ptr(dy), None, ptr(z), ptr(mean), ptr(rstd), ptr(ln.weight), ptr(dz), ptr(dd), ptr(ensure_grad(ln.weight)),
+                                   ptr(ensure_grad(ln.bias)), ptr(ensure_grad(mod.dense.bias)), T, H, 1, p, seed, off, 0, ptr(ws), wsb, st)
+            return dz, dd
+
+        dz2, dd2 = norm(dy.contiguous(), z2, m2, s2, out, ctx.ps[2], *ctx.r2)
+        du, dh, dc = torch.empty_like(u), torch.empty_like(h), torch.empty_like(c)
+        C.uniter_gemm_dgrad_gelu(ptr(dd2), ptr(out.dense.weight), ptr(u), ptr(du), T, H, I, st)
+        C.uniter_gemm_dgrad(ptr(du), ptr(im.dense.weight), ptr(dz2), ptr(dh), T, I, H, st)
+        dz1, dd1 = norm(dh, z1, m1, s1, ao, ctx.ps[1], *ctx.r1)
+        C.uniter_gemm_dgrad(ptr(dd1), ptr(ao.dense.weight), None, ptr(dc), T, H, H, st)
+        dqkv = _bert_diff_backward(qkv, mask, positions, cu, ctx.cfg, att, saved, dc)
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = torch.empty_like(xc)
+            C.uniter_gemm_dgrad(ptr(dqkv), ptr(att.fused_qkv()[0]), ptr(dz1), ptr(dx), T, 3 * H, H, st)
+        gw, gb = att.fused_qkv_grad()
+        wgrad_group([ptr(t) for t in (dd2, du, dd1, dqkv)], [0] * 4, [ptr(t) for t in (g, h, c, xc)], [0] * 4,
+                    [ptr(ensure_grad(out.dense.weight)), ptr(ensure_grad(im.dense.weight)), ptr(ensure_grad(ao.dense.weight)), ptr(gw)],
+                    [None, ptr(ensure_grad(im.dense.bias)), None, ptr(gb)], T, [H, I, H, 3 * H], [I, H, H, H], layer.training)
         return (dx,) + (None,) * (len(ctx.needs_input_grad) - 1)
 
 
@@ -1254,8 +1327,8 @@ def tune_layer_gemms(cfg_like, hidden_states, training):
     _maybe_autotune(_shape(dict(cfg_like, heads=cfg_like["H"] // 64, p_hidden=0.0, p_attn=0.0), B, L, training), training)
 
 
-def bert_differential_self_attention(att, hidden_states, attention_mask=None, positions=None, cu_seqlens=None, max_len=None):
-    """model/layer.py::BertDifferentialSelfAttention.forward.  Parameter gradients are accumulated into `.grad`."""
+def _bert_diff_inputs(att, hidden_states, attention_mask, positions, cu_seqlens, max_len):
+    """Checks; (mask, positions, cu_seqlens) as the kernels take them."""
     _check_dev(hidden_states, "hidden_states")
     packed = cu_seqlens is not None
     if hidden_states.dim() != (2 if packed else 3) or hidden_states.shape[-1] != att.all_head_size:
@@ -1263,10 +1336,6 @@ def bert_differential_self_attention(att, hidden_states, attention_mask=None, po
                                                                       "[B, L, %d]" % att.all_head_size, tuple(hidden_states.shape)))
     if hidden_states.get_device() != torch._C._cuda_getDevice():
         raise _lib.UniterHipError("hidden_states is on %s, which is not the current device" % (hidden_states.device,))
-    lin = (att.query, att.key, att.value)
-    prm = [m.weight for m in lin] + [m.bias for m in lin] + list(att.lambdas()) + [att.LayerNorm.weight]
-    _check_mod(prm, "attention parameter")
-    params_ready(*prm)
     if packed:
         _check_dev(cu_seqlens, "cu_seqlens", torch.int32)
         if attention_mask is not None or max_len is None or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
@@ -1275,21 +1344,46 @@ def bert_differential_self_attention(att, hidden_states, attention_mask=None, po
         if att.rotary is not None and positions is None:
             positions = packed_positions(cu_seqlens, hidden_states.shape[0])
     mask = key_mask(attention_mask, hidden_states)
-    if positions is not None and att.rotary is None:
-        raise _lib.UniterHipError("positions are given, but this attention has no rotary positions (config.rotary)")
     if positions is not None:
+        if att.rotary is None:
+            raise _lib.UniterHipError("positions are given, but this attention has no rotary positions (config.rotary)")
         rows = hidden_states.shape[:-1]
         if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int64, torch.int32) or positions.device != hidden_states.device \
                 or (positions.shape != rows and positions.shape != rows[-1:]):
             raise _lib.UniterHipError("positions must be an integer tensor %s or %s on %s" % (list(rows), list(rows[-1:]), hidden_states.device))
         positions = positions.to(torch.int64).contiguous()
-    for t, what in ((mask, "attention_mask"), (cu_seqlens, "cu_seqlens")):
-        if t is not None and t.device != hidden_states.device:
-            raise _lib.UniterHipError("%s is on %s, hidden_states on %s" % (what, t.device, hidden_states.device))
+    _check_same_device(hidden_states, "hidden_states", ((mask, "attention_mask"), (cu_seqlens, "cu_seqlens")))
+    return mask, positions, cu_seqlens
+
+
+def _p_of(mod):
+    return float(mod.dropout.p) if (mod.training and torch.is_grad_enabled()) else 0.0
+
+
+def bert_differential_self_attention(att, hidden_states, attention_mask=None, positions=None, cu_seqlens=None, max_len=None):
+    """model/layer.py::BertDifferentialSelfAttention.forward.  Parameter gradients are accumulated into `.grad`."""
+    mask, positions, cu_seqlens = _bert_diff_inputs(att, hidden_states, attention_mask, positions, cu_seqlens, max_len)
+    prm = list(att.parameters())
+    _check_mod(prm, "attention parameter")
+    params_ready(*prm)
+    keep = torch.is_grad_enabled() and (hidden_states.requires_grad or any(q.requires_grad for q in prm))
+    return _BertDiffAttentionFn.apply(hidden_states, mask, positions, cu_seqlens, max_len, att, _p_of(att), keep, *_anchor(prm))
+
+
+def bert_differential_layer(layer, hidden_states, attention_mask=None, positions=None, cu_seqlens=None, max_len=None):
+    """A BertLayer with differential attention (arguments as above); parameter gradients are accumulated into `.grad`.  One autograd node,
+    or one for each block where some of the parameters are frozen."""
+    att = layer.attention.self
+    prm = list(layer.parameters())
     track = torch.is_grad_enabled()
-    p = float(att.dropout.p) if (att.training and track) else 0.0
-    keep = track and (hidden_states.requires_grad or any(q.requires_grad for q in prm))
-    return _BertDiffAttentionFn.apply(hidden_states, mask, positions, cu_seqlens, max_len, att, p, keep, *_anchor(prm))
+    if layer._enc_cfg["act"] != 0 or (track and not all([q.requires_grad for q in prm])):      # (BertIntermediate says which activations it has)
+        a = layer.attention.output(att(hidden_states, attention_mask, positions, cu_seqlens, max_len), hidden_states)
+        return layer.output(layer.intermediate(a), a)
+    mask, positions, cu_seqlens = _bert_diff_inputs(att, hidden_states, attention_mask, positions, cu_seqlens, max_len)
+    _check_mod(prm, "layer parameter")
+    params_ready(*prm)
+    ps = (_p_of(att), _p_of(layer.attention.output), _p_of(layer.output))
+    return _BertDiffLayerFn.apply(hidden_states, mask, positions, cu_seqlens, max_len, layer, ps, track, *_anchor(prm))
 
 
 # ----------------------------------------------------------------------------------------------------
