@@ -165,7 +165,8 @@ def encoder(cfg, seed=0):
 # squares (terms of a row summed, or each for itself: whichever is more); e: twice the written-out error of dx, four deviations allowed.
 # A single call's lambda gradients are held to strict bounds in the tests of the operator.
 @pytest.mark.gpu
-@pytest.mark.parametrize("heads,hidden,rotary,L", [(2, 128, ROTARY, 50), (1, 128, None, 33), (3, 192, {"interleaved": False}, 130), (2, 256, ROTARY, 64)])
+@pytest.mark.parametrize("heads,hidden,rotary,L", [(2, 128, ROTARY, 50), (1, 128, None, 33), (3, 192, {"interleaved": False}, 130), (2, 256, ROTARY, 64),
+                                                   (6, 384, None, 64), (4, 256, None, 64)])
 def test_encoder_against_plain_layers(heads, hidden, rotary, L):
     cfg = config(heads, hidden, 3, rotary)
     e = encoder(cfg)

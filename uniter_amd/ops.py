@@ -1250,6 +1250,21 @@ class _BertDiffAttentionFn(torch.autograd.Function):
         return (dx,) + (None,) * (len(ctx.needs_input_grad) - 1)
 
 
+# csrc/gemm.hip kTileG6 / kTileG8: the deep-pipelined 192 x 192 and 256 x 256 tiles of the grouped weight gradients
+_TILE_192, _TILE_256 = 59, 58
+
+
+def _layer_wgrads(dys, xs_, dws, dbs, T, Ns, Ks, training):
+    """The four weight gradients of a layer in one launch, on the widest deep-pipelined tile that fits: 3072 tokens at 768 / 3072 62 us on
+    192 x 192 (256 x 256: 77, 128 x 128: 112), 2880 tokens at 1024 / 4096 84 us on 256 x 256 (128 x 128: 184), 320 tokens 15.5 against 14.4 of
+    the best small tile.  Rows that are not a multiple of 64 take the tuned tile (wgrad_group)."""
+    tile = next((c for c, e in ((_TILE_192, 192), (_TILE_256, 256)) if T % 64 == 0 and all(n % e == 0 for n in Ns + Ks)), None)
+    if tile is None:
+        return wgrad_group(dys, [0] * 4, xs_, [0] * 4, dws, dbs, T, Ns, Ks, training)
+    PA, IA = ctypes.c_void_p * 4, ctypes.c_int64 * 4
+    C.uniter_gemm_wgrad_group_ws(4, PA(*dys), None, PA(*xs_), None, PA(*dws), PA(*dbs), T, IA(*Ns), IA(*Ks), 1, None, 0, tile, 1, _lib.stream_ptr())
+
+
 class _BertDiffLayerFn(torch.autograd.Function):
     """A whole BertLayer with differential attention and erf GELU: the kernels of its blocks as one node, the residual sums in the
     data-gradient GEMMs' epilogues and the four weight gradients in one launch."""
@@ -1308,9 +1323,9 @@ class _BertDiffLayerFn(torch.autograd.Function):
             dx = torch.empty_like(xc)
             C.uniter_gemm_dgrad(ptr(dqkv), ptr(att.fused_qkv()[0]), ptr(dz1), ptr(dx), T, 3 * H, H, st)
         gw, gb = att.fused_qkv_grad()
-        wgrad_group([ptr(t) for t in (dd2, du, dd1, dqkv)], [0] * 4, [ptr(t) for t in (g, h, c, xc)], [0] * 4,
-                    [ptr(ensure_grad(out.dense.weight)), ptr(ensure_grad(im.dense.weight)), ptr(ensure_grad(ao.dense.weight)), ptr(gw)],
-                    [None, ptr(ensure_grad(im.dense.bias)), None, ptr(gb)], T, [H, I, H, 3 * H], [I, H, H, H], layer.training)
+        _layer_wgrads([ptr(t) for t in (dd2, du, dd1, dqkv)], [ptr(t) for t in (g, h, c, xc)],
+                      [ptr(ensure_grad(out.dense.weight)), ptr(ensure_grad(im.dense.weight)), ptr(ensure_grad(ao.dense.weight)), ptr(gw)],
+                      [None, ptr(ensure_grad(im.dense.bias)), None, ptr(gb)], T, [H, I, H, 3 * H], [I, H, H, H], layer.training)
         return (dx,) + (None,) * (len(ctx.needs_input_grad) - 1)
 
 
