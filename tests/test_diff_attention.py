@@ -325,6 +325,35 @@ def test_no_key_left_among_many(dim, Lq, Lk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [32, 64])
+def test_one_token_after_the_other_against_a_cache(dim):
+    """Serving: a prompt of 37 tokens, then single ones; keys are turned straight into a cache that is longer than what it holds (NaN behind),
+    queries attend to what is there.  Every step against the formula on the same turned queries and keys."""
+    from uniter_amd.model.rotary import RotaryPositions
+    g = torch.Generator().manual_seed(dim)
+    B, heads, room, prompt, end = 2, 3, 80, 37, 66
+    H = heads * 2 * dim
+    rot = RotaryPositions(dim, scaling={"type": "linear", "factor": 2.0})
+    lams, w = params(g, heads, dim)
+    x = torch.randn(B, end, 3 * H, generator=g).to(BF16).cuda()
+    cache = torch.full((2, B, room, H), math.nan, dtype=BF16, device="cuda")
+    at = 0
+    with torch.no_grad():
+        for n in [prompt] + [1] * (end - prompt):
+            q, k, v = x[:, at:at + n].split(H, dim=-1)
+            q = ops.rotary(q.unflatten(-1, (2 * heads, dim)), None, rot, offset=at).flatten(2)
+            ops.rotary(k.unflatten(-1, (2 * heads, dim)), None, rot, offset=at, out=cache[0, :, at:at + n].unflatten(-1, (2 * heads, dim)))
+            cache[1, :, at:at + n] = v
+            at += n
+            out = ops.differential_attention(q, cache[0, :, :at], cache[1, :, :at], heads, lams, 0.4, norm_weight=w)
+            value, bound = whole(q, cache[0, :, :at], cache[1, :, :at], heads, lams, 0.4, w, 1e-5)["out"]
+            over = (out.cpu().double() - value).abs() - bound - U * value.abs()
+            assert (over <= 0).all(), (at, float(over.max()))
+    whole_prompt = ops.rotary(x[..., H:2 * H].unflatten(-1, (2 * heads, dim)), None, rot).flatten(2)
+    assert torch.equal(cache[0, :, :end], whole_prompt) and cache[0, :, end:].isnan().all()
+
+
+@pytest.mark.gpu
 def test_strides_and_alignment():
     g = torch.Generator().manual_seed(9)
     heads, dim, B, L = 2, 32, 2, 45
