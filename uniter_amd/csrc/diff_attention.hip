@@ -19,6 +19,7 @@
 // 625 (d = 64).  The vector unit bounds it (two exponentials and about seven more instructions per query, key and map pair: 47 % of the
 // cycles at d = 64, where matrix instructions take 35 %: on one SIMD the two add up).  One query, 16381 keys, 4 x 12 heads: 36 us (5.5 TB/s) and
 // 5 for the join.  32 x 96, 12 heads, d = 32: 11 us forward, 16 with what the backward pass wants kept, 9 + 23 backward: latency.
+// Dropout: two generator calls per lane and 32 keys, in all three loops (32 x 512, 12 heads, d = 32: forward 63 -> 93 us, backward 201 -> 253).
 #include "common.cuh"
 #include "kernels.h"
 #include "../../include/uniter_hip.h"
@@ -283,12 +284,28 @@ __device__ __forceinline__ void lambda_of(const DiffArgs& p, const int h, const 
     e2 = uniform(__expf(wave_sum(b)));
 }
 
-// keep bits of the 16 elements (query of this lane, 32 keys from kb): bit r belongs to register r.  One generator call covers the 8
-// registers of a 16-key step that one lane holds: group ((row * ceil(Lk / 16) + key / 16) * 2 + half).
-__device__ __forceinline__ uint32_t keep16(const DiffArgs& p, const uint64_t row, const int kb, const int half) {
+// Random fields of the 16 elements (query of this lane, 32 keys from kb): word i holds those of registers 2 i and 2 i + 1; an element is kept
+// when its field is at least drop.thresh.  One generator call covers the 8 registers of a 16-key step that one lane holds: group
+// ((row * ceil(Lk / 16) + key / 16) * 2 + half).
+struct Fields { uint32_t w[8]; };
+__device__ __forceinline__ Fields fields16(const DiffArgs& p, const uint64_t row, const int kb, const int half) {
     const uint64_t n16 = (uint64_t)((p.Lk + 15) >> 4);
     const uint64_t g = (row * n16 + (uint64_t)(kb >> 4)) * 2 + (uint64_t)half;
-    return dropout_keep8(p.drop, g) | (dropout_keep8(p.drop, g + 2) << 8);
+    const u32x4 a = dropout_bits8(p.drop, g), b = dropout_bits8(p.drop, g + 2);
+    Fields f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f.w[i] = a[i]; f.w[4 + i] = b[i]; }
+    return f;
+}
+__device__ __forceinline__ bool kept(const DiffArgs& p, const Fields& f, const int r) {
+    return (r & 1 ? f.w[r >> 1] >> 16 : f.w[r >> 1] & 0xffffu) >= p.drop.thresh;
+}
+// all ones in the halves of word i whose element is kept (packed 16-bit arithmetic: 0 from a saturated thresh - field, then 0 - 1)
+__device__ __forceinline__ uint32_t keep_mask(const DiffArgs& p, const Fields& f, const int i) {
+    typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+    const unsigned short t = (unsigned short)p.drop.thresh;
+    const u16x2 x = __builtin_elementwise_sub_sat(u16x2{t, t}, __builtin_bit_cast(u16x2, f.w[i]));
+    return __builtin_bit_cast(uint32_t, (u16x2)(__builtin_elementwise_min(x, u16x2{1, 1}) - u16x2{1, 1}));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -369,7 +386,7 @@ __device__ __forceinline__ void fwd_arrive(FwdState<D>& f, f32x16 (&s)[2], const
     }
 }
 template <int D, bool DROP>
-__device__ __forceinline__ void fwd_weights(FwdState<D>& f, f32x16 (&s)[2], bf16x8 (&pf)[2][2], const uint32_t keep) {
+__device__ __forceinline__ void fwd_weights(FwdState<D>& f, f32x16 (&s)[2], bf16x8 (&pf)[2][2], const uint32_t (&keep)[8]) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         float sum[2];
@@ -377,11 +394,18 @@ __device__ __forceinline__ void fwd_weights(FwdState<D>& f, f32x16 (&s)[2], bf16
         for (int r = 0; r < 16; ++r) {
             s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], f.se, -f.m[j]));
             sum[r & 1] = r < 2 ? s[j][r] : sum[r & 1] + s[j][r];
-            if constexpr (DROP) s[j][r] = (keep >> r) & 1u ? s[j][r] : 0.f;
         }
         f.l[j] += sum[0] + sum[1];
-        pf[j][0] = pack_step(s[j], 0);
-        pf[j][1] = pack_step(s[j], 1);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            pf[j][kk] = pack_step(s[j], kk);
+            if constexpr (DROP) {
+                u32x4 w = __builtin_bit_cast(u32x4, pf[j][kk]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] &= keep[4 * kk + i];
+                pf[j][kk] = __builtin_bit_cast(bf16x8, w);
+            }
+        }
     }
 }
 
@@ -449,8 +473,12 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const Di
             bf16x8 pf[2][2];
             fwd_scores<D>(s, f, kt.Kb(t), u, lane);
             fwd_arrive<D>(f, s, p, kt.Mb(t), general, u, lane);
-            uint32_t keep = 0xffffu;
-            if constexpr (DROP) keep = keep16(p, drow, t * KT + u * 32, half);
+            uint32_t keep[8];
+            if constexpr (DROP) {
+                const Fields fl = fields16(p, drow, t * KT + u * 32, half);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) keep[i] = keep_mask(p, fl, i);
+            }
             fwd_weights<D, DROP>(f, s, pf, keep);
             fwd_products<D>(f, pf, kt.Vb(t), u, lane);
         }
@@ -798,12 +826,13 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
     }
     const f32x4 st = *reinterpret_cast<const f32x4*>(p.stats + ((int64_t)bh * p.Lq + qs) * NSTAT);
     const float m[2] = {st[0], st[2]}, ll[2] = {st[1], st[3]};
-    float Dq[2] = {p.D[((int64_t)bh * p.Lq + qs) * 2], p.D[((int64_t)bh * p.Lq + qs) * 2 + 1]};
+    // with dropout: G without its factor `dscale`, D over dscale, and dscale with the other factors at the end
+    const float dscale = DROP ? p.drop.scale : 1.f, iscale = DROP ? 1.f / p.drop.scale : 1.f;
+    float Dq[2] = {p.D[((int64_t)bh * p.Lq + qs) * 2] * iscale, p.D[((int64_t)bh * p.Lq + qs) * 2 + 1] * iscale};
     float e1, e2;
     lambda_of<D>(p, h, lane, e1, e2);
     const float lam = e1 - e2 + p.lambda_init;
     const uint64_t drow = (uint64_t)bh * (uint64_t)p.Lq + (uint64_t)q;
-    const float dscale = DROP ? p.drop.scale : 1.f;
 
     f32x16 dq[2][ND];
 #pragma unroll
@@ -861,9 +890,9 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
                 }
             }
             if constexpr (DROP) {
-                const uint32_t keep = keep16(p, drow, t * KT + u * 32, half);
+                const Fields fl = fields16(p, drow, t * KT + u * 32, half);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) g[r] = (keep >> r) & 1u ? g[r] * dscale : 0.f;
+                for (int r = 0; r < 16; ++r) g[r] = kept(p, fl, r) ? g[r] : 0.f;
             }
             bf16x8 df[2][2];
 #pragma unroll
@@ -883,7 +912,7 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
         }
         if (t + 1 < nt) kt.finish(t + 1);
     }
-    const float z = p.sc * (1.f / LOG2E);
+    const float z = p.sc * (1.f / LOG2E) * dscale;
     bf16_t* dst = p.dq + (int64_t)b * p.bdq * (p.cu_q == nullptr) + (sq.row + q) * p.ldq + h * W;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -898,7 +927,7 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
 // backward, keys: dV = sum_q A dO with A = dropout(P_1 - lambda P_2);  dK_j = sum_q dS_j Q_j
 // ------------------------------------------------------------------------------------------------
 // per query of a tile: max and log2(sum) of both maps, their sums, and D of both maps
-enum { ST_M = 0, ST_LL = 2, ST_LSE = 4, ST_D = 6, ST_N = 8 };            // (without dropout ST_D holds -D_1 and D_2 - D_1)
+enum { ST_M = 0, ST_LL = 2, ST_LSE = 4, ST_D = 6, ST_N = 8 };            // (ST_D without dropout: -D_1 and D_2 - D_1)
 
 template <int D, bool DROP>
 __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, const int bid, char* smem) {
@@ -927,6 +956,7 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
     const bf16_t* dO = p.dctx != nullptr ? p.dctx + ((p.cu_q != nullptr ? sq.row : (int64_t)b * p.Lq) * p.heads + h) * W
                                          : p.dout + (int64_t)b * p.bdo * (p.cu_q == nullptr) + sq.row * p.ldo + h * W;
     const int64_t ldO = p.dctx != nullptr ? (int64_t)p.heads * W : p.ldo;
+    const float dscale = DROP ? p.drop.scale : 1.f, iscale = DROP ? 1.f / p.drop.scale : 1.f;       // (as in the dQ pass)
     f32x4 s4;
     float d0, d1;
     auto start = [&](const int t) {
@@ -951,8 +981,8 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
                 w[ST_LL + j][lane] = in ? s4[2 * j + 1] : INFINITY;
                 w[ST_LSE + j][lane] = in ? s4[2 * j] + s4[2 * j + 1] : INFINITY;
             }
-            w[ST_D][lane] = DROP ? d0 : -d0;
-            w[ST_D + 1][lane] = DROP ? d1 : d1 - d0;
+            w[ST_D][lane] = DROP ? d0 * iscale : -d0;
+            w[ST_D + 1][lane] = DROP ? d1 * iscale : d1 - d0;
         }
         __syncthreads();
     };
@@ -974,7 +1004,6 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
     float e1, e2;
     lambda_of<D>(p, h, lane, e1, e2);
     const float lam = e1 - e2 + p.lambda_init;
-    const float dscale = DROP ? p.drop.scale : 1.f;
 
     f32x16 dk[2][ND], dv[NV];
 #pragma unroll
@@ -1030,16 +1059,16 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
             if constexpr (DROP) {
                 // the draws come with a query per lane; the ballot of bit r holds, for either half of the wave, one key over the queries
                 const uint64_t drow = (uint64_t)bh * (uint64_t)p.Lq + (uint64_t)(t * KT + u * 32 + (lane & 31));
-                const uint32_t mine = keep16(p, drow, kbase, half);
+                const Fields fl = fields16(p, drow, kbase, half);
                 const int kl = lane & 31, reg = 4 * (kl >> 3) + (kl & 3), kh = (kl >> 2) & 1;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const unsigned long long bal = __ballot((mine >> r) & 1u);
+                    const unsigned long long bal = __ballot(kept(p, fl, r));
                     const uint32_t part = kh ? (uint32_t)(bal >> 32) : (uint32_t)bal;
                     keep = reg == r ? part : keep;                             // bit: query of this block
                 }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) g[r] = (keep >> (acc_row(r) + 4 * half)) & 1u ? g[r] * dscale : 0.f;
+                for (int r = 0; r < 16; ++r) g[r] = (keep >> (acc_row(r) + 4 * half)) & 1u ? g[r] : 0.f;
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
@@ -1057,7 +1086,7 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
                 }
             if constexpr (DROP) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) a[r] = (keep >> (acc_row(r) + 4 * half)) & 1u ? a[r] * dscale : 0.f;
+                for (int r = 0; r < 16; ++r) a[r] = (keep >> (acc_row(r) + 4 * half)) & 1u ? a[r] : 0.f;
             }
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
@@ -1074,11 +1103,14 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
         }
         if (t + 1 < nt) finish(t + 1);
     }
-    const float z = p.sc * (1.f / LOG2E);
+    const float z = p.sc * (1.f / LOG2E) * dscale;
     bf16_t* dkp = p.dk + (int64_t)b * p.bdk * (p.cu_k == nullptr) + (sk.row + key) * p.ldk + h * W;
     bf16_t* dvp = p.dv + (int64_t)b * p.bdv * (p.cu_k == nullptr) + (sk.row + key) * p.ldv + h * W;
 #pragma unroll
-    for (int t = 0; t < NV; ++t) store_block32(dvp + t * 32, dv[t], half, live);
+    for (int t = 0; t < NV; ++t) {
+        if constexpr (DROP) dv[t] *= dscale;
+        store_block32(dvp + t * 32, dv[t], half, live);
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
