@@ -91,9 +91,9 @@ class RotaryPositions(object):
 
     def turns(self, device):
         """float64 [rotary_dim / 2] on `device`: turns per position (angle / 2 pi), made once per device."""
-        device = torch.device(device)
         t = self._turns.get(device)
         if t is None:
+            device = torch.device(device)
             t = torch.tensor([f / (2.0 * math.pi) for f in self.inv_freq], dtype=torch.float64, device=device)
             self._turns[device] = t
         return t

@@ -869,7 +869,9 @@ def _check_same_device(first, name, others):
 
 
 def _rows16(t):
-    """`t` with contiguous rows that start on 16 bytes (a copy when they do not)."""
+    """`t` (rows of a multiple of 8 elements) with contiguous rows that start on 16 bytes; a copy when they do not."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     st = t.stride()
     if st[-1] == 1 and t.data_ptr() % 16 == 0:
         for s, n in zip(st[:-1], t.shape):
@@ -880,9 +882,12 @@ def _rows16(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _rows_like(t):
+    """An empty contiguous tensor like t (empty_like costs half of what new_empty does)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _rotary_launch(x, y, positions, offset, rot, inverse):
-    if x.numel() == 0:
-        return
     shape, sx, sy = x.shape, x.stride(), y.stride()
     if len(shape) == 4:
         B, L, heads, dim = shape
@@ -890,6 +895,8 @@ def _rotary_launch(x, y, positions, offset, rot, inverse):
     else:
         B, (L, heads, dim) = 1, shape
         sx, sy = _I3(0, sx[0], sx[1]), _I3(0, sy[0], sy[1])
+    if B == 0 or L == 0 or heads == 0:
+        return
     pos, pos_b = (None, 0) if positions is None else (positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0)
     r = _lib.UniterRotary(B, L, heads, dim, rot.rotary_dim, rot.turns(x.device).data_ptr(), pos, pos_b, offset, rot.multiplier,
                           rot.interleaved, inverse)
@@ -899,7 +906,7 @@ def _rotary_launch(x, y, positions, offset, rot, inverse):
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, offset, rot):
-        y = x.new_empty(x.shape)
+        y = _rows_like(x)
         _rotary_launch(x, y, positions, offset, rot, False)
         ctx.offset, ctx.rot = offset, rot
         ctx.save_for_backward(positions)
@@ -910,7 +917,7 @@ class _RotaryFn(torch.autograd.Function):
     def backward(ctx, dy):
         positions, = ctx.saved_tensors
         dy = dy if dy.stride(-1) == 1 or dy.numel() == 0 else dy.contiguous()
-        dx = dy.new_empty(dy.shape)
+        dx = _rows_like(dy)
         _rotary_launch(dy, dx, positions, ctx.offset, ctx.rot, True)
         return dx, None, None, None
 
@@ -923,21 +930,26 @@ def rotary(x, positions, rot, offset=0, out=None):
     0 .. L - 1 (of every row of the batch); `offset` is added to either.  Returns a new tensor; out=x turns x in place, out=another
     tensor of x's shape writes there (both outside autograd only).  The gradient is turned back by the same kernel."""
     _check_dev(x, "rotary input")
-    nd = x.dim()
-    if nd not in (3, 4) or x.shape[-1] != rot.head_dim:
-        raise _lib.UniterHipError("rotary input must be [B, L, heads, %d] or [T, heads, %d], got %s" % (rot.head_dim, rot.head_dim, tuple(x.shape)))
+    shape = x.shape
+    nd = len(shape)
+    if nd not in (3, 4) or shape[-1] != rot.head_dim:
+        raise _lib.UniterHipError("rotary input must be [B, L, heads, %d] or [T, heads, %d], got %s" % (rot.head_dim, rot.head_dim, tuple(shape)))
     if positions is None:
         if nd == 3:
             raise _lib.UniterHipError("rotary: rows stored back to back need their positions")
     else:
-        if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int64, torch.int32):
+        kind = positions.dtype if isinstance(positions, torch.Tensor) else None
+        if kind is not torch.int64 and kind is not torch.int32:
             raise _lib.UniterHipError("rotary: positions must be an int64 or int32 tensor (or None)")
-        _check_same_device(x, "x", ((positions, "positions"),))
-        if nd == 4 and positions.dim() == 2 and positions.shape[0] == 1:
+        if positions.get_device() != x.get_device():
+            raise _lib.UniterHipError("positions is on %s, x on %s" % (positions.device, x.device))
+        at = positions.shape
+        if nd == 4 and len(at) == 2 and at[0] == 1 != shape[0]:
             positions = positions[0]
-        if positions.shape != x.shape[:-2] and positions.shape != x.shape[-3:-2]:
-            raise _lib.UniterHipError("rotary: positions must be %s or %s, got %s" % (list(x.shape[:-2]), list(x.shape[-3:-2]), list(positions.shape)))
-        if positions.dtype != torch.int64:
+            at = at[1:]
+        if at != shape[:-2] and at != shape[-3:-2]:
+            raise _lib.UniterHipError("rotary: positions must be %s or %s, got %s" % (list(shape[:-2]), list(shape[-3:-2]), list(at)))
+        if kind is torch.int32:
             positions = positions.to(torch.int64)
         if positions.stride(-1) != 1:
             positions = positions.contiguous()
@@ -948,7 +960,7 @@ def rotary(x, positions, rot, offset=0, out=None):
     if out is None:
         if x.requires_grad and torch.is_grad_enabled():
             return _RotaryFn.apply(x, positions, int(offset), rot)
-        out = x.new_empty(x.shape)
+        out = _rows_like(x)
     else:
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise _lib.UniterHipError("rotary: out= writes outside autograd; call it without gradients or let it return a new tensor")
@@ -993,17 +1005,22 @@ def _qkv_of(t, k, v):
 
 def _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams):
     heads, dim, lambda_init, eps, max_q, max_k, p, seed, off = cfg
-    ptrs, rows, batches = _qkv_of(q, k, v)
+    (pq, pk, pv), rows, batches = _qkv_of(q, k, v)
     if cu_q is None:
-        Lq = q.shape[1]
-        packed = (None, None, 0, 0)
-        B, Lk = q.shape[0], Lq if k is None else k.shape[1]
+        B, Lq = q.shape[:2]
+        Lk = Lq if k is None else k.shape[1]
+        cu_q_p = cu_k_p = None
+        nq = nk = 0
     else:
-        packed = (cu_q.data_ptr(), cu_k.data_ptr(), q.shape[0], q.shape[0] if k is None else k.shape[0])
+        nq = q.shape[0]
+        nk = nq if k is None else k.shape[0]
+        cu_q_p, cu_k_p = cu_q.data_ptr(), cu_k.data_ptr()
         B, Lq, Lk = cu_q.shape[0] - 1, max_q, max_k
-    return _lib.UniterDiffAttention(*ptrs, *rows, *batches, ptr(mask), 0 if mask is None else mask.stride(0), *packed,
-                                    lams[0].data_ptr(), lams[1].data_ptr(), lams[2].data_ptr(), lams[3].data_ptr(), ptr(weight),
-                                    B, Lq, Lk, heads, dim, lambda_init, eps, p, lams[0].dim() == 2, seed, off)
+    mask_p, mask_row = (None, 0) if mask is None else (mask.data_ptr(), mask.stride(0))
+    a, b, c, d = lams
+    return _lib.UniterDiffAttention(pq, pk, pv, *rows, *batches, mask_p, mask_row, cu_q_p, cu_k_p, nq, nk,
+                                    a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(), None if weight is None else weight.data_ptr(),
+                                    B, Lq, Lk, heads, dim, lambda_init, eps, p, a.dim() == 2, seed, off)
 
 
 def _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, keep):
@@ -1012,7 +1029,10 @@ def _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, keep):
     a = _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams)
     H = a.heads * 2 * a.head_dim
     # rows of a packed batch that belong to no example are not written: they are zeros
-    out = (q.new_empty if cu_q is None else q.new_zeros)((*q.shape[:-1], H))
+    if cu_q is None:
+        out = _rows_like(q) if k is not None else q.new_empty((a.B, a.Lq, H))
+    else:
+        out = q.new_zeros((q.shape[0], H))
     saved = maps = stats = ws = None
     if keep:
         n = out.numel() * 2
@@ -1057,11 +1077,11 @@ class _DiffAttentionFn(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, mask, cu_q, cu_k, weight, saved, *lams = ctx.saved_tensors
         dout = _rows16(dout)
-        new = q.new_empty if cu_q is None else q.new_zeros             # rows of no example have no gradient
-        dq = new(q.shape)
+        new = _rows_like if cu_q is None else lambda t: t.new_zeros(t.shape)       # rows of no example have no gradient
+        dq = new(q)
         dk = dv = None
         if k is not None:
-            dk, dv = new(k.shape), new(v.shape)
+            dk, dv = new(k), new(v)
         dlams = q.new_empty((4, *lams[0].shape)).unbind(0)
         dweight = None if weight is None else torch.empty_like(weight)
         _diff_backward(q, k, v, mask, cu_q, cu_k, ctx.cfg, weight, lams, saved, dout, dq, dk, dv, dlams, dweight, False)
@@ -1209,7 +1229,7 @@ def _bert_diff_forward(xc, mask, positions, cu, max_len, att, p, keep):
 def _bert_diff_backward(qkv, mask, positions, cu, cfg, att, saved, dout):
     """Gradient of the projection's output; those of lambda and of the per-head norm are accumulated into `.grad`."""
     H = qkv.shape[-1] // 3
-    dqkv = (qkv.new_empty if cu is None else qkv.new_zeros)(qkv.shape)
+    dqkv = _rows_like(qkv) if cu is None else qkv.new_zeros(qkv.shape)
     dl = [ensure_grad(t) if t.requires_grad else None for t in att.lambdas()]
     w = att.LayerNorm.weight
     dw = ensure_grad(w) if w.requires_grad else None
