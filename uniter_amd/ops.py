@@ -1063,10 +1063,12 @@ def _diff_backward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, saved, dout, dq
 
 
 class _DiffAttentionFn(torch.autograd.Function):
-    """fused: `q` is the whole [.., 3 H] projection (k, v None), and so is its gradient."""
+    """fused: `q` is the whole [.., 3 H] projection (k, v None), and so is its gradient.  fixed: what has no gradient, in one argument
+    (apply's own work goes with their number)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, mask, cu_q, cu_k, cfg, weight, *lams):
+    def forward(ctx, fixed, q, k, v, weight, *lams):
+        mask, cu_q, cu_k, cfg = fixed
         out, saved = _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, True)
         ctx.cfg = cfg
         ctx.save_for_backward(q, k, v, mask, cu_q, cu_k, weight, saved, *lams)
@@ -1085,7 +1087,7 @@ class _DiffAttentionFn(torch.autograd.Function):
         dlams = q.new_empty((4, *lams[0].shape)).unbind(0)
         dweight = None if weight is None else torch.empty_like(weight)
         _diff_backward(q, k, v, mask, cu_q, cu_k, ctx.cfg, weight, lams, saved, dout, dq, dk, dv, dlams, dweight, False)
-        return (dq, dk, dv, None, None, None, None, dweight, *dlams)
+        return (None, dq, dk, dv, dweight, *dlams)
 
 
 def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, eps, p_drop):
@@ -1164,7 +1166,7 @@ def _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop):
     seed, off = _next_offsets(1) if p_drop > 0.0 else (0, 0)
     cfg = (heads, dim, lambda_init, eps, max_q, max_k, p_drop, seed, off)
     if torch.is_grad_enabled() and any([t.requires_grad for t in (q, k, v, weight, *lams) if t is not None]):
-        return _DiffAttentionFn.apply(q, k, v, mask, cu_q, cu_k, cfg, weight, *lams)
+        return _DiffAttentionFn.apply((mask, cu_q, cu_k, cfg), q, k, v, weight, *lams)
     return _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, False)[0]
 
 
@@ -1244,7 +1246,8 @@ class _BertDiffAttentionFn(torch.autograd.Function):
     """BertDifferentialSelfAttention.forward."""
 
     @staticmethod
-    def forward(ctx, x, mask, positions, cu, max_len, att, p, keep, *anchor):
+    def forward(ctx, x, fixed, *anchor):
+        mask, positions, cu, max_len, att, p, keep = fixed
         xc = x.contiguous()
         out, qkv, saved, ctx.cfg = _bert_diff_forward(xc, mask, positions, cu, max_len, att, p, keep)
         ctx.att = att
@@ -1290,7 +1293,8 @@ class _BertDiffLayerFn(torch.autograd.Function):
     data-gradient GEMMs' epilogues and the four weight gradients in one launch."""
 
     @staticmethod
-    def forward(ctx, x, mask, positions, cu, max_len, layer, ps, keep, *anchor):
+    def forward(ctx, x, fixed, *anchor):
+        mask, positions, cu, max_len, layer, ps, keep = fixed
         att, ao, im, out = layer.attention.self, layer.attention.output, layer.intermediate, layer.output
         H, I = x.shape[-1], im.dense.weight.shape[0]
         st = _lib.stream_ptr()
@@ -1402,7 +1406,7 @@ def bert_differential_self_attention(att, hidden_states, attention_mask=None, po
     _check_mod(prm, "attention parameter")
     params_ready(*prm)
     keep = torch.is_grad_enabled() and (hidden_states.requires_grad or any(q.requires_grad for q in prm))
-    return _BertDiffAttentionFn.apply(hidden_states, mask, positions, cu_seqlens, max_len, att, _p_of(att), keep, *_anchor(prm))
+    return _BertDiffAttentionFn.apply(hidden_states, (mask, positions, cu_seqlens, max_len, att, _p_of(att), keep), *_anchor(prm))
 
 
 def bert_differential_layer(layer, hidden_states, attention_mask=None, positions=None, cu_seqlens=None, max_len=None):
@@ -1418,7 +1422,7 @@ def bert_differential_layer(layer, hidden_states, attention_mask=None, positions
     _check_mod(prm, "layer parameter")
     params_ready(*prm)
     ps = (_p_of(att), _p_of(layer.attention.output), _p_of(layer.output))
-    return _BertDiffLayerFn.apply(hidden_states, mask, positions, cu_seqlens, max_len, layer, ps, track, *_anchor(prm))
+    return _BertDiffLayerFn.apply(hidden_states, (mask, positions, cu_seqlens, max_len, layer, ps, track), *_anchor(prm))
 
 
 # ----------------------------------------------------------------------------------------------------
