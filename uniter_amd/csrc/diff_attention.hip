@@ -1232,18 +1232,28 @@ BwdSpace bwd_space(const UniterDiffAttention* a) {
     return s;
 }
 
-// Splits of the keys in the forward pass.  The time of a launch goes with the waves that share a SIMD times the tiles each goes through
-// (about 1 us with d = 32, 1.5 with d = 64) plus about two tiles' worth of prologue and epilogue; joining costs a second launch (3 us) and
-// the partial sums' way to memory and back.
+// Splits of the keys in the forward pass.  Estimated time (us) of a launch whose fullest CU runs k workgroups side by side: tiles per
+// workgroup, and two tiles' worth of prologue and epilogue, times the most of
+//   one workgroup's own round (latency of its transfers and products):  2.0 (d = 32), 3.0 (d = 64)
+//   its share of HBM where no other query block reads the same keys:   0.79 k, 1.58 k (16 / 32 KiB at 5.3 TB/s over 256 CUs)
+//   the SIMDs' work:                                                   1.13, 1.85 per wave that shares one
+// and joining costs a second launch and the partial sums' way to memory and back.  One query, keys out of memory (us): 4 x 12 heads, d = 32,
+// 16381 keys: 16 splits (3 workgroups on every CU) 47, 20 50, 10 60; 8 x 8 heads, d = 64, 8192 keys: 8 splits 64, 16 68, 4 104; 6 heads,
+// d = 64, 32768 keys: 85 splits 40, 64 41, 16 104.
 int splits_for(const UniterDiffAttention* a) {
+    const bool wide = a->head_dim == 64;
     const int nw = waves_for(a->Lq);
-    const int64_t wg = a->B * a->heads * ((a->Lq + 32 * nw - 1) / (32 * nw)), nt = (a->Lk + KT - 1) / KT;
-    const double tile = a->head_dim == 32 ? 1.0 : 1.5, part = (double)(a->B * a->heads * a->Lq) * (16.0 * a->head_dim + 16.0) * 2e-6 / 2.5;
+    const int64_t nqb = (a->Lq + 32 * nw - 1) / (32 * nw), wg = a->B * a->heads * nqb, nt = (a->Lk + KT - 1) / KT;
+    const int side = wide ? 2 : nw == 4 ? 3 : 4;               // workgroups per CU: LDS (66 / 33 KiB), three waves per SIMD with d = 32
+    const double alone = wide ? 3.0 : 2.0, simd = wide ? 1.85 : 1.13, hbm = (wide ? 1.58 : 0.79) / (double)nqb;
+    const double part = (double)(a->B * a->heads * a->Lq) * (16.0 * a->head_dim + 16.0) * 2e-6 / 2.5;
     int best = 1;
     double cost = 1e30;
-    for (int ns = 1; ns <= 64 && ns <= nt && wg * ns <= 4096 + wg; ++ns) {
-        const double c = tile * (double)((wg * ns * nw + 1023) / 1024) * (double)((nt + ns - 1) / ns + 2) + (ns > 1 ? 3.0 + ns * part : 0.0);
-        if (c < cost) { cost = c; best = ns; }
+    for (int64_t ns = 1; ns <= 256 && ns <= nt && wg * ns <= 1024 + wg; ++ns) {
+        const int64_t c = (wg * ns + 255) / 256;
+        auto round = [&](int64_t k) { return fmax(alone, fmax(hbm * (double)k, simd * (double)((k * nw + 3) / 4))); };
+        const double t = (double)((nt + ns - 1) / ns + 2) * ((double)(c / side) * round(side) + (c % side ? round(c % side) : 0.0)) + (ns > 1 ? 5.5 + (double)ns * part : 0.0);
+        if (t < cost) { cost = t; best = (int)ns; }
     }
     return best;
 }
