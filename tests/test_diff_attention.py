@@ -728,3 +728,7 @@ def test_refusals():
     first, = torch.autograd.grad(f(x, k, k, 2, lam, 0.5), x, q, create_graph=True)
     with pytest.raises(RuntimeError):                                       # no second derivative
         torch.autograd.grad(first.sum(), x)
+    dy = q.clone().requires_grad_(True)
+    first, = torch.autograd.grad(f(x, k, k, 2, lam, 0.5), x, dy, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.float().square().sum(), dy)

@@ -205,6 +205,25 @@ def test_refusals():
 
 
 @pytest.mark.gpu
+def test_an_entry_that_refuses_raises_the_packages_error():
+    """Past the Python checks: the status of the C entry, with its message."""
+    x, turns = torch.zeros(1, 2, 3, 64, dtype=BF16, device="cuda"), torch.zeros(32, dtype=torch.float64, device="cuda")
+    for leaf in (x, x.clone().requires_grad_(True)):
+        with pytest.raises(_lib.UniterHipError, match="rot_dim"):
+            _lib.nodes().rotary(leaf, None, None, 0, turns, 7, 1.0, False, False)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    rot = RotaryPositions(64)
+    x = torch.randn(1, 2, 3, 64).to(BF16).cuda().requires_grad_(True)
+    dy = torch.randn(1, 2, 3, 64).to(BF16).cuda().requires_grad_(True)
+    dx, = torch.autograd.grad(ops.rotary(x, None, rot), x, dy, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.float().square().sum(), dy)
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """The map is linear: y(x + h) - y(x) = y(h).  With x = 0 the difference is the derivative itself, so <y(h), dy> = <h, dx(dy)> up to
     the roundings of y and dx: half a step each, on every product."""

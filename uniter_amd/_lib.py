@@ -250,6 +250,30 @@ def load():
     return lib
 
 
+NODES_PATH = os.path.join(_HERE, "csrc", "build", "uniter_nodes.so")
+_nodes = None
+
+
+def nodes():
+    """The autograd nodes of rotary positions and differential attention (csrc/nodes.cpp), bound to the library that load() has loaded."""
+    global _nodes
+    if _nodes is None:
+        lib = load()
+        if not os.path.exists(NODES_PATH):
+            raise UniterHipError("uniter_nodes.so not found at %s — build it with `python uniter_amd/csrc/build.py`" % NODES_PATH)
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (the module's own libraries)
+        loader = importlib.machinery.ExtensionFileLoader("uniter_nodes", NODES_PATH)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("uniter_nodes", loader))
+        loader.exec_module(mod)
+        names = ("uniter_rotary", "uniter_diff_attention_fwd_workspace_bytes", "uniter_diff_attention_fwd",
+                 "uniter_diff_attention_bwd_workspace_bytes", "uniter_diff_attention_bwd", "uniter_hip_last_error")
+        mod.init({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, UniterHipError)
+        _nodes = mod
+    return _nodes
+
+
 class _Checked:
     """Attribute access returns a wrapper that raises on a non-zero status."""
 

@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""Build libuniter_hip.so (gfx950) in-tree with hipcc.
+"""Build libuniter_hip.so (gfx950) in-tree with hipcc, and uniter_nodes.so (nodes.cpp: host code, autograd nodes) with g++.
 
     python uniter_amd/csrc/build.py [--force] [--verbose]
 
@@ -8,11 +8,13 @@ objects whose sources (or the headers they include) are newer.  hipcc cross-comp
 """
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
@@ -20,6 +22,7 @@ ROOT = os.path.dirname(os.path.dirname(HERE))
 #  a variant up through UNITER_AMD_LIB=<path to its libuniter_hip.so> / LD_LIBRARY_PATH for the native harness)
 BUILD = os.path.join(HERE, os.environ.get("UNITER_BUILD_DIR", "build"))
 LIB = os.path.join(BUILD, "libuniter_hip.so")
+NODES = os.path.join(BUILD, "uniter_nodes.so")
 SOURCES = ["capi.hip", "gemm.hip", "attention.hip", "layernorm.hip", "embed.hip", "adamw.hip", "encoder.hip", "comm.hip", "ot.hip", "pool.hip", "lmhead.hip", "head.hip", "rotary.hip",
            "diff_attention.hip"]
 ARCH = "gfx950"
@@ -54,6 +57,29 @@ def _sources_of(path, seen=None):
     return seen
 
 
+def build_nodes(force=False, verbose=False):
+    """nodes.cpp against the torch that is installed (found without importing it).  It links no part of libuniter_hip.so."""
+    src = os.path.join(HERE, "nodes.cpp")
+    if not force and not _stale(NODES, _sources_of(src)):
+        return NODES
+    os.makedirs(BUILD, exist_ok=True)
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    inc = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D_GLIBCXX_USE_CXX11_ABI=1", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-DTORCH_EXTENSION_NAME=uniter_nodes"]
+    for d in inc:
+        cmd += ["-isystem", d]
+    cmd += [src, "-o", NODES, "-L" + os.path.join(torch, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed on %s" % src)
+    return NODES
+
+
 def build(force=False, verbose=False):
     hipcc = find_hipcc()
     os.makedirs(BUILD, exist_ok=True)
@@ -76,14 +102,15 @@ def build(force=False, verbose=False):
         r = subprocess.run(cmd, capture_output=True, text=True)
         return s, r
 
-    if jobs:
-        with cf.ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
-            for s, r in ex.map(compile_one, jobs):
-                if r.returncode != 0:
-                    sys.stderr.write(r.stdout + r.stderr)
-                    raise RuntimeError("hipcc failed on %s" % s)
-                if verbose and r.stderr:
-                    sys.stderr.write(r.stderr)
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(jobs) + 1)) as ex:
+        nodes = ex.submit(build_nodes, force, verbose)
+        for s, r in ex.map(compile_one, jobs):
+            if r.returncode != 0:
+                sys.stderr.write(r.stdout + r.stderr)
+                raise RuntimeError("hipcc failed on %s" % s)
+            if verbose and r.stderr:
+                sys.stderr.write(r.stderr)
+        nodes.result()
     if jobs or force or _stale(LIB, objs):
         cmd = [hipcc, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", LIB] + objs + ["-ldl"]
         if verbose:

@@ -1,0 +1,310 @@
+// nodes.cpp — the autograd nodes of the operators whose calls are short: rotary positions and differential attention.
+//
+// A training call of these operators is three to five kernels of 5 to 25 us.  As Python autograd functions over ctypes their host work is
+// 45 us in a loop that stays in the CPU's caches and twice that when autograd's own thread takes the backward half to another core; here
+// it is C++ on both sides and the backward pass needs no interpreter.  The kernels are reached through the C ABI all the same: the
+// package hands over the addresses of the entry points of the library that it has loaded (init), nothing is linked.
+//
+// Arguments arrive checked (uniter_amd/ops.py); workspaces come from torch's caching allocator.
+#include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <c10/core/DeviceGuard.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include "../../include/uniter_hip.h"
+
+namespace {
+
+using at::Tensor;
+using std::optional;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Entries {
+    decltype(&uniter_rotary) rotary;
+    decltype(&uniter_diff_attention_fwd_workspace_bytes) fwd_bytes;
+    decltype(&uniter_diff_attention_fwd) fwd;
+    decltype(&uniter_diff_attention_bwd_workspace_bytes) bwd_bytes;
+    decltype(&uniter_diff_attention_bwd) bwd;
+    decltype(&uniter_hip_last_error) last_error;
+} lib{};
+PyObject* error_type = nullptr;
+
+struct Error : std::runtime_error { using std::runtime_error::runtime_error; };
+
+void ok(int rc, const char* name) {
+    if (rc == 0) return;
+    const char* why = lib.last_error();
+    throw Error(std::string(name) + " failed with status " + std::to_string(rc) + ": " + (why ? why : ""));
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor get(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
+Tensor rows_like(const Tensor& t) { return at::empty_like(t, t.options(), at::MemoryFormat::Contiguous); }
+// contiguous rows that start on 16 bytes (row strides of whole 8s); a copy where they do not
+Tensor rows16(const Tensor& t) {
+    bool fits = t.stride(-1) == 1 && (uintptr_t)t.data_ptr() % 16 == 0;
+    for (int64_t i = 0; fits && i + 1 < t.dim(); ++i) fits = t.stride(i) % 8 == 0 || t.size(i) == 1;
+    return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// Gradients of a pass that has no derivative of its own: where the incoming gradient wants one, asking for it is an error.
+variable_list once(variable_list grads, const Tensor& incoming) {
+    if (!at::GradMode::is_enabled() || !incoming.requires_grad()) return grads;
+    variable_list known;
+    for (auto& g : grads)
+        if (g.defined()) known.push_back(g);
+    auto error = std::make_shared<torch::autograd::DelayedError>("the gradient of this operator has no derivative", (int64_t)known.size());
+    known = (*error)(std::move(known));
+    size_t i = 0;
+    for (auto& g : grads)
+        if (g.defined()) g = known[i++];
+    return grads;
+}
+
+// ------------------------------------------------------------------------------------------------
+// rotary positions
+// ------------------------------------------------------------------------------------------------
+struct Rotary {
+    Tensor positions;                    // int64 [L] / [B, L] / [T], or undefined
+    Tensor turns;                        // float64 [rot / 2]
+    int64_t offset, rot;
+    double multiplier;
+    bool interleaved;
+};
+
+void rotary_run(const Tensor& x, const Tensor& y, const Rotary& r, bool inverse) {
+    if (x.numel() == 0) return;
+    const int64_t d = x.dim();
+    UniterRotary a{};
+    a.B = d == 4 ? x.size(0) : 1;
+    a.L = x.size(-3); a.heads = x.size(-2); a.head_dim = x.size(-1);
+    a.rot_dim = r.rot;
+    a.freq = (const double*)r.turns.data_ptr();
+    if (r.positions.defined()) {
+        a.positions = (const int64_t*)r.positions.data_ptr();
+        a.positions_batch_stride = r.positions.dim() == 2 ? r.positions.stride(0) : 0;
+    }
+    a.position_offset = r.offset;
+    a.multiplier = (float)r.multiplier;
+    a.interleaved = r.interleaved;
+    a.inverse = inverse;
+    const int64_t sx[3] = {d == 4 ? x.stride(0) : 0, x.stride(-3), x.stride(-2)}, sy[3] = {d == 4 ? y.stride(0) : 0, y.stride(-3), y.stride(-2)};
+    const c10::DeviceGuard on(x.device());
+    ok(lib.rotary(&a, x.data_ptr(), sx, y.data_ptr(), sy, stream_of(x)), "uniter_rotary");
+}
+
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Rotary& r) {
+        Tensor y = rows_like(x);
+        rotary_run(x, y, r, false);
+        ctx->save_for_backward({r.positions, r.turns});
+        ctx->saved_data["n"] = std::vector<int64_t>{r.offset, r.rot, r.interleaved};
+        ctx->saved_data["m"] = r.multiplier;
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list t = ctx->get_saved_variables();
+        const auto n = ctx->saved_data["n"].toIntVector();
+        const Rotary r{t[0], t[1], n[0], n[1], ctx->saved_data["m"].toDouble(), n[2] != 0};
+        Tensor dy = grads[0];
+        if (!dy.defined()) return {Tensor(), Tensor()};
+        if (dy.stride(-1) != 1) dy = dy.contiguous();
+        Tensor dx = rows_like(dy);
+        rotary_run(dy, dx, r, true);
+        return once({dx, Tensor()}, grads[0]);
+    }
+};
+
+Tensor rotary(const Tensor& x, const optional<Tensor>& out, const optional<Tensor>& positions, int64_t offset, const Tensor& turns, int64_t rot,
+              double multiplier, bool interleaved, bool inverse) {
+    const Rotary r{get(positions), turns, offset, rot, multiplier, interleaved};
+    if (!out.has_value() && !inverse && at::GradMode::is_enabled() && x.requires_grad()) return RotaryNode::apply(x, r);
+    Tensor y = out.has_value() ? *out : rows_like(x);
+    rotary_run(x, y, r, inverse);
+    return y;
+}
+
+// ------------------------------------------------------------------------------------------------
+// differential attention
+// ------------------------------------------------------------------------------------------------
+struct Fixed {                           // what a call has besides its differentiable tensors
+    Tensor mask, cu_q, cu_k;
+    int64_t heads, dim, max_q, max_k, seed, offset;
+    double lambda_init, eps, p_drop;
+    bool keep;                           // a backward pass will come
+};
+struct Operands {                        // k and v undefined: q is a fused [.., 3 H] projection
+    Tensor q, k, v, weight, lams[4];
+};
+
+// q, k, v (or dq, dk, dv): three tensors, or the thirds of one projection's rows
+template <class A>
+void set_rows(A& a, const Tensor& q, const Tensor& k, const Tensor& v) {
+    char* p = (char*)q.data_ptr();
+    const bool fused = !k.defined();
+    const int64_t third = fused ? q.size(-1) / 3 * 2 : 0;      // bytes
+    a.q = p;
+    a.k = fused ? (p ? p + third : nullptr) : k.data_ptr();
+    a.v = fused ? (p ? p + 2 * third : nullptr) : v.data_ptr();
+    a.q_row = q.stride(-2);
+    a.k_row = fused ? a.q_row : k.stride(-2);
+    a.v_row = fused ? a.q_row : v.stride(-2);
+    a.q_batch = q.stride(0);
+    a.k_batch = fused ? a.q_batch : k.stride(0);
+    a.v_batch = fused ? a.q_batch : v.stride(0);
+}
+
+UniterDiffAttention args_of(const Operands& t, const Fixed& f) {
+    UniterDiffAttention a{};
+    set_rows(a, t.q, t.k, t.v);
+    const bool fused = !t.k.defined();
+    if (f.mask.defined()) {
+        a.mask_bias = (const float*)f.mask.data_ptr();
+        a.mask_row = f.mask.stride(0);
+    }
+    if (f.cu_q.defined()) {
+        a.cu_seqlens_q = (const int32_t*)f.cu_q.data_ptr();
+        a.cu_seqlens_k = (const int32_t*)f.cu_k.data_ptr();
+        a.total_q = t.q.size(0);
+        a.total_k = fused ? a.total_q : t.k.size(0);
+        a.B = f.cu_q.size(0) - 1;
+        a.Lq = f.max_q; a.Lk = f.max_k;
+    } else {
+        a.B = t.q.size(0);
+        a.Lq = t.q.size(1);
+        a.Lk = fused ? a.Lq : t.k.size(1);
+    }
+    a.lambda_q1 = t.lams[0].data_ptr(); a.lambda_k1 = t.lams[1].data_ptr();
+    a.lambda_q2 = t.lams[2].data_ptr(); a.lambda_k2 = t.lams[3].data_ptr();
+    a.lambda_per_head = t.lams[0].dim() == 2;
+    a.norm_weight = ptr(t.weight);
+    a.heads = f.heads; a.head_dim = f.dim;
+    a.lambda_init = (float)f.lambda_init; a.norm_eps = (float)f.eps; a.p_drop = (float)f.p_drop;
+    a.seed = (uint64_t)f.seed; a.offset = (uint64_t)f.offset;
+    return a;
+}
+
+// (out, saved): saved (fp32: both maps' outputs, then the rows' statistics) only where a backward pass will want it
+std::pair<Tensor, Tensor> diff_forward(const Operands& t, const Fixed& f) {
+    UniterDiffAttention a = args_of(t, f);
+    const int64_t H = f.heads * 2 * f.dim;
+    // (rows of a packed batch that belong to no example are not written: they are zeros)
+    Tensor out = f.cu_q.defined() ? at::zeros({t.q.size(0), H}, t.q.options()) : at::empty({a.B, a.Lq, H}, t.q.options());
+    Tensor saved, ws;
+    float *maps = nullptr, *stats = nullptr;
+    if (f.keep) {
+        const int64_t n = out.numel() * 2;
+        saved = at::empty({n + a.B * a.heads * a.Lq * 4}, t.q.options().dtype(at::kFloat));
+        maps = (float*)saved.data_ptr();
+        stats = maps ? maps + n : nullptr;
+    }
+    const c10::DeviceGuard on(t.q.device());
+    const size_t bytes = lib.fwd_bytes(&a);
+    if (bytes) ws = at::empty({(int64_t)bytes}, t.q.options().dtype(at::kByte));
+    ok(lib.fwd(&a, out.data_ptr(), H, out.stride(0), stats, maps, ptr(ws), bytes, stream_of(t.q)), "uniter_diff_attention_fwd");
+    return {out, saved};
+}
+
+// dq / dk / dv: like q / k / v (one [.., 3 H] tensor for a fused projection); undefined parameter gradients are not formed
+void diff_backward(const Operands& t, const Fixed& f, const Tensor& saved, const Tensor& incoming, const Operands& d, bool accumulate) {
+    UniterDiffAttention a = args_of(t, f);
+    UniterDiffAttentionGrads g{};
+    set_rows(g, d.q, d.k, d.v);
+    g.lambda_q1 = ptr(d.lams[0]); g.lambda_k1 = ptr(d.lams[1]); g.lambda_q2 = ptr(d.lams[2]); g.lambda_k2 = ptr(d.lams[3]);
+    g.norm_weight = ptr(d.weight);
+    g.accumulate_params = accumulate;
+    const Tensor dout = rows16(incoming);
+    const c10::DeviceGuard on(t.q.device());
+    const size_t bytes = lib.bwd_bytes(&a);
+    Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 16)}, t.q.options().dtype(at::kByte));
+    const float* maps = (const float*)saved.data_ptr();
+    ok(lib.bwd(&a, maps ? maps + 2 * dout.numel() : nullptr, maps, dout.data_ptr(), dout.stride(-2), dout.stride(0), &g, ws.data_ptr(), bytes,
+               stream_of(t.q)), "uniter_diff_attention_bwd");
+}
+
+struct DiffNode : torch::autograd::Function<DiffNode> {
+    static Tensor forward(AutogradContext* ctx, const Fixed& f, const Tensor& q, const optional<Tensor>& k, const optional<Tensor>& v,
+                          const optional<Tensor>& weight, const Tensor& l0, const Tensor& l1, const Tensor& l2, const Tensor& l3) {
+        const Operands t{q, get(k), get(v), get(weight), {l0, l1, l2, l3}};
+        auto [out, saved] = diff_forward(t, f);
+        ctx->save_for_backward({q, t.k, t.v, t.weight, l0, l1, l2, l3, f.mask, f.cu_q, f.cu_k, saved});
+        ctx->saved_data["n"] = std::vector<int64_t>{f.heads, f.dim, f.max_q, f.max_k, f.seed, f.offset};
+        ctx->saved_data["x"] = std::vector<double>{f.lambda_init, f.eps, f.p_drop};
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        if (!grads[0].defined()) return variable_list(9);
+        const variable_list s = ctx->get_saved_variables();
+        const auto n = ctx->saved_data["n"].toIntVector();
+        const auto x = ctx->saved_data["x"].toDoubleVector();
+        const Operands t{s[0], s[1], s[2], s[3], {s[4], s[5], s[6], s[7]}};
+        const Fixed f{s[8], s[9], s[10], n[0], n[1], n[2], n[3], n[4], n[5], x[0], x[1], x[2], true};
+        const at::AutoDispatchBelowADInplaceOrView below;      // (buffers of kernels: nothing here is recorded)
+        auto like = [&](const Tensor& a) { return !a.defined() ? Tensor() : f.cu_q.defined() ? at::zeros(a.sizes(), a.options()) : rows_like(a); };
+        Operands d{like(t.q), like(t.k), like(t.v), t.weight.defined() ? rows_like(t.weight) : Tensor(), {}};
+        for (int i = 0; i < 4; ++i) d.lams[i] = rows_like(t.lams[i]);
+        diff_backward(t, f, s[11], grads[0], d, false);
+        return once({Tensor(), d.q, d.k, d.v, d.weight, d.lams[0], d.lams[1], d.lams[2], d.lams[3]}, grads[0]);
+    }
+};
+
+Fixed fixed_of(const optional<Tensor>& mask, const optional<Tensor>& cu_q, const optional<Tensor>& cu_k, int64_t heads, int64_t dim, double lambda_init,
+               double eps, int64_t max_q, int64_t max_k, double p_drop, int64_t seed, int64_t offset, bool keep) {
+    return Fixed{get(mask), get(cu_q), get(cu_k), heads, dim, max_q, max_k, seed, offset, lambda_init, eps, p_drop, keep};
+}
+
+void init(py::dict addresses, py::object error) {
+    auto at = [&](const char* name) { return addresses[name].cast<uintptr_t>(); };
+    lib.rotary = (decltype(lib.rotary))at("uniter_rotary");
+    lib.fwd_bytes = (decltype(lib.fwd_bytes))at("uniter_diff_attention_fwd_workspace_bytes");
+    lib.fwd = (decltype(lib.fwd))at("uniter_diff_attention_fwd");
+    lib.bwd_bytes = (decltype(lib.bwd_bytes))at("uniter_diff_attention_bwd_workspace_bytes");
+    lib.bwd = (decltype(lib.bwd))at("uniter_diff_attention_bwd");
+    lib.last_error = (decltype(lib.last_error))at("uniter_hip_last_error");
+    error_type = error.release().ptr();
+}
+
+}  // namespace
+
+PYBIND11_MODULE(uniter_nodes, m) {
+    py::register_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const Error& e) {
+            PyErr_SetString(error_type ? error_type : PyExc_RuntimeError, e.what());
+        }
+    });
+    m.def("init", &init);
+    // (without the interpreter lock, as torch's own operators: a launch may wait for room in its queue)
+    using unlocked = py::call_guard<py::gil_scoped_release>;
+    m.def("rotary", &rotary, unlocked());
+    m.def("diff_attention", [](const Tensor& q, const optional<Tensor>& k, const optional<Tensor>& v, const optional<Tensor>& weight, const Tensor& l0,
+                               const Tensor& l1, const Tensor& l2, const Tensor& l3, const optional<Tensor>& mask, const optional<Tensor>& cu_q,
+                               const optional<Tensor>& cu_k, int64_t heads, int64_t dim, double lambda_init, double eps, int64_t max_q, int64_t max_k,
+                               double p_drop, int64_t seed, int64_t offset) {
+        auto wants = [](const optional<Tensor>& t) { return t.has_value() && t->requires_grad(); };
+        const bool keep = at::GradMode::is_enabled() && (q.requires_grad() || wants(k) || wants(v) || wants(weight) || l0.requires_grad() ||
+                                                         l1.requires_grad() || l2.requires_grad() || l3.requires_grad());
+        const Fixed f = fixed_of(mask, cu_q, cu_k, heads, dim, lambda_init, eps, max_q, max_k, p_drop, seed, offset, keep);
+        if (keep) return DiffNode::apply(f, q, k, v, weight, l0, l1, l2, l3);
+        return diff_forward(Operands{q, get(k), get(v), get(weight), {l0, l1, l2, l3}}, f).first;
+    }, unlocked());
+    // the two passes by themselves, on a fused projection, for nodes that hold more than the attention
+    m.def("diff_self_forward", [](const Tensor& qkv, const optional<Tensor>& weight, const std::vector<Tensor>& l, const optional<Tensor>& mask,
+                                  const optional<Tensor>& cu, int64_t heads, int64_t dim, double lambda_init, double eps, int64_t max_len, double p_drop,
+                                  int64_t seed, int64_t offset, bool keep) -> std::pair<Tensor, optional<Tensor>> {
+        auto [out, saved] = diff_forward(Operands{qkv, Tensor(), Tensor(), get(weight), {l[0], l[1], l[2], l[3]}},
+                                         fixed_of(mask, cu, cu, heads, dim, lambda_init, eps, max_len, max_len, p_drop, seed, offset, keep));
+        return {out, saved.defined() ? optional<Tensor>(saved) : std::nullopt};
+    }, unlocked());
+    m.def("diff_self_backward", [](const Tensor& qkv, const optional<Tensor>& weight, const std::vector<Tensor>& l, const optional<Tensor>& mask,
+                                   const optional<Tensor>& cu, int64_t heads, int64_t dim, double lambda_init, double eps, int64_t max_len, double p_drop,
+                                   int64_t seed, int64_t offset, const Tensor& saved, const Tensor& dout, const Tensor& dqkv,
+                                   const optional<Tensor>& dweight, const std::vector<optional<Tensor>>& dl, bool accumulate) {
+        diff_backward(Operands{qkv, Tensor(), Tensor(), get(weight), {l[0], l[1], l[2], l[3]}},
+                      fixed_of(mask, cu, cu, heads, dim, lambda_init, eps, max_len, max_len, p_drop, seed, offset, true), saved, dout,
+                      Operands{dqkv, Tensor(), Tensor(), get(dweight), {get(dl[0]), get(dl[1]), get(dl[2]), get(dl[3])}}, accumulate);
+    }, unlocked());
+}

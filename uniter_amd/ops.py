@@ -849,18 +849,6 @@ def dense_gelu(mod, hidden_states):
 # rotary positions and differential attention (no counterpart in the reference: they stand beside BertSelfAttention's learned
 # positions and softmax attention, model/layer.py:75-101, model/model.py:217-245)
 # ----------------------------------------------------------------------------------------------------
-_I3 = ctypes.c_int64 * 3
-
-
-def _launch_on(t, fn, *args):
-    """fn(*args, stream) on t's device (the current one or not) and that device's current stream."""
-    if t.get_device() == torch._C._cuda_getDevice():
-        fn(*args, _lib.stream_ptr())
-    else:
-        with torch.cuda.device(t.device):
-            fn(*args, _lib.stream_ptr())
-
-
 def _check_same_device(first, name, others):
     dev = first.get_device()
     for t, what in others:
@@ -882,44 +870,9 @@ def _rows16(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _rows_like(t):
-    """An empty contiguous tensor like t (empty_like costs half of what new_empty does)."""
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
-
-
-def _rotary_launch(x, y, positions, offset, rot, inverse):
-    shape, sx, sy = x.shape, x.stride(), y.stride()
-    if len(shape) == 4:
-        B, L, heads, dim = shape
-        sx, sy = _I3(sx[0], sx[1], sx[2]), _I3(sy[0], sy[1], sy[2])
-    else:
-        B, (L, heads, dim) = 1, shape
-        sx, sy = _I3(0, sx[0], sx[1]), _I3(0, sy[0], sy[1])
-    if B == 0 or L == 0 or heads == 0:
-        return
-    pos, pos_b = (None, 0) if positions is None else (positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0)
-    r = _lib.UniterRotary(B, L, heads, dim, rot.rotary_dim, rot.turns(x.device).data_ptr(), pos, pos_b, offset, rot.multiplier,
-                          rot.interleaved, inverse)
-    _launch_on(x, C.uniter_rotary, ctypes.byref(r), x.data_ptr(), sx, y.data_ptr(), sy)
-
-
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, positions, offset, rot):
-        y = _rows_like(x)
-        _rotary_launch(x, y, positions, offset, rot, False)
-        ctx.offset, ctx.rot = offset, rot
-        ctx.save_for_backward(positions)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        positions, = ctx.saved_tensors
-        dy = dy if dy.stride(-1) == 1 or dy.numel() == 0 else dy.contiguous()
-        dx = _rows_like(dy)
-        _rotary_launch(dy, dx, positions, ctx.offset, ctx.rot, True)
-        return dx, None, None, None
+def _turn(x, out, positions, offset, rot, inverse=False):
+    """The kernel (csrc/nodes.cpp); out None: a new tensor, and a node where x wants a gradient."""
+    return _lib.nodes().rotary(x, out, positions, offset, rot.turns(x.device), rot.rotary_dim, rot.multiplier, rot.interleaved, inverse)
 
 
 def rotary(x, positions, rot, offset=0, out=None):
@@ -957,11 +910,7 @@ def rotary(x, positions, rot, offset=0, out=None):
         if out is x:
             raise _lib.UniterHipError("rotary: in place needs contiguous heads")
         x = x.contiguous()
-    if out is None:
-        if x.requires_grad and torch.is_grad_enabled():
-            return _RotaryFn.apply(x, positions, int(offset), rot)
-        out = _rows_like(x)
-    else:
+    if out is not None:
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise _lib.UniterHipError("rotary: out= writes outside autograd; call it without gradients or let it return a new tensor")
         _check_dev(out, "rotary output")
@@ -973,8 +922,7 @@ def rotary(x, positions, rot, offset=0, out=None):
         if out.numel() and (out.data_ptr() != x.data_ptr() or out.stride() != x.stride()) \
                 and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() and _overlap(out, x):
             raise _lib.UniterHipError("rotary: out overlaps x without being x")
-    _rotary_launch(x, out, positions, int(offset), rot, False)
-    return out
+    return _turn(x, out, positions, int(offset), rot)
 
 
 def _overlap(a, b):
@@ -991,103 +939,6 @@ def _overlap(a, b):
         w, d = a.shape[-2] * a.stride(-2), (abs(a0 - b0) // 2) % row
         return d < w or row - d < w
     return True
-
-
-def _qkv_of(t, k, v):
-    """(pointers, row strides, batch strides) of q, k, v: three tensors, or the thirds of one projection's rows (k, v None)."""
-    b = t.stride(0)
-    if k is None:
-        row, third = t.stride(-2), t.shape[-1] // 3 * 2
-        p = t.data_ptr()
-        return (p, p + third, p + 2 * third), (row, row, row), (b, b, b)
-    return ((t.data_ptr(), k.data_ptr(), v.data_ptr()), (t.stride(-2), k.stride(-2), v.stride(-2)), (b, k.stride(0), v.stride(0)))
-
-
-def _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams):
-    heads, dim, lambda_init, eps, max_q, max_k, p, seed, off = cfg
-    (pq, pk, pv), rows, batches = _qkv_of(q, k, v)
-    if cu_q is None:
-        B, Lq = q.shape[:2]
-        Lk = Lq if k is None else k.shape[1]
-        cu_q_p = cu_k_p = None
-        nq = nk = 0
-    else:
-        nq = q.shape[0]
-        nk = nq if k is None else k.shape[0]
-        cu_q_p, cu_k_p = cu_q.data_ptr(), cu_k.data_ptr()
-        B, Lq, Lk = cu_q.shape[0] - 1, max_q, max_k
-    mask_p, mask_row = (None, 0) if mask is None else (mask.data_ptr(), mask.stride(0))
-    a, b, c, d = lams
-    return _lib.UniterDiffAttention(pq, pk, pv, *rows, *batches, mask_p, mask_row, cu_q_p, cu_k_p, nq, nk,
-                                    a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(), None if weight is None else weight.data_ptr(),
-                                    B, Lq, Lk, heads, dim, lambda_init, eps, p, a.dim() == 2, seed, off)
-
-
-def _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, keep):
-    """(out, saved), launched on the current stream; saved (fp32: both maps' outputs, then the rows' statistics) only when a backward pass
-    will want it."""
-    a = _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams)
-    H = a.heads * 2 * a.head_dim
-    # rows of a packed batch that belong to no example are not written: they are zeros
-    if cu_q is None:
-        out = _rows_like(q) if k is not None else q.new_empty((a.B, a.Lq, H))
-    else:
-        out = q.new_zeros((q.shape[0], H))
-    saved = maps = stats = ws = None
-    if keep:
-        n = out.numel() * 2
-        saved = q.new_empty(n + a.B * a.heads * a.Lq * 4, dtype=torch.float32)
-        maps = saved.data_ptr()
-        stats = maps + 4 * n
-    ref = ctypes.byref(a)
-    n = C.uniter_diff_attention_fwd_workspace_bytes(ref)
-    if n:
-        # (workspaces come from the caching allocator, not a shared scratch buffer: other streams and captured graphs get their own)
-        ws = q.new_empty(n, dtype=torch.uint8)
-    _launch_on(q, C.uniter_diff_attention_fwd, ref, out.data_ptr(), H, out.stride(0), stats, maps, ptr(ws), n)
-    return out, saved
-
-
-def _diff_backward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, saved, dout, dq, dk, dv, dlams, dweight, accumulate):
-    """dq / dk / dv: tensors like q / k / v (one [.., 3 H] tensor and None, None for a fused projection)."""
-    a = _diff_struct(q, k, v, mask, cu_q, cu_k, cfg, weight, lams)
-    ptrs, rows, batches = _qkv_of(dq, dk, dv)
-    g = _lib.UniterDiffAttentionGrads(*ptrs, *rows, *batches, ptr(dlams[0]), ptr(dlams[1]), ptr(dlams[2]), ptr(dlams[3]), ptr(dweight),
-                                      accumulate)
-    ref = ctypes.byref(a)
-    n = C.uniter_diff_attention_bwd_workspace_bytes(ref)
-    ws = q.new_empty(max(n, 16), dtype=torch.uint8)
-    maps = saved.data_ptr()
-    _launch_on(q, C.uniter_diff_attention_bwd, ref, maps + 8 * dout.numel(), maps, dout.data_ptr(), dout.stride(-2), dout.stride(0),
-               ctypes.byref(g), ws.data_ptr(), n)
-
-
-class _DiffAttentionFn(torch.autograd.Function):
-    """fused: `q` is the whole [.., 3 H] projection (k, v None), and so is its gradient.  fixed: what has no gradient, in one argument
-    (apply's own work goes with their number)."""
-
-    @staticmethod
-    def forward(ctx, fixed, q, k, v, weight, *lams):
-        mask, cu_q, cu_k, cfg = fixed
-        out, saved = _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, True)
-        ctx.cfg = cfg
-        ctx.save_for_backward(q, k, v, mask, cu_q, cu_k, weight, saved, *lams)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        q, k, v, mask, cu_q, cu_k, weight, saved, *lams = ctx.saved_tensors
-        dout = _rows16(dout)
-        new = _rows_like if cu_q is None else lambda t: t.new_zeros(t.shape)       # rows of no example have no gradient
-        dq = new(q)
-        dk = dv = None
-        if k is not None:
-            dk, dv = new(k), new(v)
-        dlams = q.new_empty((4, *lams[0].shape)).unbind(0)
-        dweight = None if weight is None else torch.empty_like(weight)
-        _diff_backward(q, k, v, mask, cu_q, cu_k, ctx.cfg, weight, lams, saved, dout, dq, dk, dv, dlams, dweight, False)
-        return (None, dq, dk, dv, dweight, *dlams)
 
 
 def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, eps, p_drop):
@@ -1164,10 +1015,7 @@ def _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop):
     if k is not None:
         k, v = _rows16(k), _rows16(v)
     seed, off = _next_offsets(1) if p_drop > 0.0 else (0, 0)
-    cfg = (heads, dim, lambda_init, eps, max_q, max_k, p_drop, seed, off)
-    if torch.is_grad_enabled() and any([t.requires_grad for t in (q, k, v, weight, *lams) if t is not None]):
-        return _DiffAttentionFn.apply((mask, cu_q, cu_k, cfg), q, k, v, weight, *lams)
-    return _diff_forward(q, k, v, mask, cu_q, cu_k, cfg, weight, lams, False)[0]
+    return _lib.nodes().diff_attention(q, k, v, weight, *lams, mask, cu_q, cu_k, heads, dim, lambda_init, eps, max_q or 0, max_k or 0, p_drop, seed, off)
 
 
 def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=None, mask_bias=None, cu_seqlens=None, cu_seqlens_k=None,
@@ -1221,24 +1069,24 @@ def _bert_diff_forward(xc, mask, positions, cu, max_len, att, p, keep):
     C.uniter_gemm_bias_fwd(ptr(xc), ptr(wqkv), ptr(bqkv), ptr(qkv), xc.numel() // H, 3 * H, H, _lib.stream_ptr())
     if att.rotary is not None:
         qk = qkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
-        _rotary_launch(qk, qk, positions, 0, att.rotary, False)
+        _turn(qk, qk, positions, 0, att.rotary)
     seed, off = _next_offsets(1) if p > 0.0 else (0, 0)
-    cfg = (att.num_attention_heads, att.map_size, att.lambda_init, att.LayerNorm.eps, max_len, max_len, p, seed, off)
-    out, saved = _diff_forward(qkv, None, None, mask, cu, cu, cfg, att.LayerNorm.weight, att.lambdas(), keep)
+    cfg = (att.num_attention_heads, att.map_size, att.lambda_init, att.LayerNorm.eps, max_len or 0, p, seed, off)
+    out, saved = _lib.nodes().diff_self_forward(qkv, att.LayerNorm.weight, att.lambdas(), mask, cu, *cfg, keep)
     return out, qkv, saved, cfg
 
 
 def _bert_diff_backward(qkv, mask, positions, cu, cfg, att, saved, dout):
     """Gradient of the projection's output; those of lambda and of the per-head norm are accumulated into `.grad`."""
     H = qkv.shape[-1] // 3
-    dqkv = _rows_like(qkv) if cu is None else qkv.new_zeros(qkv.shape)
+    dqkv = torch.empty_like(qkv) if cu is None else torch.zeros_like(qkv)
     dl = [ensure_grad(t) if t.requires_grad else None for t in att.lambdas()]
     w = att.LayerNorm.weight
     dw = ensure_grad(w) if w.requires_grad else None
-    _diff_backward(qkv, None, None, mask, cu, cu, cfg, w, att.lambdas(), saved, _rows16(dout), dqkv, None, None, dl, dw, True)
+    _lib.nodes().diff_self_backward(qkv, w, att.lambdas(), mask, cu, *cfg, saved, dout, dqkv, dw, dl, True)
     if att.rotary is not None:
         dqk = dqkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
-        _rotary_launch(dqk, dqk, positions, 0, att.rotary, True)
+        _turn(dqk, dqk, positions, 0, att.rotary, True)
     return dqkv
 
 
