@@ -17,7 +17,7 @@
 // Measured (MI355X; a library bf16 product of 8192^3 reaches 1195 TFLOP/s, a large copy 5.0 TB/s).  Forward, 12 d flops: 8192 keys d = 64
 // 1015 TFLOP/s from 16 heads on, d = 32 880; 2048 keys 900 and 700 with 64 heads.  Backward, 28 d flops, 2048 keys and 64 heads: 655 (d = 32),
 // 625 (d = 64).  The vector unit bounds it (two exponentials and about seven more instructions per query, key and map pair: 47 % of the
-// cycles at d = 64, where matrix instructions take 35 %: on one SIMD the two add up).  One query, 16381 keys, 4 x 12 heads: 36 us (5.5 TB/s) and
+// cycles at d = 64, where matrix instructions take 35 %: on one SIMD the two add up).  One query, 16381 keys, 4 x 12 heads: 38 us (5.3 TB/s) and
 // 5 for the join.  32 x 96, 12 heads, d = 32: 11 us forward, 16 with what the backward pass wants kept, 9 + 23 backward: latency.
 // Dropout: two generator calls per lane and 32 keys, in all three loops (32 x 512, 12 heads, d = 32: forward 63 -> 93 us, backward 201 -> 253).
 #include "common.cuh"
@@ -568,7 +568,7 @@ __device__ __forceinline__ float lambda_of_group(const DiffArgs& p, const int h,
 }
 
 // Joins the splits of a row (example, head, query): W / 8 lanes of 8 columns.  Few splits: every such group of lanes has a row of its own;
-// many (GS > 1): GS groups share the splits of a row.  HBM bound: 102 MB in 24 us (8191 rows x 6 heads, d = 64, 2 splits).
+// many (GS > 1): GS groups share the splits of a row.  HBM bound: 102 MB in 19 us (8191 rows x 6 heads, d = 64, 2 splits).
 template <int D, int GS>
 __global__ __launch_bounds__(256) void diff_join_kernel(const DiffArgs p, const int nsplit) {
     constexpr int W = 2 * D, LN = W / 8;
