@@ -134,6 +134,21 @@ __device__ __forceinline__ void store_block32(bf16_t* row, const f32x16& v, cons
     }
 }
 
+// A kernel's arguments arrive through the scalar cache, cold, and the compiler asks for them where it needs them: five waits for memory one
+// after the other before the first tile is under way.  One word of each of the N lines at once: the later loads hit.  (BYTES: of the
+// arguments, which fill the lines up to there; the launch's own hidden ones follow.)
+template <int BYTES>
+__device__ __forceinline__ void warm_args() {
+    typedef const __attribute__((address_space(4))) uint32_t* words;
+    const words a = (words)__builtin_amdgcn_kernarg_segment_ptr();
+    constexpr int N = (BYTES + 63) / 64;
+    uint32_t x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = a[16 * i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" ::"s"(x[i]));
+}
+
 // Workgroups go to the 8 XCDs in turn.  `chunk` consecutive units of work (they share K and V, or Q and dO) stay on one XCD and its L2;
 // successive chunks go to successive XCDs, so that sequences of different lengths spread over all of them.  The grid is padded to whole
 // rounds of 8 chunks: an answer of `total` or more has nothing to do.
@@ -416,6 +431,7 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const Di
     __shared__ __attribute__((aligned(16))) bf16_t Ks[2 * KT * W];
     __shared__ __attribute__((aligned(16))) bf16_t Vs[2 * KT * W];
     __shared__ __attribute__((aligned(16))) float mb[2 * KT];
+    warm_args<sizeof(DiffArgs) + 16>();
     const int bid = chunk_map((int)blockIdx.x, chunk);
     if (bid >= total) return;
     const int unit = SPLIT ? bid / nsplit : bid, sp = SPLIT ? bid - unit * nsplit : 0;
@@ -453,6 +469,10 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const Di
         f.l[j] = 0.f;
 #pragma unroll
         for (int t = 0; t < NV; ++t) f.o[j][t] = zero16();
+    }
+    if (!SPLIT && p.w != nullptr) {                            // (the epilogue's weights: into the cache)
+        const int touch = reinterpret_cast<const int*>(p.w)[lane & (D - 1)];
+        asm volatile("" ::"v"(touch));
     }
     float e1, e2;
     lambda_of<D>(p, h, lane, e1, e2);
@@ -572,6 +592,7 @@ __device__ __forceinline__ float lambda_of_group(const DiffArgs& p, const int h,
 template <int D, int GS>
 __global__ __launch_bounds__(256) void diff_join_kernel(const DiffArgs p, const int nsplit) {
     constexpr int W = 2 * D, LN = W / 8;
+    warm_args<sizeof(DiffArgs) + 4>();
     const int lane = threadIdx.x & 63, li = lane % LN, c = li * 8, gi = (lane / LN) % GS;
     const int64_t rows = (int64_t)p.B * p.heads * p.Lq;
     const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / (LN * GS);
@@ -660,6 +681,7 @@ __global__ __launch_bounds__(256) void diff_bwd_rows_kernel(const DiffArgs p, co
     constexpr int LN = W / 8, RP = 256 / LN;
     __shared__ float sw[RP][W];
     __shared__ float sl[RP];
+    warm_args<sizeof(DiffArgs) + 4>();
     const int h = (int)blockIdx.y;
     const int c = ((int)threadIdx.x % LN) * 8, ri = (int)threadIdx.x / LN;
     const float lam = lambda_of_group<W / 2>(p, h, (int)threadIdx.x % LN), so = 1.f - p.lambda_init;
@@ -1128,6 +1150,7 @@ struct BwdGrid { int nb, total, chunk, blocks; };              // blocks of rows
 template <int D, bool DROP>
 __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(const DiffArgs p, const ParamGrads g, const BwdGrid gq) {
     __shared__ __attribute__((aligned(16))) char smem[bwd_lds<D>()];
+    warm_args<sizeof(DiffArgs) + sizeof(ParamGrads) + sizeof(BwdGrid)>();
     if ((int)blockIdx.x >= gq.blocks) return bwd_params_block<D>(p, g, (int)blockIdx.x - gq.blocks, reinterpret_cast<float*>(smem));
     const int bid = chunk_map((int)blockIdx.x, gq.chunk);
     if (bid < gq.total) bwd_dq_block<D, DROP>(p, gq.nb, bid, smem);
@@ -1135,6 +1158,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(const DiffArgs p, c
 template <int D, bool DROP>
 __global__ __launch_bounds__(256, 1) void diff_bwd_dkv_kernel(const DiffArgs p, const BwdGrid gk) {
     __shared__ __attribute__((aligned(16))) char smem[bwd_lds<D>()];
+    warm_args<sizeof(DiffArgs) + sizeof(BwdGrid)>();
     const int bid = chunk_map((int)blockIdx.x, gk.chunk);
     if (bid < gk.total) bwd_dkv_block<D, DROP>(p, gk.nb, bid, smem);
 }
@@ -1142,6 +1166,7 @@ __global__ __launch_bounds__(256, 1) void diff_bwd_dkv_kernel(const DiffArgs p, 
 template <int D, bool DROP>
 __global__ __launch_bounds__(256, 2) void diff_bwd_kernel(const DiffArgs p, const ParamGrads g, const BwdGrid gk, const BwdGrid gq) {
     __shared__ __attribute__((aligned(16))) char smem[bwd_lds<D>()];
+    warm_args<sizeof(DiffArgs) + sizeof(ParamGrads) + 2 * sizeof(BwdGrid)>();
     int id = (int)blockIdx.x;
     if (id < gk.blocks) {
         const int bid = chunk_map(id, gk.chunk);
