@@ -35,6 +35,11 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int KT = 64;                   // rows of a staged tile
 constexpr int NSTAT = 4;                 // saved per (row, head): max and log2(sum) of both maps, in log2 units
 
+// Division by a number that the host knows, for 0 <= n < 2^31: (n + high half of n mul) >> shift.  (The compiler's own takes 25
+// instructions of code that every launch fetches cold.)
+struct Div { uint32_t d, mul, shift; };
+__device__ __forceinline__ int over(const int n, const Div v) { return (int)(((uint32_t)n + __umulhi((uint32_t)n, v.mul)) >> v.shift); }
+
 struct DiffArgs {
     const bf16_t *q, *k, *v;
     int64_t lq, lk, lv, bq, bk, bv;      // strides in elements: row, batch
@@ -49,6 +54,7 @@ struct DiffArgs {
     float eps;
     int B, heads;
     int Lq, Lk;                          // rows per example (packed: the longest)
+    Div by_heads, by_Lq;
     float sc;                            // log2(e) / sqrt(d)
     DropoutCfg drop;
     bf16_t* out;                         // forward: rows [.., heads * W]
@@ -152,9 +158,9 @@ __device__ __forceinline__ void warm_args() {
 // Workgroups go to the 8 XCDs in turn.  `chunk` consecutive units of work (they share K and V, or Q and dO) stay on one XCD and its L2;
 // successive chunks go to successive XCDs, so that sequences of different lengths spread over all of them.  The grid is padded to whole
 // rounds of 8 chunks: an answer of `total` or more has nothing to do.
-__device__ __forceinline__ int chunk_map(const int bid, const int chunk) {
-    const int loc = bid >> 3, c = loc / chunk;
-    return (c * 8 + (bid & 7)) * chunk + loc - c * chunk;
+__device__ __forceinline__ int chunk_map(const int bid, const Div chunk) {
+    const int loc = bid >> 3, c = over(loc, chunk), n = (int)chunk.d;
+    return (c * 8 + (bid & 7)) * n + loc - c * n;
 }
 
 // ---- examples: rows [q0, q0 + nq) of q / out and [k0, k0 + nk) of k / v
@@ -424,19 +430,21 @@ __device__ __forceinline__ void fwd_weights(FwdState<D>& f, f32x16 (&s)[2], bf16
     }
 }
 
+struct FwdGrid { Div nqb, ns, chunk; int total; };             // query blocks per (example, head), splits, units per chunk; units
+
 // one workgroup: `nw` waves of 32 queries each, key tiles [t0, t1) of its split.  SPLIT: writes partial sums for diff_join_kernel.
 template <int D, bool DROP, bool SPLIT>
-__global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const DiffArgs p, const int nqb, const int nsplit, const int total, const int chunk) {
+__global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const DiffArgs p, const FwdGrid g) {
     constexpr int W = 2 * D, NS = D / 16, NV = W / 32;
     __shared__ __attribute__((aligned(16))) bf16_t Ks[2 * KT * W];
     __shared__ __attribute__((aligned(16))) bf16_t Vs[2 * KT * W];
     __shared__ __attribute__((aligned(16))) float mb[2 * KT];
-    warm_args<sizeof(DiffArgs) + 16>();
-    const int bid = chunk_map((int)blockIdx.x, chunk);
-    if (bid >= total) return;
-    const int unit = SPLIT ? bid / nsplit : bid, sp = SPLIT ? bid - unit * nsplit : 0;
-    const int bh = unit / nqb, qb = unit - bh * nqb;
-    const int b = bh / p.heads, h = bh - b * p.heads;
+    warm_args<sizeof(DiffArgs) + sizeof(FwdGrid)>();
+    const int bid = chunk_map((int)blockIdx.x, g.chunk);
+    if (bid >= g.total) return;
+    const int nsplit = (int)g.ns.d, unit = SPLIT ? over(bid, g.ns) : bid, sp = SPLIT ? bid - unit * nsplit : 0;
+    const int bh = over(unit, g.nqb), qb = unit - bh * (int)g.nqb.d;
+    const int b = over(bh, p.by_heads), h = bh - b * p.heads;
     const Span sq = span_of(p.cu_q, p.tot_q, b, p.Lq), sk = span_of(p.cu_k, p.tot_k, b, p.Lk);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), half = lane >> 5;
     const int nw = (int)blockDim.x >> 6, tid = (int)threadIdx.x;
@@ -597,8 +605,7 @@ __global__ __launch_bounds__(256) void diff_join_kernel(const DiffArgs p, const 
     const int64_t rows = (int64_t)p.B * p.heads * p.Lq;
     const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / (LN * GS);
     const int64_t rc = r < rows ? r : rows - 1;                // (no lane leaves: the exchanges below are wave operations)
-    const int64_t bh = rc / p.Lq;
-    const int q = (int)(rc - bh * p.Lq), b = (int)(bh / p.heads), h = (int)(bh - (int64_t)b * p.heads);
+    const int bh = over((int)rc, p.by_Lq), q = (int)rc - bh * p.Lq, b = over(bh, p.by_heads), h = bh - b * p.heads;
     const Span sq = span_of(p.cu_q, p.tot_q, b, p.Lq);
     const bool live = r < rows && q < sq.n;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[2][8];
@@ -692,7 +699,7 @@ __global__ __launch_bounds__(256) void diff_bwd_rows_kernel(const DiffArgs p, co
     const int64_t r0 = (int64_t)blockIdx.x * rows_per;
     for (int i = ri; i < rows_per; i += RP) {
         const int64_t rr = r0 + i;
-        const int b = (int)(rr / p.Lq), q = (int)(rr - (int64_t)b * p.Lq);
+        const int b = over((int)rr, p.by_Lq), q = (int)rr - b * p.Lq;
         bool ok = rr < total;
         Span sq{0, 0};
         if (ok) { sq = span_of(p.cu_q, p.tot_q, b, p.Lq); ok = q < sq.n; }
@@ -811,12 +818,12 @@ __device__ __forceinline__ void bwd_params_block(const DiffArgs& p, const ParamG
 // backward, queries: dQ_j = sum_k dS_j K_j,  dS_1 = P_1 (G - D_1) / sqrt(d),  dS_2 = -lambda P_2 (G - D_2) / sqrt(d),  G = dropout(dO V^T)
 // ------------------------------------------------------------------------------------------------
 template <int D, bool DROP>
-__device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, const int bid, char* smem) {
+__device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const Div nqb, const int bid, char* smem) {
     constexpr int W = 2 * D, NS = D / 16, ND = D / 32;
     bf16_t *Ks = reinterpret_cast<bf16_t*>(smem), *Vs = Ks + 2 * KT * W;
     float* mb = reinterpret_cast<float*>(Vs + 2 * KT * W);
-    const int bh = bid / nqb, qb = bid - bh * nqb;
-    const int b = bh / p.heads, h = bh - b * p.heads;
+    const int bh = over(bid, nqb), qb = bid - bh * (int)nqb.d;
+    const int b = over(bh, p.by_heads), h = bh - b * p.heads;
     const Span sq = span_of(p.cu_q, p.tot_q, b, p.Lq), sk = span_of(p.cu_k, p.tot_k, b, p.Lk);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), half = lane >> 5;
     const int nw = (int)blockDim.x >> 6;
@@ -952,12 +959,12 @@ __device__ __forceinline__ void bwd_dq_block(const DiffArgs& p, const int nqb, c
 enum { ST_M = 0, ST_LL = 2, ST_LSE = 4, ST_D = 6, ST_N = 8 };            // (ST_D without dropout: -D_1 and D_2 - D_1)
 
 template <int D, bool DROP>
-__device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, const int bid, char* smem) {
+__device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const Div nkb, const int bid, char* smem) {
     constexpr int W = 2 * D, NS = D / 16, ND = D / 32, NV = W / 32;
     bf16_t *Qs = reinterpret_cast<bf16_t*>(smem), *Os = Qs + 2 * KT * W;
     float(*st)[ST_N][KT] = reinterpret_cast<float(*)[ST_N][KT]>(Os + 2 * KT * W);
-    const int bh = bid / nkb, kb = bid - bh * nkb;
-    const int b = bh / p.heads, h = bh - b * p.heads;
+    const int bh = over(bid, nkb), kb = bid - bh * (int)nkb.d;
+    const int b = over(bh, p.by_heads), h = bh - b * p.heads;
     const Span sq = span_of(p.cu_q, p.tot_q, b, p.Lq), sk = span_of(p.cu_k, p.tot_k, b, p.Lk);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), half = lane >> 5;
     const int nw = (int)blockDim.x >> 6;
@@ -1144,7 +1151,7 @@ __device__ __forceinline__ void bwd_dkv_block(const DiffArgs& p, const int nkb, 
 
 template <int D>
 constexpr int bwd_lds() { return 4 * KT * 2 * D * 2 + 2 * ST_N * KT * 4; }     // the larger of the two: dK / dV
-struct BwdGrid { int nb, total, chunk, blocks; };              // blocks of rows per (example, head); units; units per chunk; workgroups
+struct BwdGrid { Div nb, chunk; int total, blocks; };          // blocks of rows per (example, head); units per chunk; units; workgroups
 
 // dQ; the sums of the parameters' gradients ride along behind its last workgroups
 template <int D, bool DROP>
@@ -1212,6 +1219,15 @@ int check(const UniterDiffAttention* a) {
 bool has_queries(const UniterDiffAttention* a) { return a->B > 0 && a->Lq > 0 && (a->cu_seqlens_q == nullptr || a->total_q > 0); }
 bool has_keys(const UniterDiffAttention* a) { return a->B > 0 && a->Lk > 0 && (a->cu_seqlens_k == nullptr || a->total_k > 0); }
 
+Div div_of(int64_t d) {
+    Div v;
+    v.d = (uint32_t)d;
+    v.shift = 0;
+    while (((int64_t)1 << v.shift) < d) ++v.shift;
+    v.mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << v.shift) - (uint64_t)d)) / (uint64_t)d + 1);
+    return v;
+}
+
 DiffArgs args_of(const UniterDiffAttention* a) {
     DiffArgs p{};
     p.q = (const bf16_t*)a->q; p.k = (const bf16_t*)a->k; p.v = (const bf16_t*)a->v;
@@ -1225,6 +1241,7 @@ DiffArgs args_of(const UniterDiffAttention* a) {
     p.lambda_init = a->lambda_init;
     p.w = (const bf16_t*)a->norm_weight; p.eps = a->norm_eps;
     p.B = (int)a->B; p.heads = (int)a->heads; p.Lq = (int)a->Lq; p.Lk = (int)a->Lk;
+    p.by_heads = div_of(p.heads); p.by_Lq = div_of(p.Lq > 0 ? p.Lq : 1);
     p.sc = LOG2E / sqrtf((float)a->head_dim);
     p.drop = make_dropout(a->p_drop, a->seed, a->offset);
     return p;
@@ -1302,18 +1319,19 @@ int launch_fwd(const DiffArgs& p, int ns, hipStream_t st) {
     const int nw = waves_for(p.Lq), nqb = (p.Lq + 32 * nw - 1) / (32 * nw);
     const Grid gr = grid_of((int64_t)p.B * p.heads * nqb * ns, nqb * ns);
     const dim3 grid(gr.blocks), block(64 * nw);
+    const FwdGrid g{div_of(nqb), div_of(ns), div_of(gr.chunk), gr.total};
     const bool drop = p.drop.p > 0.f;
     if (ns > 1) {
-        if (drop) hipLaunchKernelGGL((diff_fwd_kernel<D, true, true>), grid, block, 0, st, p, nqb, ns, gr.total, gr.chunk);
-        else hipLaunchKernelGGL((diff_fwd_kernel<D, false, true>), grid, block, 0, st, p, nqb, ns, gr.total, gr.chunk);
+        if (drop) hipLaunchKernelGGL((diff_fwd_kernel<D, true, true>), grid, block, 0, st, p, g);
+        else hipLaunchKernelGGL((diff_fwd_kernel<D, false, true>), grid, block, 0, st, p, g);
         UH_LAUNCH_CHECK();
         const int64_t rows = (int64_t)p.B * p.heads * p.Lq;
         constexpr int NG = 64 / (2 * D / 8);                   // groups of lanes in a wave
         if (ns <= NG) hipLaunchKernelGGL((diff_join_kernel<D, 1>), dim3((unsigned)((rows + 4 * NG - 1) / (4 * NG))), dim3(256), 0, st, p, ns);
         else hipLaunchKernelGGL((diff_join_kernel<D, NG>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, ns);
     } else {
-        if (drop) hipLaunchKernelGGL((diff_fwd_kernel<D, true, false>), grid, block, 0, st, p, nqb, ns, gr.total, gr.chunk);
-        else hipLaunchKernelGGL((diff_fwd_kernel<D, false, false>), grid, block, 0, st, p, nqb, ns, gr.total, gr.chunk);
+        if (drop) hipLaunchKernelGGL((diff_fwd_kernel<D, true, false>), grid, block, 0, st, p, g);
+        else hipLaunchKernelGGL((diff_fwd_kernel<D, false, false>), grid, block, 0, st, p, g);
     }
     UH_LAUNCH_CHECK();
     return 0;
@@ -1330,7 +1348,7 @@ int launch_bwd(const DiffArgs& p, const BwdSpace& s, const ParamGrads& g, hipStr
     auto plan = [&](int L, int nw) {
         const int nb = (L + 32 * nw - 1) / (32 * nw);
         const Grid gr = grid_of((int64_t)p.B * p.heads * nb, nb);
-        return BwdGrid{nb, gr.total, gr.chunk, (int)gr.blocks};
+        return BwdGrid{div_of(nb > 0 ? nb : 1), div_of(gr.chunk), gr.total, (int)gr.blocks};
     };
     const bool drop = p.drop.p > 0.f;
     // d = 32: one launch for dQ and dK / dV, which fill the chip better together than one after the other (d = 32, 28 d flops counted:
