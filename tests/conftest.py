@@ -20,11 +20,11 @@ def golden():
 
 @pytest.fixture(scope="session", autouse=True)
 def _built_library():
-    """The suites need libuniter_hip.so (symbol / argument-error tests on CPU, everything on the GPU).  It is built
+    """The suites need libuniter_hip.so and uniter_nodes.so (symbol / argument-error tests on CPU, everything on the GPU).  It is built
     in-tree by __graft_entry__.build(); if a fresh checkout runs the tests first, build it here (hipcc cross-compiles
     gfx950 without a GPU, ~1 min).  A missing hipcc just leaves the library absent — the tests that need it say so."""
     from uniter_amd import _lib
-    if not os.path.exists(_lib.LIB_PATH):
+    if not (os.path.exists(_lib.LIB_PATH) and os.path.exists(_lib.NODES_PATH)):
         try:
             sys.path.insert(0, os.path.join(ROOT, "uniter_amd", "csrc"))
             import build as libbuild

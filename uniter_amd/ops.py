@@ -1126,9 +1126,9 @@ _TILE_192, _TILE_256 = 59, 58
 
 
 def _layer_wgrads(dys, xs_, dws, dbs, T, Ns, Ks, training):
-    """The four weight gradients of a layer in one launch, on the widest deep-pipelined tile that fits: 3072 tokens at 768 / 3072 62 us on
-    192 x 192 (256 x 256: 77, 128 x 128: 112), 2880 tokens at 1024 / 4096 84 us on 256 x 256 (128 x 128: 184), 320 tokens 15.5 against 14.4 of
-    the best small tile.  Rows that are not a multiple of 64 take the tuned tile (wgrad_group)."""
+    """The four weight gradients of a layer in one launch, on the widest deep-pipelined tile that fits: the base encoder's layer at 32 x 96
+    tokens 62 us on 192 x 192 (256 x 256: 77, 128 x 128: 112), the large one's at 2880 tokens 84 us on 256 x 256 (128 x 128: 184), base at 320
+    tokens 15.5 against 14.4 of the best small tile.  Rows that are not a multiple of 64 take the tuned tile (wgrad_group)."""
     tile = next((c for c, e in ((_TILE_192, 192), (_TILE_256, 256)) if T % 64 == 0 and all(n % e == 0 for n in Ns + Ks)), None)
     if tile is None:
         return wgrad_group(dys, [0] * 4, xs_, [0] * 4, dws, dbs, T, Ns, Ks, training)
