@@ -206,11 +206,13 @@ def test_refusals():
 
 @pytest.mark.gpu
 def test_an_entry_that_refuses_raises_the_packages_error():
-    """Past the Python checks: the status of the C entry, with its message."""
-    x, turns = torch.zeros(1, 2, 3, 64, dtype=BF16, device="cuda"), torch.zeros(32, dtype=torch.float64, device="cuda")
+    """Past the checks of the call: the status of the C entry, with its message."""
+    rot = RotaryPositions(64)
+    rot.rotary_dim = 7
+    x = torch.zeros(1, 2, 3, 64, dtype=BF16, device="cuda")
     for leaf in (x, x.clone().requires_grad_(True)):
         with pytest.raises(_lib.UniterHipError, match="rot_dim"):
-            _lib.nodes().rotary(leaf, None, None, 0, turns, 7, 1.0, False, False)
+            ops.rotary(leaf, None, rot)
 
 
 @pytest.mark.gpu

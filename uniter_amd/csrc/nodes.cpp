@@ -5,7 +5,7 @@
 // it is C++ on both sides and the backward pass needs no interpreter.  The kernels are reached through the C ABI all the same: the
 // package hands over the addresses of the entry points of the library that it has loaded (init), nothing is linked.
 //
-// Arguments arrive checked (uniter_amd/ops.py); workspaces come from torch's caching allocator.
+// The arguments' checks are here too, for the same reason (ops.py holds the documentation); workspaces come from torch's caching allocator.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <c10/core/DeviceGuard.h>
@@ -38,12 +38,26 @@ void ok(int rc, const char* name) {
     throw Error(std::string(name) + " failed with status " + std::to_string(rc) + ": " + (why ? why : ""));
 }
 
+template <class... T>
+[[noreturn]] void refuse(const T&... words) { throw Error(c10::str(words...)); }
+
+void check(const Tensor& t, at::ScalarType type, const char* what) {
+    if (!t.defined() || !t.is_cuda())
+        refuse(what, " must be a CUDA(HIP) tensor: the kernels exist for gfx950 only (no CPU / PyTorch fallback)");
+    if (t.scalar_type() != type) refuse(what, " must be ", type, ", got ", t.scalar_type(), type == at::kBFloat16 ? " (cast the model with .bfloat16())" : "");
+}
+void check_beside(const Tensor& first, const char* name, const Tensor& t, at::ScalarType type, const char* what) {
+    check(t, type, what);
+    if (t.get_device() != first.get_device()) refuse(what, " is on ", t.device(), ", ", name, " on ", first.device());
+}
+
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor get(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
 Tensor rows_like(const Tensor& t) { return at::empty_like(t, t.options(), at::MemoryFormat::Contiguous); }
 // contiguous rows that start on 16 bytes (row strides of whole 8s); a copy where they do not
 Tensor rows16(const Tensor& t) {
+    if (t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0) return t;
     bool fits = t.stride(-1) == 1 && (uintptr_t)t.data_ptr() % 16 == 0;
     for (int64_t i = 0; fits && i + 1 < t.dim(); ++i) fits = t.stride(i) % 8 == 0 || t.size(i) == 1;
     return fits ? t : t.clone(at::MemoryFormat::Contiguous);
@@ -117,13 +131,69 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
     }
 };
 
-Tensor rotary(const Tensor& x, const optional<Tensor>& out, const optional<Tensor>& positions, int64_t offset, const Tensor& turns, int64_t rot,
-              double multiplier, bool interleaved, bool inverse) {
-    const Rotary r{get(positions), turns, offset, rot, multiplier, interleaved};
-    if (!out.has_value() && !inverse && at::GradMode::is_enabled() && x.requires_grad()) return RotaryNode::apply(x, r);
-    Tensor y = out.has_value() ? *out : rows_like(x);
-    rotary_run(x, y, r, inverse);
+// Whether the address ranges of two views of one storage meet AND their rows can (equal strides and interleaved rows that stay apart — q and
+// k blocks of one projection — do not).
+bool overlap(const Tensor& a, const Tensor& b) {
+    if (a.storage().data() != b.storage().data()) return false;
+    auto end = [](const Tensor& t) {
+        int64_t n = 1;
+        for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+        return (char*)t.data_ptr() + 2 * n;
+    };
+    const char *a0 = (char*)a.data_ptr(), *b0 = (char*)b.data_ptr();
+    if (end(a) <= b0 || end(b) <= a0) return false;
+    const int64_t row = a.stride(-3), w = a.size(-2) * a.stride(-2);
+    if (a.strides() == b.strides() && row >= w) {              // same row pitch: rows of width w at offsets d apart modulo the pitch
+        const int64_t d = (a0 < b0 ? b0 - a0 : a0 - b0) / 2 % row;
+        return d < w || row - d < w;
+    }
+    return true;
+}
+
+Tensor rotary(Tensor x, const optional<Tensor>& positions, int64_t offset, const optional<Tensor>& out, const Tensor& turns, int64_t head_dim,
+              int64_t rot, double multiplier, bool interleaved) {
+    check(x, at::kBFloat16, "rotary input");
+    const int64_t d = x.dim();
+    if ((d != 3 && d != 4) || x.size(-1) != head_dim)
+        refuse("rotary input must be [B, L, heads, ", head_dim, "] or [T, heads, ", head_dim, "], got ", x.sizes());
+    Tensor pos = get(positions);
+    if (!pos.defined()) {
+        if (d == 3) refuse("rotary: rows stored back to back need their positions");
+    } else {
+        if (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt) refuse("rotary: positions must be an int64 or int32 tensor (or None)");
+        if (!pos.is_cuda() || pos.get_device() != x.get_device()) refuse("positions is on ", pos.device(), ", x on ", x.device());
+        if (d == 4 && pos.dim() == 2 && pos.size(0) == 1 && x.size(0) != 1) pos = pos[0];
+        const auto rows = x.sizes().slice(0, d - 2), last = x.sizes().slice(d - 3, 1);
+        if (pos.sizes() != rows && pos.sizes() != last) refuse("rotary: positions must be ", rows, " or ", last, ", got ", pos.sizes());
+        if (pos.scalar_type() == at::kInt) pos = pos.to(at::kLong);
+        if (pos.stride(-1) != 1) pos = pos.contiguous();
+    }
+    if (x.stride(-1) != 1) {
+        if (out.has_value() && out->is_same(x)) refuse("rotary: in place needs contiguous heads");
+        x = x.contiguous();
+    }
+    const Rotary r{pos, turns, offset, rot, multiplier, interleaved};
+    if (!out.has_value()) {
+        if (at::GradMode::is_enabled() && x.requires_grad()) return RotaryNode::apply(x, r);
+        Tensor y = rows_like(x);
+        rotary_run(x, y, r, false);
+        return y;
+    }
+    const Tensor& y = *out;
+    if (at::GradMode::is_enabled() && (x.requires_grad() || y.requires_grad()))
+        refuse("rotary: out= writes outside autograd; call it without gradients or let it return a new tensor");
+    check_beside(x, "x", y, at::kBFloat16, "rotary output");
+    if (y.sizes() != x.sizes() || y.stride(-1) != 1) refuse("rotary: out must have x's shape and contiguous heads");
+    for (int64_t i = 0; i < d; ++i)
+        if (y.stride(i) == 0 && y.size(i) > 1) refuse("rotary: out must not be a broadcast view");
+    if (y.numel() != 0 && !(y.data_ptr() == x.data_ptr() && y.strides() == x.strides()) && overlap(y, x)) refuse("rotary: out overlaps x without being x");
+    rotary_run(x, y, r, false);
     return y;
+}
+
+// the kernel by itself, in place, on checked arguments
+void rotary_turn(const Tensor& x, const optional<Tensor>& positions, const Tensor& turns, int64_t rot, double multiplier, bool interleaved, bool inverse) {
+    rotary_run(x, x, Rotary{get(positions), turns, 0, rot, multiplier, interleaved}, inverse);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -255,6 +325,72 @@ Fixed fixed_of(const optional<Tensor>& mask, const optional<Tensor>& cu_q, const
     return Fixed{get(mask), get(cu_q), get(cu_k), heads, dim, max_q, max_k, seed, offset, lambda_init, eps, p_drop, keep};
 }
 
+// ops.differential_attention; k and v nullopt: q is a fused projection
+Tensor diff_attention(Tensor q, const optional<Tensor>& k_, const optional<Tensor>& v_, int64_t heads, const std::vector<Tensor>& lams, double lambda_init,
+                      const optional<Tensor>& weight_, const optional<Tensor>& mask_, const optional<Tensor>& cu_q_, const optional<Tensor>& cu_k_,
+                      optional<int64_t> max_q, optional<int64_t> max_k, double eps, double p_drop, int64_t seed, int64_t offset) {
+    const bool fused = !k_.has_value(), packed = cu_q_.has_value() || cu_k_.has_value();
+    const char* name = fused ? "qkv" : "q";
+    check(q, at::kBFloat16, name);
+    Tensor k = get(k_), v = get(v_), weight = get(weight_), mask = get(mask_), cu_q = get(cu_q_), cu_k = get(cu_k_), l[4];
+    if (!fused) {
+        check_beside(q, name, k, at::kBFloat16, "k");
+        check_beside(q, name, v, at::kBFloat16, "v");
+    }
+    const int64_t nd = packed ? 2 : 3;
+    if (q.dim() != nd || (!fused && (k.dim() != nd || v.dim() != nd)))
+        refuse(fused ? "qkv" : "q, k and v", " must be ", packed ? "[rows, columns] when cu_seqlens is given" : "[B, L, columns]", ", got ", q.sizes());
+    const int64_t cols = q.size(-1), H = fused ? cols / 3 : cols, dim = heads > 0 ? H / (2 * heads) : 0;
+    if ((fused && cols % 3 != 0) || (dim != 32 && dim != 64) || H != heads * 2 * dim)
+        refuse("differential attention: a head is 64 or 128 columns (two maps of 32 or 64), got ", H, " columns for ", heads, " heads");
+    if (!fused && (k.sizes() != v.sizes() || k.size(-1) != H || (!packed && k.size(0) != q.size(0))))
+        refuse("differential attention: q ", q.sizes(), ", k ", k.sizes(), " and v ", v.sizes(), " do not fit");
+    if (lams.size() != 4) refuse("lambdas are four tensors: q1, k1, q2, k2");
+    const bool per_head = lams[0].sizes() == at::IntArrayRef({heads, dim});
+    if (!per_head && lams[0].sizes() != at::IntArrayRef({dim})) refuse("lambda vectors must be [", dim, "] or [", heads, ", ", dim, "], got ", lams[0].sizes());
+    for (int i = 0; i < 4; ++i) {
+        check_beside(q, name, lams[i], at::kBFloat16, "lambda vector");
+        if (lams[i].sizes() != lams[0].sizes()) refuse("lambda vectors must have one shape, got ", lams[0].sizes(), " and ", lams[i].sizes());
+        l[i] = lams[i].contiguous();
+    }
+    if (weight.defined()) {
+        check_beside(q, name, weight, at::kBFloat16, "norm_weight");
+        if (weight.sizes() != at::IntArrayRef({2 * dim})) refuse("norm_weight must be [", 2 * dim, "], got ", weight.sizes());
+        weight = rows16(weight);
+        if (!(eps > 0.0)) refuse("eps must be positive, got ", eps);
+    }
+    if (!(p_drop >= 0.0 && p_drop < 1.0)) refuse("dropout probability must be in [0, 1), got ", p_drop);
+    if (packed) {
+        if (mask.defined()) refuse("packed rows take no mask_bias: only real tokens are there");
+        if (!cu_k.defined()) cu_k = cu_q;
+        if (!max_k.has_value()) max_k = max_q;
+        if (!cu_q.defined() || !max_q.has_value() || *max_q < 0 || *max_k < 0)
+            refuse("packed rows need cu_seqlens and max_len (and those of the keys where they differ)");
+        for (Tensor* c : {&cu_q, &cu_k}) {
+            check_beside(q, name, *c, at::kInt, "cu_seqlens");
+            if (c->dim() != 1 || c->numel() != cu_q.numel() || c->numel() < 1) refuse("cu_seqlens must be int32 [examples + 1]");
+            *c = c->contiguous();
+        }
+    } else if (mask.defined()) {
+        check_beside(q, name, mask, at::kFloat, "mask_bias");
+        if (mask.dim() == 4 && mask.size(1) == 1 && mask.size(2) == 1) mask = mask.select(1, 0).select(1, 0);      // UniterModel's extended mask [B, 1, 1, L]
+        const int64_t Lk = fused ? q.size(1) : k.size(1);
+        if (mask.sizes() != at::IntArrayRef({q.size(0), Lk})) refuse("mask_bias must be [", q.size(0), ", ", Lk, "] (or [B, 1, 1, Lk]), got ", mask.sizes());
+        if (mask.stride(1) != 1) mask = mask.contiguous();
+    }
+    q = rows16(q);
+    if (!fused) {
+        k = rows16(k);
+        v = rows16(v);
+    }
+    auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    const bool keep = at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v) || wants(weight) || wants(l[0]) || wants(l[1]) || wants(l[2]) || wants(l[3]));
+    const Fixed f{mask, cu_q, cu_k, heads, dim, max_q.value_or(0), max_k.value_or(0), seed, offset, lambda_init, eps, p_drop, keep};
+    if (!keep) return diff_forward(Operands{q, k, v, weight, {l[0], l[1], l[2], l[3]}}, f).first;
+    auto given = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; };
+    return DiffNode::apply(f, q, given(k), given(v), given(weight), l[0], l[1], l[2], l[3]);
+}
+
 void init(py::dict addresses, py::object error) {
     auto at = [&](const char* name) { return addresses[name].cast<uintptr_t>(); };
     lib.rotary = (decltype(lib.rotary))at("uniter_rotary");
@@ -280,17 +416,8 @@ PYBIND11_MODULE(uniter_nodes, m) {
     // (without the interpreter lock, as torch's own operators: a launch may wait for room in its queue)
     using unlocked = py::call_guard<py::gil_scoped_release>;
     m.def("rotary", &rotary, unlocked());
-    m.def("diff_attention", [](const Tensor& q, const optional<Tensor>& k, const optional<Tensor>& v, const optional<Tensor>& weight, const Tensor& l0,
-                               const Tensor& l1, const Tensor& l2, const Tensor& l3, const optional<Tensor>& mask, const optional<Tensor>& cu_q,
-                               const optional<Tensor>& cu_k, int64_t heads, int64_t dim, double lambda_init, double eps, int64_t max_q, int64_t max_k,
-                               double p_drop, int64_t seed, int64_t offset) {
-        auto wants = [](const optional<Tensor>& t) { return t.has_value() && t->requires_grad(); };
-        const bool keep = at::GradMode::is_enabled() && (q.requires_grad() || wants(k) || wants(v) || wants(weight) || l0.requires_grad() ||
-                                                         l1.requires_grad() || l2.requires_grad() || l3.requires_grad());
-        const Fixed f = fixed_of(mask, cu_q, cu_k, heads, dim, lambda_init, eps, max_q, max_k, p_drop, seed, offset, keep);
-        if (keep) return DiffNode::apply(f, q, k, v, weight, l0, l1, l2, l3);
-        return diff_forward(Operands{q, get(k), get(v), get(weight), {l0, l1, l2, l3}}, f).first;
-    }, unlocked());
+    m.def("rotary_turn", &rotary_turn, unlocked());
+    m.def("diff_attention", &diff_attention, unlocked());
     // the two passes by themselves, on a fused projection, for nodes that hold more than the attention
     m.def("diff_self_forward", [](const Tensor& qkv, const optional<Tensor>& weight, const std::vector<Tensor>& l, const optional<Tensor>& mask,
                                   const optional<Tensor>& cu, int64_t heads, int64_t dim, double lambda_init, double eps, int64_t max_len, double p_drop,

@@ -856,25 +856,6 @@ def _check_same_device(first, name, others):
             raise _lib.UniterHipError("%s is on %s, %s on %s" % (what, t.device, name, first.device))
 
 
-def _rows16(t):
-    """`t` (rows of a multiple of 8 elements) with contiguous rows that start on 16 bytes; a copy when they do not."""
-    if t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return t
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0:
-        for s, n in zip(st[:-1], t.shape):
-            if s % 8 != 0 and n != 1:
-                break
-        else:
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _turn(x, out, positions, offset, rot, inverse=False):
-    """The kernel (csrc/nodes.cpp); out None: a new tensor, and a node where x wants a gradient."""
-    return _lib.nodes().rotary(x, out, positions, offset, rot.turns(x.device), rot.rotary_dim, rot.multiplier, rot.interleaved, inverse)
-
-
 def rotary(x, positions, rot, offset=0, out=None):
     """Turn the heads of x by their token positions (model/rotary.py::RotaryPositions `rot`).
 
@@ -883,139 +864,9 @@ def rotary(x, positions, rot, offset=0, out=None):
     0 .. L - 1 (of every row of the batch); `offset` is added to either.  Returns a new tensor; out=x turns x in place, out=another
     tensor of x's shape writes there (both outside autograd only).  The gradient is turned back by the same kernel."""
     _check_dev(x, "rotary input")
-    shape = x.shape
-    nd = len(shape)
-    if nd not in (3, 4) or shape[-1] != rot.head_dim:
-        raise _lib.UniterHipError("rotary input must be [B, L, heads, %d] or [T, heads, %d], got %s" % (rot.head_dim, rot.head_dim, tuple(shape)))
-    if positions is None:
-        if nd == 3:
-            raise _lib.UniterHipError("rotary: rows stored back to back need their positions")
-    else:
-        kind = positions.dtype if isinstance(positions, torch.Tensor) else None
-        if kind is not torch.int64 and kind is not torch.int32:
-            raise _lib.UniterHipError("rotary: positions must be an int64 or int32 tensor (or None)")
-        if positions.get_device() != x.get_device():
-            raise _lib.UniterHipError("positions is on %s, x on %s" % (positions.device, x.device))
-        at = positions.shape
-        if nd == 4 and len(at) == 2 and at[0] == 1 != shape[0]:
-            positions = positions[0]
-            at = at[1:]
-        if at != shape[:-2] and at != shape[-3:-2]:
-            raise _lib.UniterHipError("rotary: positions must be %s or %s, got %s" % (list(shape[:-2]), list(shape[-3:-2]), list(at)))
-        if kind is torch.int32:
-            positions = positions.to(torch.int64)
-        if positions.stride(-1) != 1:
-            positions = positions.contiguous()
-    if x.stride(-1) != 1:
-        if out is x:
-            raise _lib.UniterHipError("rotary: in place needs contiguous heads")
-        x = x.contiguous()
-    if out is not None:
-        if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
-            raise _lib.UniterHipError("rotary: out= writes outside autograd; call it without gradients or let it return a new tensor")
-        _check_dev(out, "rotary output")
-        _check_same_device(x, "x", ((out, "out"),))
-        if out.shape != x.shape or out.stride(-1) != 1:
-            raise _lib.UniterHipError("rotary: out must have x's shape and contiguous heads")
-        if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
-            raise _lib.UniterHipError("rotary: out must not be a broadcast view")
-        if out.numel() and (out.data_ptr() != x.data_ptr() or out.stride() != x.stride()) \
-                and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() and _overlap(out, x):
-            raise _lib.UniterHipError("rotary: out overlaps x without being x")
-    return _turn(x, out, positions, int(offset), rot)
-
-
-def _overlap(a, b):
-    """Whether the address ranges of two views of one storage meet AND their rows can (equal strides and interleaved rows that stay
-    apart — q and k blocks of one projection — do not)."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + 2 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-    (a0, a1), (b0, b1) = span(a), span(b)
-    if a1 <= b0 or b1 <= a0:
-        return False
-    row = a.stride(-3)
-    if a.stride() == b.stride() and a.dim() >= 3 and row >= a.shape[-2] * a.stride(-2):
-        # same row pitch: rows of width w at offsets d apart modulo the pitch
-        w, d = a.shape[-2] * a.stride(-2), (abs(a0 - b0) // 2) % row
-        return d < w or row - d < w
-    return True
-
-
-def _diff_check(q, k, v, heads, lams, weight, mask, cu_q, cu_k, max_q, max_k, eps, p_drop):
-    """What both calls ask of their arguments (k, v None: q is a fused projection); (dim, mask, cu_q, cu_k, max_q, max_k, lams, weight)."""
-    fused = k is None
-    H, odd = divmod(q.shape[-1], 3) if fused else (q.shape[-1], 0)
-    dim = H // (2 * heads) if heads > 0 else 0
-    if odd or dim not in (32, 64) or H != heads * 2 * dim:
-        raise _lib.UniterHipError("differential attention: a head is 64 or 128 columns (two maps of 32 or 64), got %d columns for %d heads" % (H, heads))
-    packed = cu_q is not None or cu_k is not None
-    nd = 2 if packed else 3
-    _check_dev(q, "qkv" if fused else "q")
-    dev = q.get_device()
-
-    def bf16_here(t, what):
-        if not isinstance(t, torch.Tensor) or t.dtype is not _BF16 or t.get_device() != dev:
-            _check_dev(t, what)
-            _check_same_device(q, "qkv" if fused else "q", ((t, what),))
-
-    if q.dim() != nd or not fused and (k.dim() != nd or v.dim() != nd):
-        raise _lib.UniterHipError("%s must be %s, got %s" % ("qkv" if fused else "q, k and v", "[rows, columns] when cu_seqlens is given" if packed else
-                                                             "[B, L, columns]", [tuple(t.shape) for t in (q, k, v) if t is not None]))
-    if not fused:
-        bf16_here(k, "k")
-        bf16_here(v, "v")
-    Bk = q if fused else k
-    if not fused and (k.shape != v.shape or k.shape[-1] != H or (not packed and k.shape[0] != q.shape[0])):
-        raise _lib.UniterHipError("differential attention: q %s, k %s and v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    if len(lams) != 4:
-        raise _lib.UniterHipError("lambdas are four tensors: q1, k1, q2, k2")
-    shape = lams[0].shape
-    if shape != (heads, dim) and shape != (dim,):
-        raise _lib.UniterHipError("lambda vectors must be [%d] or [%d, %d], got %s" % (dim, heads, dim, tuple(shape)))
-    for t in lams:
-        bf16_here(t, "lambda vector")
-        if t.shape != shape:
-            raise _lib.UniterHipError("lambda vectors must have one shape, got %s and %s" % (tuple(shape), tuple(t.shape)))
-    if weight is not None:
-        bf16_here(weight, "norm_weight")
-        if weight.shape != (2 * dim,):
-            raise _lib.UniterHipError("norm_weight must be [%d], got %s" % (2 * dim, tuple(weight.shape)))
-        weight = _rows16(weight)
-        if not eps > 0.0:
-            raise _lib.UniterHipError("eps must be positive, got %r" % (eps,))
-    if not 0.0 <= p_drop < 1.0:
-        raise _lib.UniterHipError("dropout probability must be in [0, 1), got %r" % (p_drop,))
-    if packed:
-        if mask is not None:
-            raise _lib.UniterHipError("packed rows take no mask_bias: only real tokens are there")
-        cu_k = cu_q if cu_k is None else cu_k
-        max_k = max_q if max_k is None else max_k
-        if cu_q is None or max_q is None or max_k is None or max_q < 0 or max_k < 0:
-            raise _lib.UniterHipError("packed rows need cu_seqlens and max_len (and those of the keys where they differ)")
-        for c in (cu_q, cu_k):
-            _check_dev(c, "cu_seqlens", torch.int32)
-            if c.dim() != 1 or c.numel() != cu_q.numel() or c.numel() < 1:
-                raise _lib.UniterHipError("cu_seqlens must be int32 [examples + 1]")
-        cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
-    elif mask is not None:
-        _check_dev(mask, "mask_bias", torch.float32)
-        if mask.dim() == 4 and mask.shape[1] == mask.shape[2] == 1:        # UniterModel's extended mask [B, 1, 1, L]
-            mask = mask[:, 0, 0]
-        if mask.shape != (q.shape[0], Bk.shape[1]):
-            raise _lib.UniterHipError("mask_bias must be [%d, %d] (or [B, 1, 1, Lk]), got %s" % (q.shape[0], Bk.shape[1], tuple(mask.shape)))
-        if mask.stride(1) != 1:
-            mask = mask.contiguous()
-    _check_same_device(q, "qkv" if fused else "q", ((mask, "mask_bias"), (cu_q, "cu_seqlens"), (cu_k, "cu_seqlens_k")))
-    return dim, mask, cu_q, cu_k, max_q, max_k, [t.contiguous() for t in lams], weight
-
-
-def _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop):
-    dim, mask, cu_q, cu_k, max_q, max_k, lams, weight = checked
-    q = _rows16(q)
-    if k is not None:
-        k, v = _rows16(k), _rows16(v)
-    seed, off = _next_offsets(1) if p_drop > 0.0 else (0, 0)
-    return _lib.nodes().diff_attention(q, k, v, weight, *lams, mask, cu_q, cu_k, heads, dim, lambda_init, eps, max_q or 0, max_k or 0, p_drop, seed, off)
+    if positions is not None and not isinstance(positions, torch.Tensor):
+        raise _lib.UniterHipError("rotary: positions must be an int64 or int32 tensor (or None)")
+    return _lib.nodes().rotary(x, positions, offset, out, rot.turns(x.device), rot.head_dim, rot.rotary_dim, rot.multiplier, rot.interleaved)
 
 
 def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=None, mask_bias=None, cu_seqlens=None, cu_seqlens_k=None,
@@ -1033,16 +884,18 @@ def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=Non
     backward pass."""
     if not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor):
         raise _lib.UniterHipError("differential attention needs k and v (differential_self_attention takes a fused projection)")
-    checked = _diff_check(q, k, v, heads, lambdas, norm_weight, mask_bias, cu_seqlens, cu_seqlens_k, max_len, max_len_k, eps, p_drop)
-    return _diff_apply(q, k, v, heads, checked, lambda_init, eps, p_drop)
+    seed, off = _next_offsets(1) if p_drop > 0.0 else (0, 0)
+    return _lib.nodes().diff_attention(q, k, v, heads, lambdas, lambda_init, norm_weight, mask_bias, cu_seqlens, cu_seqlens_k, max_len, max_len_k, eps,
+                                       p_drop, seed, off)
 
 
 def differential_self_attention(qkv, heads, lambdas, lambda_init, norm_weight=None, mask_bias=None, cu_seqlens=None, max_len=None,
                                 eps=1e-5, p_drop=0.0):
     """differential_attention on a fused projection qkv [B, L, 3 H] (or packed [T, 3 H]), H = heads * 2 d: the q | k | v layout that
     BertSelfAttention.fused_qkv produces.  Its gradient is one [.., 3 H] tensor too."""
-    checked = _diff_check(qkv, None, None, heads, lambdas, norm_weight, mask_bias, cu_seqlens, None, max_len, None, eps, p_drop)
-    return _diff_apply(qkv, None, None, heads, checked, lambda_init, eps, p_drop)
+    seed, off = _next_offsets(1) if p_drop > 0.0 else (0, 0)
+    return _lib.nodes().diff_attention(qkv, None, None, heads, lambdas, lambda_init, norm_weight, mask_bias, cu_seqlens, None, max_len, None, eps,
+                                       p_drop, seed, off)
 
 
 def key_mask(attention_mask, hidden_states):
@@ -1061,6 +914,11 @@ def packed_positions(cu_seqlens, total):
     return torch.arange(total, device=cu.device) - torch.repeat_interleave(cu[:-1], cu.diff(), output_size=total)
 
 
+def _rotary_turn(rot, x, positions, inverse):
+    """x (a view of a projection's q | k columns) turned in place."""
+    _lib.nodes().rotary_turn(x, positions, rot.turns(x.device), rot.rotary_dim, rot.multiplier, rot.interleaved, inverse)
+
+
 def _bert_diff_forward(xc, mask, positions, cu, max_len, att, p, keep):
     """Fused [3H, H] projection, q | k turned in place, differential attention: (out, qkv, saved, cfg)."""
     H = xc.shape[-1]
@@ -1069,7 +927,7 @@ def _bert_diff_forward(xc, mask, positions, cu, max_len, att, p, keep):
     C.uniter_gemm_bias_fwd(ptr(xc), ptr(wqkv), ptr(bqkv), ptr(qkv), xc.numel() // H, 3 * H, H, _lib.stream_ptr())
     if att.rotary is not None:
         qk = qkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
-        _turn(qk, qk, positions, 0, att.rotary)
+        _rotary_turn(att.rotary, qk, positions, False)
     seed, off = _next_offsets(1) if p > 0.0 else (0, 0)
     cfg = (att.num_attention_heads, att.map_size, att.lambda_init, att.LayerNorm.eps, max_len or 0, p, seed, off)
     out, saved = _lib.nodes().diff_self_forward(qkv, att.LayerNorm.weight, att.lambdas(), mask, cu, *cfg, keep)
@@ -1086,7 +944,7 @@ def _bert_diff_backward(qkv, mask, positions, cu, cfg, att, saved, dout):
     _lib.nodes().diff_self_backward(qkv, w, att.lambdas(), mask, cu, *cfg, saved, dout, dqkv, dw, dl, True)
     if att.rotary is not None:
         dqk = dqkv[..., :2 * H].unflatten(-1, (2 * H // att.map_size, att.map_size))
-        _turn(dqk, dqk, positions, 0, att.rotary, True)
+        _rotary_turn(att.rotary, dqk, positions, True)
     return dqkv
 
 
