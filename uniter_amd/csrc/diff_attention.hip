@@ -118,24 +118,28 @@ __device__ __forceinline__ bf16x8 pack_step(const f32x16& s, const int kk) {
 // the larger one, or a NaN (one instruction for two of them: v_maximum3; fmaxf would quieten its operands first)
 __device__ __forceinline__ float max2(const float a, const float b) { return __builtin_elementwise_maximum(a, b); }
 // the value of lane ^ 32
-__device__ __forceinline__ float other_half(const float x) { return __shfl_xor(x, 32, WAVE); }
+__device__ __forceinline__ float other_half(const float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);       // (lower half twice, upper half twice)
+    return __uint_as_float((threadIdx.x & 32) ? s[0] : s[1]);
+}
 // row (or column) of an accumulator register: 8 (r / 4) + 4 half + r % 4
 __device__ __forceinline__ constexpr int acc_row(const int r) { return 8 * (r >> 2) + (r & 3); }
 
-// A lane holds columns 8 g + 4 half + {0..3}, g = 0..3, of one 32-column block of its row.  The two halves swap a group of every pair,
-// so that a lane stores 16 bytes: half 0 the 8 columns of the even group, half 1 those of the odd one.
+// A lane holds columns 8 g + 4 half + {0..3}, g = 0..3, of one 32-column block of its row.  The two halves swap a group of every pair
+// (v_permlane32_swap: the upper half of one register with the lower half of another), so that a lane stores 16 bytes: half 0 the 8 columns of the
+// even group, half 1 those of the odd one.
 __device__ __forceinline__ void store_block32(bf16_t* row, const f32x16& v, const int half, const bool valid) {
 #pragma unroll
     for (int g = 0; g < 4; g += 2) {
-        uint32_t a[2], b[2];
+        u32x4 w;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            a[e] = pack_bf16x2(v[4 * g + 2 * e], v[4 * g + 2 * e + 1]);
-            b[e] = pack_bf16x2(v[4 * g + 4 + 2 * e], v[4 * g + 4 + 2 * e + 1]);
+            const auto s = __builtin_amdgcn_permlane32_swap(pack_bf16x2(v[4 * g + 2 * e], v[4 * g + 2 * e + 1]),
+                                                            pack_bf16x2(v[4 * g + 4 + 2 * e], v[4 * g + 4 + 2 * e + 1]), false, false);
+            w[e] = s[0];
+            w[2 + e] = s[1];
         }
-        const uint32_t s0 = half ? a[0] : b[0], s1 = half ? a[1] : b[1];
-        const uint32_t r0 = (uint32_t)__shfl_xor((int)s0, 32, WAVE), r1 = (uint32_t)__shfl_xor((int)s1, 32, WAVE);
-        const u32x4 w = half ? u32x4{r0, r1, b[0], b[1]} : u32x4{a[0], a[1], r0, r1};
         if (valid) out_store16(row + 8 * (g + half), w);
     }
 }
@@ -478,12 +482,11 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void diff_fwd_kernel(const Di
 #pragma unroll
         for (int t = 0; t < NV; ++t) f.o[j][t] = zero16();
     }
-    if (!SPLIT && p.w != nullptr) {                            // (the epilogue's weights: into the cache)
-        const int touch = reinterpret_cast<const int*>(p.w)[lane & (D - 1)];
-        asm volatile("" ::"v"(touch));
-    }
+    int touch = 0;
+    if (!SPLIT && p.w != nullptr) touch = reinterpret_cast<const int*>(p.w)[lane & (D - 1)];      // (the epilogue's weights: into the cache)
     float e1, e2;
     lambda_of<D>(p, h, lane, e1, e2);
+    if constexpr (!SPLIT) asm volatile("" ::"v"(touch));
     const float lam = e1 - e2 + p.lambda_init;
     const uint64_t drow = (uint64_t)bh * (uint64_t)p.Lq + (uint64_t)q;
     if (t0 < t1) t1 = min(t1, live_tiles(kt.mk.row, sk.n, lane));
