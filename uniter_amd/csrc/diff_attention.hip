@@ -18,7 +18,7 @@
 // 1015 TFLOP/s from 16 heads on, d = 32 880; 2048 keys 900 and 700 with 64 heads.  Backward, 28 d flops, 2048 keys and 64 heads: 655 (d = 32),
 // 625 (d = 64).  The vector unit bounds it (two exponentials and about seven more instructions per query, key and map pair: 47 % of the
 // cycles at d = 64, where matrix instructions take 35 %: on one SIMD the two add up).  One query, 16381 keys, 4 x 12 heads: 38 us (5.3 TB/s) and
-// 5 for the join.  32 x 96, 12 heads, d = 32: 11 us forward, 16 with what the backward pass wants kept, 9 + 23 backward: latency.
+// 5 for the join.  32 x 96, 12 heads, d = 32: 10 us forward, 15 with what the backward pass wants kept, 8 + 22 backward: latency.
 // Dropout: two generator calls per lane and 32 keys, in all three loops (32 x 512, 12 heads, d = 32: forward 63 -> 93 us, backward 201 -> 253).
 #include "common.cuh"
 #include "kernels.h"

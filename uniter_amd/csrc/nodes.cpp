@@ -1,8 +1,9 @@
 // nodes.cpp — the autograd nodes of the operators whose calls are short: rotary positions and differential attention.
 //
-// A training call of these operators is three to five kernels of 5 to 25 us.  As Python autograd functions over ctypes their host work is
+// A training call of these operators is two to four kernels of 5 to 25 us.  As Python autograd functions over ctypes their host work is
 // 45 us in a loop that stays in the CPU's caches and twice that when autograd's own thread takes the backward half to another core; here
-// it is C++ on both sides and the backward pass needs no interpreter.  The kernels are reached through the C ABI all the same: the
+// it is C++ on both sides and the backward pass needs no interpreter (32 x 96, 12 heads, forward and gradients, call to call: 167 -> 93 us; one
+// rotary training call 95 -> 49, one token 11.6 -> 7.5).  The kernels are reached through the C ABI all the same: the
 // package hands over the addresses of the entry points of the library that it has loaded (init), nothing is linked.
 //
 // The arguments' checks are here too, for the same reason (ops.py holds the documentation); workspaces come from torch's caching allocator.
