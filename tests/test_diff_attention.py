@@ -390,6 +390,29 @@ def test_strides_and_alignment():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,L", [(1, 7), (3, 1), (1, 1)])
+def test_strides_that_nothing_steps_over(B, L):
+    """A dimension of one has a stride that no address uses: any value of it is taken."""
+    g = torch.Generator().manual_seed(31)
+    heads, dim = 2, 32
+    H = heads * 2 * dim
+    lams, w = params(g, heads, dim)
+    parts = [torch.randn(B, L, H, generator=g).to(BF16).cuda() for _ in range(4)]
+
+    def odd(t):                     # the strides of dimensions of one are 5 and 2^24 + 3
+        room = torch.zeros(B * L * H, dtype=BF16, device="cuda")
+        return room.as_strided((B, L, H), (L * H if B > 1 else 5, H if L > 1 else (1 << 24) + 3, 1)).copy_(t)
+
+    def both(q, k, v, dy):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        y = ops.differential_attention(q, k, v, heads, lams, 0.4, norm_weight=w)
+        return [y.detach(), *torch.autograd.grad(y, (q, k, v), dy)]
+
+    for a, b in zip(both(*map(odd, parts)), both(*parts)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_scores_of_any_size():
     """Large scores: one key takes all the weight of a map; the running maximum moves late in the row."""
     g = torch.Generator().manual_seed(4)

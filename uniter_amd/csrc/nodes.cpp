@@ -56,6 +56,9 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor get(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
 Tensor rows_like(const Tensor& t) { return at::empty_like(t, t.options(), at::MemoryFormat::Contiguous); }
+// strides of [.., rows, columns]; a dimension of one has one that no address uses and that may be anything
+int64_t row_step(const Tensor& t) { return t.size(-2) == 1 ? t.size(-1) : t.stride(-2); }
+int64_t batch_step(const Tensor& t) { return t.size(0) == 1 ? 0 : t.stride(0); }
 // contiguous rows that start on 16 bytes (row strides of whole 8s); a copy where they do not
 Tensor rows16(const Tensor& t) {
     if (t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0) return t;
@@ -219,12 +222,12 @@ void set_rows(A& a, const Tensor& q, const Tensor& k, const Tensor& v) {
     a.q = p;
     a.k = fused ? (p ? p + third : nullptr) : k.data_ptr();
     a.v = fused ? (p ? p + 2 * third : nullptr) : v.data_ptr();
-    a.q_row = q.stride(-2);
-    a.k_row = fused ? a.q_row : k.stride(-2);
-    a.v_row = fused ? a.q_row : v.stride(-2);
-    a.q_batch = q.stride(0);
-    a.k_batch = fused ? a.q_batch : k.stride(0);
-    a.v_batch = fused ? a.q_batch : v.stride(0);
+    a.q_row = row_step(q);
+    a.k_row = fused ? a.q_row : row_step(k);
+    a.v_row = fused ? a.q_row : row_step(v);
+    a.q_batch = batch_step(q);
+    a.k_batch = fused ? a.q_batch : batch_step(k);
+    a.v_batch = fused ? a.q_batch : batch_step(v);
 }
 
 UniterDiffAttention args_of(const Operands& t, const Fixed& f) {
@@ -291,7 +294,7 @@ void diff_backward(const Operands& t, const Fixed& f, const Tensor& saved, const
     const size_t bytes = lib.bwd_bytes(&a);
     Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 16)}, t.q.options().dtype(at::kByte));
     const float* maps = (const float*)saved.data_ptr();
-    ok(lib.bwd(&a, maps ? maps + 2 * dout.numel() : nullptr, maps, dout.data_ptr(), dout.stride(-2), dout.stride(0), &g, ws.data_ptr(), bytes,
+    ok(lib.bwd(&a, maps ? maps + 2 * dout.numel() : nullptr, maps, dout.data_ptr(), row_step(dout), batch_step(dout), &g, ws.data_ptr(), bytes,
                stream_of(t.q)), "uniter_diff_attention_bwd");
 }
 
