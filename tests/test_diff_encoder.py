@@ -89,6 +89,24 @@ def test_no_weight_decay_on_the_head_norm():
     assert id(m.layer[0].attention.self.LayerNorm.weight) in plain
 
 
+@pytest.mark.parametrize("cu,total", [([0, 5, 10], 10), ([0, 5, 10], 13), ([0, 5, 10], 8), ([0, 0, 3, 3, 3, 9, 9], 12), ([0], 4), ([0, 0], 3),
+                                      ([2, 4], 6), ([-5, 3, 50], 7), ([0, 10_000_000], 4), ([0, 6], 0)])
+def test_positions_of_packed_rows(cu, total):
+    """Rows of a sequence count from its first row (bounds cut to the rows there are); rows of none are 0."""
+    want = [0] * total
+    for a, b in zip(cu[:-1], cu[1:]):
+        a, b = (min(max(x, 0), total) for x in (a, b))
+        want[a:b] = range(b - a)
+    got = ops.packed_positions(torch.tensor(cu, dtype=torch.int32), total)
+    assert got.dtype == torch.int64 and got.tolist() == want
+
+
+def test_positions_of_bounds_that_do_not_ascend_stay_in_range():
+    for cu in ([0, 30, 20, 50], [7, 2, 9], [40, 0, 0], [-3, -9, 4]):
+        got = ops.packed_positions(torch.tensor(cu, dtype=torch.int32), 33)
+        assert got.shape == (33,) and ((got >= 0) & (got < 33)).all()
+
+
 # ---- against plain float32 layers ------------------------------------------------------------------------------------------
 class _Round(torch.autograd.Function):
     """Round to bf16 and go on in float32, values and gradients."""
@@ -272,6 +290,23 @@ def test_packed_rows_give_what_padded_rows_give():
         a = e(x, torch.where(mask, 0.0, -math.inf))[-1]
         b = e.forward_packed(x, mask.long(), seq_lens=lens)[-1]
     assert rel_l2(b.float()[mask], a.float()[mask]) < 4e-3 and not b[~mask].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [ROTARY, None])
+def test_packed_layer_with_rows_behind_the_last_sequence(rotary):
+    """Rows that belong to no sequence: zeros, and the others come out as where those rows are a sequence of their own, bit for bit (rows
+    are independent of each other in every product, and the sizes are the same)."""
+    torch.manual_seed(3)
+    att = BertDifferentialSelfAttention(config(rotary=rotary)).cuda().bfloat16().train()
+    x, dy = (torch.randn(15, 128).to(BF16).cuda() for _ in range(2))
+    got = []
+    for cu in ([0, 5, 5, 12], [0, 5, 5, 12, 15]):
+        xg = x.clone().requires_grad_(True)
+        y = att(xg, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"), max_len=7)
+        got.append((y, torch.autograd.grad(y, xg, dy)[0]))
+    for a, b in zip(*got):
+        assert torch.equal(a[:12], b[:12]) and not a[12:].any() and b[12:].any()
 
 
 @pytest.mark.gpu

@@ -909,9 +909,15 @@ def key_mask(attention_mask, hidden_states):
 
 
 def packed_positions(cu_seqlens, total):
-    """int64 [total]: the position of every row inside its sequence (rows stored back to back; no synchronisation)."""
+    """int64 [total]: the position of every row inside its sequence (rows stored back to back; no synchronisation), 0 for rows of no
+    sequence.  Whatever cu_seqlens holds, nothing outside it is read: bounds are cut to the rows there are, as the attention kernels cut them."""
     cu = cu_seqlens.to(torch.int64)
-    return torch.arange(total, device=cu.device) - torch.repeat_interleave(cu[:-1], cu.diff(), output_size=total)
+    rows = torch.arange(total, device=cu.device)
+    if cu.numel() < 2:
+        return torch.zeros_like(rows)
+    first, end = cu[:-1].clamp(0, total), cu[1:].contiguous()
+    at = torch.searchsorted(end, rows, right=True).clamp_(max=end.numel() - 1)
+    return torch.where(rows < end[at], rows - first[at], 0).clamp_(min=0)
 
 
 def _rotary_turn(rot, x, positions, inverse):
