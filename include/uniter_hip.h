@@ -610,7 +610,8 @@ int uniter_attn_pool_bwd(const void* x, const void* w, const float* raw, const f
  * model/model.py:217-245): the pairs of the first rot_dim elements of every head are turned by position * freq[pair].
  *   half layout   (interleaved == 0): pair i is elements i and rot_dim / 2 + i;   interleaved: elements 2 i and 2 i + 1.
  * x, y: bf16 [B, L, heads, head_dim], head elements contiguous, the other three strides free ({batch, token, head}, in elements;
- * 16-byte-aligned heads and rot_dim % 16 == 0 run on 16-byte accesses).  y == x with equal strides turns in place.
+ * 16-byte-aligned heads and rot_dim % 16 == 0 run on 16-byte accesses).  y == x with equal strides turns in place; a y that has
+ * elements in common with x without being x, or with itself, is refused (other strides than x's: where the two ranges meet).
  * inverse != 0 turns back by the same angles, with the same multiplier: the gradient of x from the gradient of y.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct UniterRotary {

@@ -69,6 +69,66 @@ def test_cpu_tensors_and_bad_c_arguments_are_refused():
     assert lib.uniter_rotary(ctypes.byref(r), 64, s, 64, t, None) < 0 and b"in place" in lib.uniter_hip_last_error()
 
 
+def _verdict(lib, sizes, dim, x, sx, y, sy):
+    """What uniter_rotary says of x and y (element addresses) before anything is launched: without frequencies it ends at the null pointer."""
+    import ctypes
+    r = _lib.UniterRotary()
+    r.B, r.L, r.heads = sizes
+    r.head_dim = r.rot_dim = dim
+    A = ctypes.c_int64 * 3
+    assert lib.uniter_rotary(ctypes.byref(r), 2 * x, A(*sx), 2 * y, A(*sy), None) < 0
+    text = lib.uniter_hip_last_error()
+    assert b"overlap" in text or b"null" in text, text
+    return b"overlap" in text
+
+
+def _elements(sizes, dim, at, st):
+    return [at + b * st[0] + l * st[1] + h * st[2] + e for b in range(sizes[0]) for l in range(sizes[1]) for h in range(sizes[2]) for e in range(dim)]
+
+
+def test_overlapping_outputs_are_refused_and_others_are_not():
+    """Against the elements themselves.  Whatever meets is refused; of equal strides, whatever does not meet is taken."""
+    lib = _lib.load()
+    # [L, B, heads, dim] underneath, one row of the batch on: x's second row is y's first
+    assert _verdict(lib, (2, 8, 2), 32, 4096, (64, 256, 32), 4096 + 64, (64, 256, 32))
+    assert not _verdict(lib, (2, 8, 2), 32, 4096, (64, 256, 32), 4096 + 128, (64, 256, 32))
+    import random
+    rng = random.Random(5)
+    seen = [0, 0, 0]
+    for _ in range(6000):
+        sizes, dim = tuple(rng.choice((1, 2, 3)) for _ in range(3)), 2 * rng.choice((1, 1, 2))
+        if rng.random() < 0.7:                       # nested in some order, with gaps or without
+            st, span = [0, 0, 0], dim
+            for i in rng.sample(range(3), 3):
+                st[i] = span + rng.choice((0, 0, 1, dim, 3 * dim))
+                span += (sizes[i] - 1) * st[i]
+        else:
+            st = [rng.randrange(0, 20) for _ in range(3)]
+        if rng.random() < 0.1:
+            st = [-s for s in st]
+        sy = list(st) if rng.random() < 0.8 else [rng.randrange(1, 20) for _ in range(3)]
+        x, y = 4096, 4096 + rng.randrange(-40, 41)
+        if x == y and sy != st:
+            continue                                 # (refused for its strides)
+        ex, ey = _elements(sizes, dim, x, st), _elements(sizes, dim, y, sy)
+        refused = _verdict(lib, sizes, dim, x, st, y, sy)
+        itself = len(set(ey)) < len(ey)
+        if itself or (x != y and set(ex) & set(ey)):
+            assert refused, (sizes, dim, st, sy, y - x)
+            seen[0] += 1
+        elif sy == st:
+            order = sorted((abs(s), n) for s, n in zip(st, sizes) if n > 1)
+            span, nested = dim, True
+            for s, n in order:
+                nested, span = nested and s >= span, span + (n - 1) * s
+            if nested:
+                assert not refused, (sizes, dim, st, sy, y - x)
+                seen[1] += 1
+        elif not refused:
+            seen[2] += 1
+    assert min(seen) > 50, seen
+
+
 # ---- kernels ---------------------------------------------------------------------------------------------------------------
 def turned(x, positions, rot, sign=1.0):
     """float64 result on the CPU: a turned pair is a complex product.  x [.., heads, dim], positions [..]."""
@@ -202,6 +262,35 @@ def test_refusals():
                 lambda: ops.rotary(x[:, :1].expand(2, 3, 4, 64), None, rot, out=x[:, :1].expand(2, 3, 4, 64))):
         with pytest.raises(_lib.UniterHipError):
             bad()
+
+
+@pytest.mark.gpu
+def test_outputs_beside_their_input_in_one_storage():
+    rot = RotaryPositions(32)
+    t = torch.randn(8, 4, 2, 32).to(BF16).cuda()             # [L, B, heads, dim] underneath
+    v = t.transpose(0, 1)
+    want = ops.rotary(v[:2], None, rot)
+    with pytest.raises(_lib.UniterHipError, match="overlap"):
+        ops.rotary(v[:2], None, rot, out=v[1:3])
+    with torch.no_grad():
+        assert torch.equal(ops.rotary(v[:2], None, rot, out=v[2:]), want) and torch.equal(v[2:], want)
+        flat = torch.zeros(400, dtype=BF16, device="cuda")
+        with pytest.raises(_lib.UniterHipError, match="overlap"):      # windows of one another
+            ops.rotary(want[0, :8], torch.arange(8).cuda(), rot, out=flat.as_strided((8, 2, 32), (40, 32, 1)))
+
+
+@pytest.mark.gpu
+def test_strides_that_nothing_steps_over():
+    """A dimension of one has a stride that no address uses: any value of it is taken, also where out is x under another name."""
+    rot = RotaryPositions(32)
+    for shape in ((1, 5, 3, 32), (2, 1, 3, 32), (3, 4, 1, 32), (1, 1, 1, 32)):
+        x = torch.randn(shape).to(BF16).cuda()
+        strange = [s if n > 1 else 7 + i for i, (n, s) in enumerate(zip(shape, x.stride()))]
+        strange[3] = 1
+        want = ops.rotary(x, None, rot, offset=3)
+        assert torch.equal(ops.rotary(x.as_strided(shape, strange), None, rot, offset=3), want)
+        with torch.no_grad():
+            assert torch.equal(ops.rotary(x.as_strided(shape, strange), None, rot, offset=3, out=x), want) and torch.equal(x, want)
 
 
 @pytest.mark.gpu

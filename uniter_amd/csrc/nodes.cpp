@@ -108,7 +108,8 @@ void rotary_run(const Tensor& x, const Tensor& y, const Rotary& r, bool inverse)
     a.multiplier = (float)r.multiplier;
     a.interleaved = r.interleaved;
     a.inverse = inverse;
-    const int64_t sx[3] = {d == 4 ? x.stride(0) : 0, x.stride(-3), x.stride(-2)}, sy[3] = {d == 4 ? y.stride(0) : 0, y.stride(-3), y.stride(-2)};
+    auto step = [d](const Tensor& t, int64_t i) { return d < i || t.size(-i) == 1 ? (int64_t)0 : t.stride(-i); };      // (what nothing steps over may be anything)
+    const int64_t sx[3] = {step(x, 4), step(x, 3), step(x, 2)}, sy[3] = {step(y, 4), step(y, 3), step(y, 2)};
     const c10::DeviceGuard on(x.device());
     ok(lib.rotary(&a, x.data_ptr(), sx, y.data_ptr(), sy, stream_of(x)), "uniter_rotary");
 }
@@ -134,25 +135,6 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
         return once({dx, Tensor()}, grads[0]);
     }
 };
-
-// Whether the address ranges of two views of one storage meet AND their rows can (equal strides and interleaved rows that stay apart — q and
-// k blocks of one projection — do not).
-bool overlap(const Tensor& a, const Tensor& b) {
-    if (a.storage().data() != b.storage().data()) return false;
-    auto end = [](const Tensor& t) {
-        int64_t n = 1;
-        for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
-        return (char*)t.data_ptr() + 2 * n;
-    };
-    const char *a0 = (char*)a.data_ptr(), *b0 = (char*)b.data_ptr();
-    if (end(a) <= b0 || end(b) <= a0) return false;
-    const int64_t row = a.stride(-3), w = a.size(-2) * a.stride(-2);
-    if (a.strides() == b.strides() && row >= w) {              // same row pitch: rows of width w at offsets d apart modulo the pitch
-        const int64_t d = (a0 < b0 ? b0 - a0 : a0 - b0) / 2 % row;
-        return d < w || row - d < w;
-    }
-    return true;
-}
 
 Tensor rotary(Tensor x, const optional<Tensor>& positions, int64_t offset, const optional<Tensor>& out, const Tensor& turns, int64_t head_dim,
               int64_t rot, double multiplier, bool interleaved) {
@@ -188,9 +170,7 @@ Tensor rotary(Tensor x, const optional<Tensor>& positions, int64_t offset, const
         refuse("rotary: out= writes outside autograd; call it without gradients or let it return a new tensor");
     check_beside(x, "x", y, at::kBFloat16, "rotary output");
     if (y.sizes() != x.sizes() || y.stride(-1) != 1) refuse("rotary: out must have x's shape and contiguous heads");
-    for (int64_t i = 0; i < d; ++i)
-        if (y.stride(i) == 0 && y.size(i) > 1) refuse("rotary: out must not be a broadcast view");
-    if (y.numel() != 0 && !(y.data_ptr() == x.data_ptr() && y.strides() == x.strides()) && overlap(y, x)) refuse("rotary: out overlaps x without being x");
+    // (the entry refuses an out that overlaps itself, or x without being x)
     rotary_run(x, y, r, false);
     return y;
 }

@@ -148,6 +148,55 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(const RotArgs p) {
     }
 }
 
+// ---- which elements a call touches: {b * s0 + l * s1 + h * s2 + [0, dim)}, dimensions of more than one with positive strides
+struct Heads {
+    int64_t at;                          // of the lowest element, in elements
+    int64_t n[3], s[3];                  // by descending stride
+    int dims;
+    __int128 span[4];                    // from the lowest to the highest element of dimensions i .. dims - 1 and a head
+    bool apart;                          // no two heads have an element in common (each stride is at least the span inside it)
+};
+Heads heads_of(const UniterRotary* r, const void* base, const int64_t* strides) {
+    const int64_t sizes[3] = {r->B, r->L, r->heads};
+    Heads a{};
+    a.at = (int64_t)((uintptr_t)base >> 1);
+    for (int i = 0; i < 3; ++i) {
+        if (sizes[i] < 2) continue;
+        int64_t s = strides[i];
+        if (s < 0) { a.at += (sizes[i] - 1) * s; s = -s; }
+        int at = a.dims++;
+        for (; at > 0 && a.s[at - 1] < s; --at) { a.s[at] = a.s[at - 1]; a.n[at] = a.n[at - 1]; }
+        a.s[at] = s;
+        a.n[at] = sizes[i];
+    }
+    a.span[a.dims] = r->head_dim;
+    a.apart = true;
+    for (int i = a.dims - 1; i >= 0; --i) {
+        a.apart = a.apart && a.s[i] >= a.span[i + 1];
+        a.span[i] = (__int128)(a.n[i] - 1) * a.s[i] + a.span[i + 1];
+    }
+    return a;
+}
+// Whether heads of two such sets `delta` elements apart meet, both with a's sizes and strides (a.apart): some t with |t_i| < n_i has
+// |delta + sum t_i s_i| < dim.  What the inner dimensions can still add is less than span[i + 1] <= s_i, so only the two t_i next to
+// -delta / s_i come into question.
+bool meet(const Heads& a, int i, __int128 delta) {
+    if (i == a.dims) return delta < a.span[i] && -delta < a.span[i];
+    __int128 t = -delta / a.s[i];
+    if (t * a.s[i] > -delta) --t;                              // (rounded down)
+    for (int k = 0; k < 2; ++k, ++t)
+        if (t > -a.n[i] && t < a.n[i] && meet(a, i + 1, delta + t * a.s[i])) return true;
+    return false;
+}
+// y is another tensor than x and they share an element.  Layouts that differ are taken to share one where their ranges meet.
+bool overlap(const Heads& x, const Heads& y) {
+    const __int128 delta = (__int128)y.at - x.at;
+    if (delta >= x.span[0] || -delta >= y.span[0]) return false;
+    bool alike = x.apart && x.dims == y.dims;
+    for (int i = 0; alike && i < x.dims; ++i) alike = x.s[i] == y.s[i] && x.n[i] == y.n[i];
+    return !alike || meet(x, 0, delta);
+}
+
 }  // namespace
 
 extern "C" int uniter_rotary(const UniterRotary* r, const void* x, const int64_t* x_strides, void* y, const int64_t* y_strides,
@@ -157,7 +206,14 @@ extern "C" int uniter_rotary(const UniterRotary* r, const void* x, const int64_t
     UH_CHECK_ARG(r->head_dim >= 2 && r->head_dim <= 1024, "head_dim must be 2 .. 1024");
     UH_CHECK_ARG(r->rot_dim >= 2 && r->rot_dim % 2 == 0 && r->rot_dim <= r->head_dim, "rot_dim must be even and at most head_dim");
     if (r->B == 0 || r->L == 0) return 0;
-    UH_CHECK_ARG(x && y && r->freq, "null pointer");
+    UH_CHECK_ARG(x && y, "null pointer");
+    const bool same = x == y && x_strides[0] == y_strides[0] && x_strides[1] == y_strides[1] && x_strides[2] == y_strides[2];
+    UH_CHECK_ARG(same || x != y, "in place needs y's strides to be x's");
+    // (a wave writes a token's heads while another may still read: any element in common would be a race)
+    const Heads hy = heads_of(r, y, y_strides);
+    UH_CHECK_ARG(hy.apart, "the heads of y overlap each other");
+    UH_CHECK_ARG(same || !overlap(heads_of(r, x, x_strides), hy), "y overlaps x without being x");
+    UH_CHECK_ARG(r->freq, "null pointer");
     UH_CHECK_ARG(((uintptr_t)r->freq & 7) == 0 && ((uintptr_t)r->positions & 7) == 0 && (((uintptr_t)x | (uintptr_t)y) & 1) == 0, "misaligned pointer");
     UH_CHECK_ARG(r->B <= ((int64_t)1 << 40) / r->L, "too many tokens");
     const int64_t rows = r->B * r->L;
@@ -177,8 +233,6 @@ extern "C" int uniter_rotary(const UniterRotary* r, const void* x, const int64_t
     p.heads = (int)r->heads; p.dim = (int)r->head_dim; p.rot = (int)r->rot_dim;
     p.mult = r->multiplier;
     p.sign = r->inverse ? -1.f : 1.f;
-    const bool same = x == y && p.xb == p.yb && p.xl == p.yl && p.xh == p.yh;
-    UH_CHECK_ARG(same || x != y, "in place needs y's strides to be x's");
     p.copy = !same && p.dim > p.rot;
     const int64_t all = p.xb | p.xl | p.xh | p.yb | p.yl | p.yh | (p.copy ? p.dim : 0);
     const bool wide = p.dim % 8 == 0 && p.dim <= 512 && p.rot % 16 == 0 && all % 8 == 0 && (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
