@@ -280,6 +280,42 @@ def test_frozen_encoders_and_what_the_blocks_refuse():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("blocks", [False, True])
+def test_two_layers_at_work_on_two_streams(blocks):
+    """No scratch is shared: every pass gives the bits of a pass alone, as one node per layer and block by block (a frozen bias)."""
+    cfg = config(2, 128, 2, ROTARY)
+    nets = [encoder(cfg, seed).cuda().train() for seed in (0, 1)]
+    for e in nets:
+        if blocks:
+            for l in e.layer:
+                l.output.dense.bias.requires_grad_(False)
+    g = torch.Generator().manual_seed(9)
+    data = [tuple(torch.randn(3, 40 + 24 * i, 128, generator=g).to(BF16).cuda() for _ in range(2)) for i in range(2)]
+
+    def step(i):
+        x, dy = data[i]
+        for q in nets[i].parameters():
+            q.grad = None
+        xg = x.clone().requires_grad_(True)
+        y = nets[i](xg, torch.zeros(x.shape[:2], device="cuda"))[-1]
+        y.backward(dy)
+        return [y.detach(), xg.grad] + [q.grad for q in nets[i].parameters() if q.requires_grad]
+
+    want = [step(i) for i in range(2)]
+    ops._scratch_cache.clear()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for r in range(8):
+        with torch.cuda.stream(streams[r % 2]):
+            got.append(step(r % 2))
+    torch.cuda.synchronize()
+    assert not ops._scratch_cache                # (buffers of the process, whatever the stream)
+    for r, ts in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(ts, want[r % 2]))
+
+
+@pytest.mark.gpu
 def test_packed_rows_give_what_padded_rows_give():
     cfg = config(2, 128, 2, ROTARY)
     e = encoder(cfg).cuda().eval()

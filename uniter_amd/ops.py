@@ -124,6 +124,12 @@ def _scratch(key, nbytes, device):
     return buf
 
 
+def _workspace(nbytes, device):
+    """Scratch of one launch on the current stream.  From the allocator, not from the cache above: calls on several streams, and captured
+    graphs, each have their own."""
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
 def _dummy_grad_like(t, pool):
     """Scratch gradient buffer for a frozen parameter (result is discarded)."""
     g = pool.get(t.numel())
@@ -658,7 +664,7 @@ def _grad_or_dummy(p, pool):
 def _wgrad_into(dy, x, gw, gb, M, N, K):
     """gw[N, K] += dy[M, N]^T x[M, K]; gb[N] += column sums of dy (gb may be None)."""
     wsb = C.uniter_gemm_wgrad_workspace_bytes(M, N, K)
-    ws = _scratch(("sub_wgrad", dy.device.index), wsb, dy.device)
+    ws = _workspace(wsb, dy.device)
     C.uniter_gemm_wgrad(ptr(dy), ptr(x), ptr(gw), ptr(gb), M, N, K, 1, ptr(ws), wsb, _lib.stream_ptr())
 
 
@@ -694,7 +700,7 @@ class _SelfAttentionFn(torch.autograd.Function):
         dout = dout.contiguous()
         dqkv = torch.empty(T, 3 * H, dtype=_BF16, device=xc.device)
         awb = C.uniter_attention_bwd_workspace_bytes(B, L, heads)
-        aws = _scratch(("sub_attn", xc.device.index), max(awb, 16), xc.device)
+        aws = _workspace(awb, xc.device)
         C.uniter_attention_bwd_ws(ptr(qkv), ptr(mask_bias), None, ptr(out), ptr(lse), ptr(dout), ptr(dqkv), B, L, heads,
                                   ctx.p, ctx.seed, ctx.off, ptr(aws), awb, st)
         wqkv, _ = att.fused_qkv()
@@ -740,7 +746,7 @@ class _DenseDropResLnFn(torch.autograd.Function):
         pool = {}
         ln = mod.LayerNorm
         wsb = C.uniter_layernorm_bwd_workspace_bytes(T, H)
-        ws = _scratch(("ln", z.device.index), wsb, z.device)
+        ws = _workspace(wsb, z.device)
         C.uniter_layernorm_bwd(ptr(dy), None, ptr(z), ptr(mean), ptr(rstd), ptr(ln.weight), ptr(dz), ptr(dd),
                                ptr(_grad_or_dummy(ln.weight, pool)), ptr(_grad_or_dummy(ln.bias, pool)),
                                ptr(_grad_or_dummy(mod.dense.bias, pool)), T, H, 1, ctx.p, ctx.seed, ctx.off, 0, ptr(ws), wsb, st)
@@ -1041,7 +1047,7 @@ class _BertDiffLayerFn(torch.autograd.Function):
         def norm(dy, z, mean, rstd, mod, p, seed, off):
             dz, dd = torch.empty_like(z), torch.empty_like(z)                  # to the residual as it is, to the dense branch through dropout
             wsb = C.uniter_layernorm_bwd_workspace_bytes(T, H)
-            ws = _scratch(("ln", z.device.index), wsb, z.device)
+            ws = _workspace(wsb, z.device)
             ln = mod.LayerNorm
             C.uniter_layernorm_bwd(ptr(dy), None, ptr(z), ptr(mean), ptr(rstd), ptr(ln.weight), ptr(dz), ptr(dd), ptr(ensure_grad(ln.weight)),
                                    ptr(ensure_grad(ln.bias)), ptr(ensure_grad(mod.dense.bias)), T, H, 1, p, seed, off, 0, ptr(ws), wsb, st)
