@@ -163,6 +163,41 @@ def _case_sparse_word_rows(rank, world, D):
             assert float((a - b).abs().max()) <= tol * float(a.abs().max()), (dtype, big_vocab, float((a - b).abs().max()), float(a.abs().max()))
 
 
+def _case_sparse_word_rows_without_layer_calls(rank, world, D):
+    """The same where nothing is reduced before finish(): an encoder whose layers run one by one (differential attention), or none."""
+    from tests.common import IMG_DIM, TINY_CONFIG
+    from uniter_amd.model.model import UniterConfig, UniterModel
+    from uniter_amd.utils.arena import flatten_model
+    cfg = UniterConfig.from_json_file(TINY_CONFIG)
+    cfg.attention_type = "differential"
+    torch.manual_seed(0)
+    model = UniterModel(cfg, IMG_DIM)
+    arena = flatten_model(model)
+    word = model.embeddings.word_embeddings.weight
+    lo, hi = arena.span([word])
+    V, H = word.shape
+    ids = torch.tensor([[3, 3, 5], [7 + rank, 5, 9]])
+    for encoder in (model.encoder, None):
+        results = []
+        for sparse in (False, True):
+            reducer = D.GradientReducer(arena, encoder, word_embeddings=word)
+            assert reducer.word_span is not None and not reducer.buckets
+            arena.grad.fill_(1.0 + rank)
+            rows = torch.zeros(V, dtype=torch.bool)
+            rows[ids.reshape(-1)] = True
+            arena.grad[lo:hi].view(V, H)[~rows] = 0
+            reducer.begin()
+            os.environ["UNITER_AMD_DP_SPARSE_WORD"] = "1"
+            assert reducer.finish(word_ids=ids if sparse else None) == 1.0 / world
+            os.environ.pop("UNITER_AMD_DP_SPARSE_WORD")
+            results.append(arena.grad.clone())
+        total = sum(1.0 + r for r in range(world))
+        assert torch.equal(results[0], results[1])
+        assert (results[1][:lo] == total).all() and (results[1][hi:] == total).all()
+        got = results[1][lo:hi].view(V, H)
+        assert (got[[3, 5, 9]] == total).all() and (got[7] == 1.0).all() and (got[8] == 2.0).all() and not got[0].any()
+
+
 def _case_task_mix_and_retrieval_gather(rank, world, D):
     """MetaLoader: every rank trains the task rank 0 drew.  itm_eval.evaluate: ranks own different numbers of texts, the
     score rows are gathered in rank order and only rank 0 reports (reference utils/itm_eval.py:68-90)."""
@@ -253,6 +288,10 @@ def _case_bf16_sum_over_8_ranks(rank, world, D):
                                   "_case_task_mix_and_retrieval_gather"])
 def test_world_size_2(case, tmp_path):
     _spawn(case, tmp_path)
+
+
+def test_sparse_word_rows_without_layer_calls(tmp_path):
+    _spawn("_case_sparse_word_rows_without_layer_calls", tmp_path)
 
 
 def test_sparse_word_rows_are_the_default_from_four_ranks(tmp_path):

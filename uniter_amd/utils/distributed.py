@@ -450,27 +450,24 @@ class GradientReducer(object):
         sparse = self._armed and _on() and word_ids is not None and self.word_span is not None \
             and os.environ.get("UNITER_AMD_DP_SPARSE_WORD") == "1"
         if self._armed:
-            if self.encoder is None:
-                self._reduce_range(0, self.arena.numel)
-            else:
-                if not self._early_done:
-                    for lo, hi in self.rest_early:
-                        self._reduce_range(lo, hi, after=self._chain_done if self.single_launch else None)
-                if self.single_launch and self._tokens:
-                    # the buckets the backward hook noted, in the order the deferred launch completes them
-                    if any(t is None for t in self._tokens.values()):
-                        from .. import _lib
-                        _lib.load().uniter_encoder_side_join_all(ctypes.c_void_p(self._stream.cuda_stream))
-                    for b in sorted(self._tokens):
-                        self._reduce_range(*self.buckets[b], token=self._tokens[b])
-                    self._tokens = {}
-                for lo, hi in self.rest:
-                    if sparse and lo <= self.word_span[0] and self.word_span[1] <= hi:
-                        # dense around the word table, rows inside it
-                        self._reduce_range(lo, self.word_span[0])
-                        self._reduce_range(self.word_span[1], hi)
-                    else:
-                        self._reduce_range(lo, hi)
+            if not self._early_done:
+                for lo, hi in self.rest_early:
+                    self._reduce_range(lo, hi, after=self._chain_done if self.single_launch else None)
+            if self.single_launch and self._tokens:
+                # the buckets the backward hook noted, in the order the deferred launch completes them
+                if any(t is None for t in self._tokens.values()):
+                    from .. import _lib
+                    _lib.load().uniter_encoder_side_join_all(ctypes.c_void_p(self._stream.cuda_stream))
+                for b in sorted(self._tokens):
+                    self._reduce_range(*self.buckets[b], token=self._tokens[b])
+                self._tokens = {}
+            for lo, hi in self.rest:
+                if sparse and lo <= self.word_span[0] and self.word_span[1] <= hi:
+                    # dense around the word table, rows inside it
+                    self._reduce_range(lo, self.word_span[0])
+                    self._reduce_range(self.word_span[1], hi)
+                else:
+                    self._reduce_range(lo, hi)
         if sparse:
             if self.arena.grad.is_cuda:
                 ev = torch.cuda.Event()
