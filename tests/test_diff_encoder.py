@@ -279,6 +279,37 @@ def test_frozen_encoders_and_what_the_blocks_refuse():
     assert not y.requires_grad
 
 
+PROJECTIONS = ["query.weight", "key.weight", "value.weight", "query.bias", "key.bias", "value.bias"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["differential", "softmax"])
+@pytest.mark.parametrize("arena", [False, True])
+@pytest.mark.parametrize("trained", [PROJECTIONS[3:], PROJECTIONS[:1], ["key.weight", "value.bias"], PROJECTIONS[:3], []])
+def test_partly_frozen_projections(trained, arena, kind):
+    """Trained ones get the gradient that they have when all are trained, bit for bit and over two passes; frozen ones get none."""
+    torch.manual_seed(5)
+    make = BertDifferentialSelfAttention if kind == "differential" else BertSelfAttention
+    x, dy = (torch.randn(2, 40, 128).to(BF16).cuda() for _ in range(2))
+    mask = torch.zeros(2, 40).cuda()
+    full = make(config()).cuda().bfloat16().train()
+    part = copy.deepcopy(full)
+    arenas = [flatten_model(m) for m in (full, part)] if arena else []
+    for n, q in part.named_parameters():
+        q.requires_grad_(n in trained)
+    for _ in range(2):
+        got = []
+        for m in (full, part):
+            xg = x.clone().requires_grad_(True)
+            y = m(xg, mask)
+            y.backward(dy)
+            got.append((y.detach(), xg.grad))
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+        for (n, q), (_, r) in zip(full.named_parameters(), part.named_parameters()):
+            assert torch.equal(q.grad, r.grad) if n in trained else r.grad is None, n
+    assert full.query.weight.grad.any() and all(a.check() for a in arenas)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("blocks", [False, True])
 def test_two_layers_at_work_on_two_streams(blocks):

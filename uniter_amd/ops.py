@@ -668,6 +668,26 @@ def _wgrad_into(dy, x, gw, gb, M, N, K):
     C.uniter_gemm_wgrad(ptr(dy), ptr(x), ptr(gw), ptr(gb), M, N, K, 1, ptr(ws), wsb, _lib.stream_ptr())
 
 
+def _qkv_wgrads(att, dqkv, x, T, H):
+    """Gradients of the query / key / value projections from that of their output dqkv [T, 3 H], accumulated into `.grad`.  Where some of
+    the six parameters are frozen, all thirds are formed in a buffer of their own, on top of the gradients that are there, and only
+    those that are wanted go back: a frozen parameter's `.grad` is not touched."""
+    prm = [m.weight for m in (att.query, att.key, att.value)] + [m.bias for m in (att.query, att.key, att.value)]
+    wanted = [q.requires_grad for q in prm]
+    if not any(wanted):
+        return
+    if all(wanted):
+        gw, gb = att.fused_qkv_grad()
+        return _wgrad_into(dqkv, x, gw, gb, T, 3 * H, H)
+    gw, gb = torch.zeros(3 * H, H, dtype=_BF16, device=x.device), torch.zeros(3 * H, dtype=_BF16, device=x.device)
+    pairs = [(ensure_grad(q), part) for q, w, part in zip(prm, wanted, gw.chunk(3) + gb.chunk(3)) if w]
+    for g, part in pairs:
+        part.copy_(g)
+    _wgrad_into(dqkv, x, gw, gb, T, 3 * H, H)
+    for g, part in pairs:
+        g.copy_(part)
+
+
 class _SelfAttentionFn(torch.autograd.Function):
     """BertSelfAttention.forward (model/layer.py:75-101): fused [3H, H] projection, then softmax(QK^T / sqrt(dh) + mask) V per head."""
 
@@ -708,9 +728,7 @@ class _SelfAttentionFn(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dx = torch.empty_like(xc)
             C.uniter_gemm_dgrad(ptr(dqkv), ptr(wqkv), None, ptr(dx), T, 3 * H, H, st)
-        if any(m.weight.requires_grad for m in (att.query, att.key, att.value)):
-            gw, gb = att.fused_qkv_grad()
-            _wgrad_into(dqkv, xc, gw, gb, T, 3 * H, H)
+        _qkv_wgrads(att, dqkv, xc, T, H)
         return (dx, None, None, None) + (None,) * (len(ctx.needs_input_grad) - 4)
 
 
@@ -985,9 +1003,7 @@ class _BertDiffAttentionFn(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dx = torch.empty_like(xc)
             C.uniter_gemm_dgrad(ptr(dqkv), ptr(att.fused_qkv()[0]), None, ptr(dx), T, 3 * H, H, _lib.stream_ptr())
-        if any(m.weight.requires_grad for m in (att.query, att.key, att.value)):
-            gw, gb = att.fused_qkv_grad()
-            _wgrad_into(dqkv, xc, gw, gb, T, 3 * H, H)
+        _qkv_wgrads(att, dqkv, xc, T, H)
         return (dx,) + (None,) * (len(ctx.needs_input_grad) - 1)
 
 
