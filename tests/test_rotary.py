@@ -350,3 +350,33 @@ def test_other_streams_and_captured_graphs():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, ops.rotary(x, pos, rot))
+
+
+@pytest.mark.gpu
+def test_written_outputs_are_seen_by_autograd():
+    """A tensor that a node has saved and that is then turned in place (or written to) makes that node's backward pass an error, as any
+    in-place operation does; what is only read does not."""
+    rot = RotaryPositions(64)
+    scale = torch.ones(64, dtype=BF16, device="cuda", requires_grad=True)
+    for write in ("x", "out", "view", "read"):
+        cache = torch.randn(2, 9, 3, 64).to(BF16).cuda()
+        y = (cache * scale).sum()                # saves `cache`
+        with torch.no_grad():
+            before = cache._version
+            if write == "x":
+                ops.rotary(cache, None, rot, out=cache)
+            elif write == "out":
+                ops.rotary(torch.zeros_like(cache), None, rot, out=cache)
+            elif write == "view":
+                ops.rotary(torch.zeros_like(cache[:, 2:5]), None, rot, out=cache[:, 2:5])
+            else:
+                ops.rotary(cache, None, rot)
+            assert cache._version == before + (write != "read")
+        if write == "read":
+            y.backward()
+        else:
+            with pytest.raises(RuntimeError, match="inplace"):
+                y.backward()
+    with torch.inference_mode():                 # tensors without a version counter
+        z = torch.zeros(1, 2, 3, 64, dtype=BF16, device="cuda")
+        assert ops.rotary(z, None, rot, out=z) is z

@@ -172,6 +172,7 @@ Tensor rotary(Tensor x, const optional<Tensor>& positions, int64_t offset, const
     if (y.sizes() != x.sizes() || y.stride(-1) != 1) refuse("rotary: out must have x's shape and contiguous heads");
     // (the entry refuses an out that overlaps itself, or x without being x)
     rotary_run(x, y, r, false);
+    if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();      // (a node that saved y, or what shares its memory, has to hear of it)
     return y;
 }
 
