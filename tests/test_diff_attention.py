@@ -723,6 +723,45 @@ def test_cpu_tensors_are_refused():
         ops.differential_attention(t, t, t, 1, (l, l, l, l), 0.5)
 
 
+def _modes_are_refused(q, k, v, lams, w, bias):
+    import torch.autograd.forward_ad as fwAD
+    args = [q, k, v, *lams, w, bias]
+
+    def call(ts):
+        return ops.differential_attention(*ts[:3], 1, ts[3:7], 0.5, norm_weight=ts[7], mask_bias=ts[8])
+
+    with fwAD.dual_level():
+        for i, t in enumerate(args):
+            with pytest.raises(_lib.UniterHipError, match="forward-mode"):
+                call([fwAD.make_dual(a, torch.ones_like(a)) if a is t else a for a in args])
+    with pytest.raises(_lib.UniterHipError, match="trace"):
+        torch.jit.trace(lambda a: call([a] + args[1:]), (q,), check_trace=False)
+
+
+def _mode_inputs(dev):
+    c = dict(dtype=BF16, device=dev)
+    return [torch.zeros(1, 2, 64, **c) for _ in range(3)] + [tuple(torch.zeros(1, 32, **c) for _ in range(4)), torch.ones(64, **c), torch.zeros(1, 2, device=dev)]
+
+
+def test_forward_mode_and_tracing_are_refused_first():
+    """(whatever else the call may have wrong: here, tensors on the CPU)"""
+    import torch.autograd.forward_ad as fwAD
+    q, k, v, lams, w, bias = _mode_inputs("cpu")
+    with fwAD.dual_level():
+        with pytest.raises(_lib.UniterHipError, match="forward-mode"):
+            ops.differential_attention(q, fwAD.make_dual(k, torch.ones_like(k)), v, 1, lams, 0.5)
+    with pytest.raises(_lib.UniterHipError, match="trace"):
+        torch.jit.trace(lambda a: ops.differential_attention(a, k, v, 1, lams, 0.5), (q,), check_trace=False)
+
+
+@pytest.mark.gpu
+def test_forward_mode_and_tracing_are_refused():
+    args = _mode_inputs("cuda")
+    _modes_are_refused(*args)
+    q, k, v, lams, w, bias = args
+    assert ops.differential_attention(q, k, v, 1, lams, 0.5, norm_weight=w, mask_bias=bias).shape == q.shape      # nothing is left over
+
+
 @pytest.mark.gpu
 def test_refusals():
     c = dict(dtype=BF16, device="cuda")

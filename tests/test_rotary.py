@@ -380,3 +380,20 @@ def test_written_outputs_are_seen_by_autograd():
     with torch.inference_mode():                 # tensors without a version counter
         z = torch.zeros(1, 2, 3, 64, dtype=BF16, device="cuda")
         assert ops.rotary(z, None, rot, out=z) is z
+
+
+@pytest.mark.gpu
+def test_forward_mode_and_tracing_are_refused():
+    import torch.autograd.forward_ad as fwAD
+    rot = RotaryPositions(64)
+    x, t = (torch.randn(1, 2, 3, 64).to(BF16).cuda() for _ in range(2))
+    with fwAD.dual_level():
+        d = fwAD.make_dual(x, t)
+        for bad in (lambda: ops.rotary(d, None, rot), lambda: ops.rotary(d[:, 1:], None, rot), lambda: ops.rotary(x.clone(), None, rot, out=d),
+                    lambda: ops.rotary(fwAD.make_dual(x.clone().requires_grad_(True), t), None, rot)):
+            with pytest.raises(_lib.UniterHipError, match="forward-mode"):
+                bad()
+        assert torch.equal(ops.rotary(x, None, rot), ops.rotary(x.clone(), None, rot))        # others go on
+    with pytest.raises(_lib.UniterHipError, match="trace"):
+        torch.jit.trace(lambda a: ops.rotary(a, None, rot), (x,), check_trace=False)
+    ops.rotary(x, None, rot)

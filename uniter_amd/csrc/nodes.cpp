@@ -9,6 +9,7 @@
 // The arguments' checks are here too, for the same reason (ops.py holds the documentation); workspaces come from torch's caching allocator.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/DeviceGuard.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
@@ -50,6 +51,14 @@ void check(const Tensor& t, at::ScalarType type, const char* what) {
 void check_beside(const Tensor& first, const char* name, const Tensor& t, at::ScalarType type, const char* what) {
     check(t, type, what);
     if (t.get_device() != first.get_device()) refuse(what, " is on ", t.device(), ", ", name, " on ", first.device());
+}
+
+// What neither a plain call nor a node here can carry on is refused, not dropped: a forward-mode tangent, and a trace (a launch through
+// a raw pointer leaves nothing in it but the empty result).
+void check_mode(const char* name, std::initializer_list<const Tensor*> inputs) {
+    if (torch::jit::tracer::isTracing()) refuse(name, " cannot be traced: nothing of it would be recorded");
+    for (const Tensor* t : inputs)
+        if (t->defined() && t->_fw_grad(0).defined()) refuse(name, " has no forward-mode derivative");
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -138,6 +147,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
 
 Tensor rotary(Tensor x, const optional<Tensor>& positions, int64_t offset, const optional<Tensor>& out, const Tensor& turns, int64_t head_dim,
               int64_t rot, double multiplier, bool interleaved) {
+    check_mode("rotary", {&x, out.has_value() ? &*out : &x});
     check(x, at::kBFloat16, "rotary input");
     const int64_t d = x.dim();
     if ((d != 3 && d != 4) || x.size(-1) != head_dim)
@@ -316,8 +326,9 @@ Tensor diff_attention(Tensor q, const optional<Tensor>& k_, const optional<Tenso
                       optional<int64_t> max_q, optional<int64_t> max_k, double eps, double p_drop, int64_t seed, int64_t offset) {
     const bool fused = !k_.has_value(), packed = cu_q_.has_value() || cu_k_.has_value();
     const char* name = fused ? "qkv" : "q";
-    check(q, at::kBFloat16, name);
     Tensor k = get(k_), v = get(v_), weight = get(weight_), mask = get(mask_), cu_q = get(cu_q_), cu_k = get(cu_k_), l[4];
+    check_mode("differential attention", {&q, &k, &v, &weight, &mask});
+    check(q, at::kBFloat16, name);
     if (!fused) {
         check_beside(q, name, k, at::kBFloat16, "k");
         check_beside(q, name, v, at::kBFloat16, "v");
@@ -334,6 +345,7 @@ Tensor diff_attention(Tensor q, const optional<Tensor>& k_, const optional<Tenso
     const bool per_head = lams[0].sizes() == at::IntArrayRef({heads, dim});
     if (!per_head && lams[0].sizes() != at::IntArrayRef({dim})) refuse("lambda vectors must be [", dim, "] or [", heads, ", ", dim, "], got ", lams[0].sizes());
     for (int i = 0; i < 4; ++i) {
+        check_mode("differential attention", {&lams[i]});
         check_beside(q, name, lams[i], at::kBFloat16, "lambda vector");
         if (lams[i].sizes() != lams[0].sizes()) refuse("lambda vectors must have one shape, got ", lams[0].sizes(), " and ", lams[i].sizes());
         l[i] = lams[i].contiguous();

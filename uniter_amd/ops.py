@@ -886,7 +886,8 @@ def rotary(x, positions, rot, offset=0, out=None):
     x: bf16 [B, L, heads, head_dim], or [T, heads, head_dim] for rows back to back (a packed batch); any strides with contiguous heads
     (a slice of a fused projection is read in place).  positions: integer tensor [B, L] or [L] ([T]) on x's device, or None for
     0 .. L - 1 (of every row of the batch); `offset` is added to either.  Returns a new tensor; out=x turns x in place, out=another
-    tensor of x's shape writes there (both outside autograd only).  The gradient is turned back by the same kernel."""
+    tensor of x's shape writes there (both outside autograd only).  The gradient is turned back by the same kernel; forward-mode
+    derivatives and torch.jit.trace are refused."""
     _check_dev(x, "rotary input")
     if positions is not None and not isinstance(positions, torch.Tensor):
         raise _lib.UniterHipError("rotary: positions must be an int64 or int32 tensor (or None)")
@@ -904,6 +905,7 @@ def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=Non
     Packed rows: q [T, ..], k / v [Tk, ..], cu_seqlens int32 [examples + 1] on the device and max_len (a longest example's length, host
     int); cu_seqlens_k / max_len_k where the keys' differ.  Rows of no example come back as zeros.
     p_drop: dropout on the difference of the maps (callers pass 0 in evaluation).  Gradients flow to q, k, v, lambdas and norm_weight.
+    Second and forward-mode derivatives and torch.jit.trace are refused.
     Both passes can be captured into a graph; as with any operator, release eager autograd graphs of the same leaves before capturing a
     backward pass."""
     if not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor):
