@@ -763,6 +763,18 @@ def test_forward_mode_and_tracing_are_refused():
 
 
 @pytest.mark.gpu
+def test_a_mask_that_wants_a_gradient_is_refused():
+    q, k, v, lams, w, bias = _mode_inputs("cuda")
+    learned = bias.clone().requires_grad_(True)
+    for m in (learned, 2 * learned, learned[:, None, None, :]):
+        with pytest.raises(_lib.UniterHipError, match="mask_bias"):
+            ops.differential_attention(q, k, v, 1, lams, 0.5, mask_bias=m)
+        with torch.no_grad():
+            assert torch.equal(ops.differential_attention(q, k, v, 1, lams, 0.5, mask_bias=m), ops.differential_attention(q, k, v, 1, lams, 0.5, mask_bias=m.detach()))
+    ops.differential_attention(q, k, v, 1, lams, 0.5, mask_bias=learned.detach())
+
+
+@pytest.mark.gpu
 def test_refusals():
     c = dict(dtype=BF16, device="cuda")
     q, k, l = torch.zeros(2, 3, 128, **c), torch.zeros(2, 4, 128, **c), torch.zeros(2, 32, **c)

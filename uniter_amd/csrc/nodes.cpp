@@ -370,6 +370,7 @@ Tensor diff_attention(Tensor q, const optional<Tensor>& k_, const optional<Tenso
         }
     } else if (mask.defined()) {
         check_beside(q, name, mask, at::kFloat, "mask_bias");
+        if (at::GradMode::is_enabled() && mask.requires_grad()) refuse("mask_bias has no gradient here: pass it detached");
         if (mask.dim() == 4 && mask.size(1) == 1 && mask.size(2) == 1) mask = mask.select(1, 0).select(1, 0);      // UniterModel's extended mask [B, 1, 1, L]
         const int64_t Lk = fused ? q.size(1) : k.size(1);
         if (mask.sizes() != at::IntArrayRef({q.size(0), Lk})) refuse("mask_bias must be [", q.size(0), ", ", Lk, "] (or [B, 1, 1, Lk]), got ", mask.sizes());

@@ -901,9 +901,11 @@ def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=Non
 
     q bf16 [B, Lq, heads * 2 d], k and v [B, Lk, heads * 2 d], d = 32 or 64; any lengths, any strides with contiguous rows.
     lambdas: (q1, k1, q2, k2), each bf16 [heads, d] or [d]: lambda = exp(q1 . k1) - exp(q2 . k2) + lambda_init.  norm_weight: bf16 [2 d].
-    mask_bias: fp32 [B, Lk], added to the scores; -inf removes a key for good, and a row without keys is zeros.
+    mask_bias: fp32 [B, Lk], added to the scores; -inf removes a key for good, and a row without keys is zeros.  It has no gradient (one
+    that requires it is refused).
     Packed rows: q [T, ..], k / v [Tk, ..], cu_seqlens int32 [examples + 1] on the device and max_len (a longest example's length, host
-    int); cu_seqlens_k / max_len_k where the keys' differ.  Rows of no example come back as zeros.
+    int; what an example has beyond it is left out); cu_seqlens_k / max_len_k where the keys' differ (either alone: the other as the
+    queries').  Rows of no example come back as zeros.
     p_drop: dropout on the difference of the maps (callers pass 0 in evaluation).  Gradients flow to q, k, v, lambdas and norm_weight.
     Second and forward-mode derivatives and torch.jit.trace are refused.
     Both passes can be captured into a graph; as with any operator, release eager autograd graphs of the same leaves before capturing a
