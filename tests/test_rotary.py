@@ -46,6 +46,15 @@ def test_bad_configurations_are_refused(kw):
         RotaryPositions(**kw)
 
 
+def test_the_table_is_an_ordinary_tensor_whatever_makes_it():
+    for mode in (torch.inference_mode, torch.no_grad, torch.enable_grad):
+        rot = RotaryPositions(8)
+        with mode():
+            made = rot.turns(torch.device("cpu"))
+        assert not made.is_inference() and rot.turns(torch.device("cpu")) is made
+        assert made.tolist() == [f / (2 * math.pi) for f in rot.inv_freq]
+
+
 def test_cpu_tensors_and_bad_c_arguments_are_refused():
     with pytest.raises(_lib.UniterHipError, match="CUDA"):
         ops.rotary(torch.zeros(1, 2, 1, 64, dtype=BF16), None, RotaryPositions(64))
@@ -397,3 +406,14 @@ def test_forward_mode_and_tracing_are_refused():
     with pytest.raises(_lib.UniterHipError, match="trace"):
         torch.jit.trace(lambda a: ops.rotary(a, None, rot), (x,), check_trace=False)
     ops.rotary(x, None, rot)
+
+
+@pytest.mark.gpu
+def test_first_call_in_inference_mode_then_gradients():
+    rot = RotaryPositions(64)
+    x = torch.randn(1, 7, 3, 64).to(BF16).cuda()
+    with torch.inference_mode():
+        ops.rotary(x, None, rot)
+    y = x.clone().requires_grad_(True)
+    dx, = torch.autograd.grad(ops.rotary(y, None, rot), y, x)
+    close(dx, turned(x, torch.arange(7)[None], rot, -1.0), x, rot)

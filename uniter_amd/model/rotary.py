@@ -94,7 +94,8 @@ class RotaryPositions(object):
         t = self._turns.get(device)
         if t is None:
             device = torch.device(device)
-            t = torch.tensor([f / (2.0 * math.pi) for f in self.inv_freq], dtype=torch.float64, device=device)
+            with torch.inference_mode(False):   # (an ordinary tensor whatever the first call runs in: later ones may have gradients)
+                t = torch.tensor([f / (2.0 * math.pi) for f in self.inv_freq], dtype=torch.float64, device=device)
             self._turns[device] = t
         return t
 
