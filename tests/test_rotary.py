@@ -417,3 +417,25 @@ def test_first_call_in_inference_mode_then_gradients():
     y = x.clone().requires_grad_(True)
     dx, = torch.autograd.grad(ops.rotary(y, None, rot), y, x)
     close(dx, turned(x, torch.arange(7)[None], rot, -1.0), x, rot)
+
+
+@pytest.mark.gpu
+def test_a_first_call_under_capture_is_refused_and_the_capture_goes_on():
+    rot = RotaryPositions(64)
+    x = torch.randn(1, 7, 3, 64).to(BF16).cuda()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(_lib.UniterHipError, match="capture"):
+            ops.rotary(x, None, rot)
+        y = x * 2
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, x * 2)
+    want = ops.rotary(x, None, rot)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.rotary(x, None, rot)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)

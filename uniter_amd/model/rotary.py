@@ -90,10 +90,13 @@ class RotaryPositions(object):
         return out
 
     def turns(self, device):
-        """float64 [rotary_dim / 2] on `device`: turns per position (angle / 2 pi), made once per device."""
+        """float64 [rotary_dim / 2] on `device`: turns per position (angle / 2 pi), made once per device.  Not while a graph is being captured:
+        the table outlives the graph, and its copy from the host could not be captured."""
         t = self._turns.get(device)
         if t is None:
             device = torch.device(device)
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise UniterHipError("rotary: the first call on %s cannot be captured; call it (or turns(%r)) once before the capture" % (device, str(device)))
             with torch.inference_mode(False):   # (an ordinary tensor whatever the first call runs in: later ones may have gradients)
                 t = torch.tensor([f / (2.0 * math.pi) for f in self.inv_freq], dtype=torch.float64, device=device)
             self._turns[device] = t
