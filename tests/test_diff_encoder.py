@@ -279,6 +279,34 @@ def test_frozen_encoders_and_what_the_blocks_refuse():
     assert not y.requires_grad
 
 
+def test_projections_fused_in_inference_mode_stay_trainable():
+    att = BertDifferentialSelfAttention(config())
+    before = [q.detach().clone() for q in att.parameters()]
+    with torch.inference_mode():
+        w, b = att.fused_qkv()
+    assert not w.is_inference() and not any(q.is_inference() or q.data.is_inference() for q in att.parameters())
+    assert all(torch.equal(q, o) for q, o in zip(att.parameters(), before)) and w.data_ptr() == att.query.weight.data_ptr()
+    att.query(torch.ones(1, 128)).sum().backward()
+    assert att.query.weight.grad.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [ROTARY, None])
+def test_evaluation_in_inference_mode_before_training(rotary):
+    e = encoder(config(rotary=rotary)).cuda()
+    other = copy.deepcopy(e)
+    x, dy = (torch.randn(2, 40, 128).to(BF16).cuda() for _ in range(2))
+    mask = torch.zeros(2, 40).cuda()
+    with torch.inference_mode():
+        seen = e.eval()(x, mask)[-1]
+    got = []
+    for m in (e, other):
+        y = m.train()(x, mask)[-1]
+        y.backward(dy)
+        got.append([y.detach()] + [q.grad for q in m.parameters()])
+    assert torch.equal(seen, got[0][0]) and all(torch.equal(a, b) for a, b in zip(*got))
+
+
 PROJECTIONS = ["query.weight", "key.weight", "value.weight", "query.bias", "key.bias", "value.bias"]
 
 

@@ -108,7 +108,8 @@ class BertSelfAttention(nn.Module):
                 self._qkv_w = torch.as_strided(ws[0].data, (3 * ws[0].shape[0], H), (H, 1))
                 self._qkv_b = torch.as_strided(bs[0].data, (3 * bs[0].shape[0],), (1,))
             return self._qkv_w, self._qkv_b
-        with torch.no_grad():
+        # (ordinary storages whatever the first call runs in: parameters set to inference tensors would get no gradient ever after)
+        with torch.inference_mode(False), torch.no_grad():
             fw = torch.cat([w.data for w in ws], dim=0).contiguous()
             fb = torch.cat([b.data for b in bs], dim=0).contiguous()
             n = ws[0].shape[0]
