@@ -325,6 +325,25 @@ def test_no_key_left_among_many(dim, Lq, Lk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,Lq,Lk", [(32, 1, 3000), (64, 40, 70), (32, 70, 40), (64, 1, 3000)])
+def test_a_mask_entry_that_is_nan_shows(dim, Lq, Lk):
+    """Every score sum of that example holds it: NaN in all its rows and gradients, as in the formula; the other example is as without it."""
+    g = torch.Generator().manual_seed(Lk + dim)
+    H = 2 * 2 * dim
+    q, k, v, dy = (torch.randn(2, n, H, generator=g).to(BF16).cuda() for n in (Lq, Lk, Lk, Lq))
+    lams, w = params(g, 2, dim)
+    bias = torch.zeros(2, Lk).cuda()
+    want, grads = run_all(q, k, v, 2, lams, 0.5, w, dy, mask_bias=bias)
+    for at in (0, Lk // 2, Lk - 1):
+        bad = bias.clone()
+        bad[1, at] = math.nan
+        assert whole(q[1:], k[1:], v[1:], 2, lams, 0.5, w, 1e-5, bias=bad[1:])["out"][0].isnan().all()
+        out, d = run_all(q, k, v, 2, lams, 0.5, w, dy, mask_bias=bad)
+        assert out[1].isnan().all() and all(d[n][1].isnan().all() for n in "qkv") and all(d[n].isnan().all() for n in ("lq1", "w"))
+        assert torch.equal(out[0], want[0]) and all(torch.equal(d[n][0], grads[n][0]) for n in "qkv")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", [32, 64])
 def test_one_token_after_the_other_against_a_cache(dim):
     """Serving: a prompt of 37 tokens, then single ones; keys are turned straight into a cache that is longer than what it holds (NaN behind),

@@ -182,7 +182,7 @@ __device__ __forceinline__ Span span_of(const int32_t* cu, const int64_t total, 
 // additive mask in log2 units; the type's lowest value stays finite and above NONE, the reference of a row without keys yet (a row of
 // nothing but lowest values is uniform over its keys)
 constexpr float NONE = -3.4028234663852886e38f;
-__device__ __forceinline__ float mask_log2(const float m) { return m == -INFINITY ? m : fmaxf(m * LOG2E, -3e38f); }
+__device__ __forceinline__ float mask_log2(const float m) { return m == -INFINITY ? m : max2(m * LOG2E, -3e38f); }      // (a NaN stays one)
 
 // ---- tiles by direct global -> LDS transfers (global_load_lds_dwordx4: a wave instruction moves 64 x 16 bytes to a contiguous 1 KiB
 // of LDS, so the swizzle is applied to the source address).  The origin of a tile is scalar, a lane's offset inside it 32 bits (the entry
