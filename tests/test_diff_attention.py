@@ -324,6 +324,42 @@ def test_no_key_left_among_many(dim, Lq, Lk):
         assert (over <= 0).all(), (n, float(over.max()))
 
 
+def with_roundings(q, k, v, lam, lam_init, w, dim, dy, rnd):
+    """One head in float64, (out, dq, dk, dv); rnd: applied where the kernels round to bf16."""
+    S = [q[:, j * dim:(j + 1) * dim] @ k[:, j * dim:(j + 1) * dim].T * dim ** -0.5 for j in range(2)]
+    e = [(s - s.amax(1, keepdim=True)).exp() for s in S]
+    P = [x / x.sum(1, keepdim=True) for x in e]
+    O = [rnd(x) @ v / x.sum(1, keepdim=True) for x in e]
+    o = O[0] - lam * O[1]
+    r = (o.square().mean(1, keepdim=True) + 1e-5).rsqrt()
+    du = (1 - lam_init) * w * dy
+    do = rnd(r * (du - o * r * r * (du * o).mean(1, keepdim=True)))
+    dS = [rnd(p * (do @ v.T - (do * x).sum(1, keepdim=True))) * f * dim ** -0.5 for f, p, x in ((1.0, P[0], O[0]), (-lam, P[1], O[1]))]
+    dq = torch.cat([t @ k[:, j * dim:(j + 1) * dim] for j, t in enumerate(dS)], 1)
+    dk = torch.cat([t.T @ q[:, j * dim:(j + 1) * dim] for j, t in enumerate(dS)], 1)
+    return rnd((1 - lam_init) * w * o * r), rnd(dq), rnd(dk), rnd(rnd(P[0] - lam * P[1]).T @ do)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,L,shift", [(32, 130, 16.0), (64, 70, 16.0), (32, 40, 4.0), (64, 200, 1.0)])
+def test_values_with_a_common_part(dim, L, shift):
+    """What all values have in common cancels in G - D, so it must not come back as an error of dQ and dK: these are held to 1.5 times what the
+    formula with the kernels' roundings written out is off by (other draws of the same sizes, and the fp32 sums beside them)."""
+    g = torch.Generator().manual_seed(L)
+    H = 2 * dim
+    q, k, v, dy = (torch.randn(L, H, generator=g) for _ in range(4))
+    q, k, v, dy = (t.to(BF16) for t in (q, k, v + shift, dy))
+    lams, w = params(g, 1, dim)
+    out, grads = run_all(*(t[None].cuda() for t in (q, k, v)), 1, lams, 0.5, w, dy[None].cuda())
+    l = [t.double().cpu()[0] for t in lams]
+    lam = float((l[0] * l[1]).sum().exp() - (l[2] * l[3]).sum().exp() + 0.5)
+    args = [t.double() for t in (q, k, v)] + [lam, 0.5, w.double().cpu(), dim, dy.double()]
+    exact, rounded = (with_roundings(*args, rnd) for rnd in (lambda t: t, lambda t: t.to(BF16).double()))
+    for n, got, x, y in zip(("out", "q", "k", "v"), (out, grads["q"], grads["k"], grads["v"]), exact, rounded):
+        off, room = float((got[0].double().cpu() - x).norm() / x.norm()), float((y - x).norm() / x.norm())
+        assert off < 1.5 * room, (n, off, room)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim,Lq,Lk", [(32, 1, 3000), (64, 40, 70), (32, 70, 40), (64, 1, 3000)])
 def test_a_mask_entry_that_is_nan_shows(dim, Lq, Lk):
