@@ -439,6 +439,21 @@ def test_model_trains_with_the_optimizer_and_dropout(loss):
 
 
 @pytest.mark.gpu
+def test_positions_in_every_form_that_rotary_takes():
+    torch.manual_seed(1)
+    att = BertDifferentialSelfAttention(config(rotary=ROTARY)).cuda().bfloat16()
+    x = torch.randn(3, 9, 128).to(BF16).cuda()
+    pos = torch.randint(0, 500, (9,)).cuda()
+    want = att(x, positions=pos.expand(3, 9).contiguous())
+    for p in (pos, pos[None], pos.int()[None], pos.expand(3, 9)):
+        assert torch.equal(att(x, positions=p), want)
+    assert torch.equal(att(x[:1], positions=pos[None]), want[:1])
+    for bad in (pos[None, None], pos[None, :8], pos.expand(2, 9)):
+        with pytest.raises(_lib.UniterHipError, match="positions"):
+            att(x, positions=bad)
+
+
+@pytest.mark.gpu
 def test_module_refusals():
     att = BertDifferentialSelfAttention(config(rotary=ROTARY)).cuda().bfloat16()
     x = torch.zeros(2, 5, 128, dtype=BF16, device="cuda")

@@ -1125,6 +1125,8 @@ def _bert_diff_inputs(att, hidden_states, attention_mask, positions, cu_seqlens,
         if att.rotary is None:
             raise _lib.UniterHipError("positions are given, but this attention has no rotary positions (config.rotary)")
         rows = hidden_states.shape[:-1]
+        if isinstance(positions, torch.Tensor) and not packed and positions.dim() == 2 and positions.shape[0] == 1:
+            positions = positions[0]                       # [1, L]: one row for the whole batch, as a model's position ids come
         if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int64, torch.int32) or positions.device != hidden_states.device \
                 or (positions.shape != rows and positions.shape != rows[-1:]):
             raise _lib.UniterHipError("positions must be an integer tensor %s or %s on %s" % (list(rows), list(rows[-1:]), hidden_states.device))
