@@ -307,6 +307,15 @@ def test_evaluation_in_inference_mode_before_training(rotary):
     assert torch.equal(seen, got[0][0]) and all(torch.equal(a, b) for a, b in zip(*got))
 
 
+def test_tile_indices_are_those_of_the_gemm_kernels():
+    """ops asks for the deep-pipelined tiles by index; gemm.hip asserts that these entries of its table are the tiles that they are named for."""
+    import os
+    import re
+    with open(os.path.join(os.path.dirname(ops.__file__), "csrc", "gemm.hip")) as f:
+        found = re.search(r"constexpr int kTileG8 = (\d+), kTileG6 = (\d+);", f.read())
+    assert (ops._TILE_256, ops._TILE_192) == tuple(int(x) for x in found.groups())
+
+
 PROJECTIONS = ["query.weight", "key.weight", "value.weight", "query.bias", "key.bias", "value.bias"]
 
 

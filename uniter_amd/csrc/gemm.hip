@@ -1067,7 +1067,8 @@ constexpr TileShape kTiles[] = {{128, 128, 2, 0}, {128, 64, 2, 0}, {64, 128, 2, 
                                 {192, 192, 3, 4},
                                 // round 5 (after the LDS-DMA issue fix the big 8 + 4 tiles win the wide outputs): deeper rings of those
                                 {192, 192, 3, 2}, {96, 192, 4, 2}, {192, 96, 4, 2}};
-constexpr int kTileG8 = 58, kTileG6 = 59;
+constexpr int kTileG8 = 58, kTileG6 = 59;                      // (ops.py names them too)
+static_assert(kTiles[kTileG8].ws == 3 && kTiles[kTileG8].bm == 256 && kTiles[kTileG6].ws == 4 && kTiles[kTileG6].bm == 192, "tile indices");
 constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 
 template <bool TRA, bool TRB>
