@@ -92,8 +92,10 @@ def test_no_weight_decay_on_the_head_norm():
 @pytest.mark.parametrize("cu,total", [([0, 5, 10], 10), ([0, 5, 10], 13), ([0, 5, 10], 8), ([0, 0, 3, 3, 3, 9, 9], 12), ([0], 4), ([0, 0], 3),
                                       ([2, 4], 6), ([-5, 3, 50], 7), ([0, 10_000_000], 4), ([0, 6], 0)])
 def test_positions_of_packed_rows(cu, total):
-    """Rows of a sequence count from its first row (bounds cut to the rows there are); rows of none are 0."""
+    """Rows of a sequence count from its first row (bounds cut to the rows there are), those behind the last one from its end; others are 0."""
     want = [0] * total
+    last = min(max(cu[-1], 0), total)
+    want[last:] = range(total - last)
     for a, b in zip(cu[:-1], cu[1:]):
         a, b = (min(max(x, 0), total) for x in (a, b))
         want[a:b] = range(b - a)

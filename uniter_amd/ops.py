@@ -937,15 +937,14 @@ def key_mask(attention_mask, hidden_states):
 
 
 def packed_positions(cu_seqlens, total):
-    """int64 [total]: the position of every row inside its sequence (rows stored back to back; no synchronisation), 0 for rows of no
-    sequence.  Whatever cu_seqlens holds, nothing outside it is read: bounds are cut to the rows there are, as the attention kernels cut them."""
-    cu = cu_seqlens.to(torch.int64)
-    rows = torch.arange(total, device=cu.device)
-    if cu.numel() < 2:
-        return torch.zeros_like(rows)
-    first, end = cu[:-1].clamp(0, total), cu[1:].contiguous()
-    at = torch.searchsorted(end, rows, right=True).clamp_(max=end.numel() - 1)
-    return torch.where(rows < end[at], rows - first[at], 0).clamp_(min=0)
+    """int64 [total]: the position of every row inside its sequence (rows stored back to back; no synchronisation).  Rows behind the last
+    sequence count on from its end, rows before the first are 0.  Whatever cu_seqlens holds, nothing outside it is read: a search
+    among its n + 1 bounds, cut to the rows there are, answers 0 .. n."""
+    rows = torch.arange(total, device=cu_seqlens.device)
+    if cu_seqlens.numel() < 2:
+        return rows
+    cu = cu_seqlens.to(torch.int64).clamp(0, total)
+    return rows.sub_(cu[torch.searchsorted(cu[1:], rows, right=True)]).clamp_(min=0)
 
 
 def _rotary_turn(rot, x, positions, inverse):
