@@ -14,12 +14,19 @@
 // One pass over the keys with running maximum and sum of BOTH maps and one accumulator each: 12 d flops per (query, key) against the
 // 8 d of a product with the finished difference, which would need both sums first.
 //
-// Measured (MI355X; a library bf16 product of 8192^3 reaches 1195 TFLOP/s, a large copy 5.0 TB/s).  Forward, 12 d flops: 8192 keys d = 64
-// 1015 TFLOP/s from 16 heads on, d = 32 880; 2048 keys 900 and 700 with 64 heads.  Backward, 28 d flops, 2048 keys and 64 heads: 655 (d = 32),
-// 625 (d = 64).  The vector unit bounds it (two exponentials and about seven more instructions per query, key and map pair: 47 % of the
-// cycles at d = 64, where matrix instructions take 35 %: on one SIMD the two add up).  One query, 16381 keys, 4 x 12 heads: 38 us (5.3 TB/s) and
-// 5 for the join.  32 x 96, 12 heads, d = 32: 10 us forward, 15 with what the backward pass wants kept, 8 + 22 backward: latency.
-// Dropout: two generator calls per lane and 32 keys, in all three loops (32 x 512, 12 heads, d = 32: forward 63 -> 93 us, backward 201 -> 253).
+// Measured (MI355X; a library bf16 product of 8192^3 reaches 1200 TFLOP/s, a large copy 5.0 TB/s).  Forward, 12 d flops: 8192 keys d = 64
+// 1000 TFLOP/s from 16 heads on, d = 32 870; 2048 keys 910 and 710 with 64 heads.  Backward, 28 d flops, 2048 keys and 64 heads: 670 (d = 32),
+// 620 (d = 64).  The vector unit bounds it (two exponentials and about seven more instructions per query, key and map pair): forward at 8192
+// keys it is busy 57 % of the SIMDs' cycles at d = 64 and the matrix cores 45 %, at d = 32 79 and 39 %: on one SIMD the two add up.  One
+// query, 16381 keys, 4 x 12 heads: 36 us (5.5 TB/s) and 5 for the join.  32 x 96, 12 heads, d = 32: 10 us forward, 16 with what the backward
+// pass wants kept, 8 + 23 backward: latency.  Dropout: two generator calls per lane and 32 keys, in all three loops (32 x 512, 12 heads,
+// d = 32: forward 61 -> 100 us, backward 206 -> 252).
+//
+// Roundings to bf16, besides that of each result: the matrix cores take 16-bit operands, so what is formed in between and multiplied once more
+// is rounded for them, each value once and by half a step (2^-9) at most — the weights exp(S - m) of the products with V (their sums l
+// keep 32 bits), A = P_1 - lambda P_2 for dV, dS_1 / dS_2 for dQ and dK, and the norm's gradient dO for all three.  Products, maxima, sums,
+// the maps' outputs kept for the backward pass, D and lambda are 32 bits.  Outputs are 2.5 - 2.7e-3 from the 64-bit result and gradients 3.0 -
+// 3.3e-3, where 32 bits rounded once at the end give 1.7 - 1.9e-3.
 #include "common.cuh"
 #include "kernels.h"
 #include "../../include/uniter_hip.h"
@@ -186,7 +193,7 @@ __device__ __forceinline__ float mask_log2(const float m) { return m == -INFINIT
 
 // ---- tiles by direct global -> LDS transfers (global_load_lds_dwordx4: a wave instruction moves 64 x 16 bytes to a contiguous 1 KiB
 // of LDS, so the swizzle is applied to the source address).  The origin of a tile is scalar, a lane's offset inside it 32 bits (the entry
-// checks the row strides).  Rows behind the end are read from the last row there is: their weight is zero, see fix_rows.
+// checks the row strides).  Rows behind the end are read from the last row there is: their weight is zero, see zero_rows.
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
@@ -738,9 +745,9 @@ __global__ __launch_bounds__(256) void diff_bwd_rows_kernel(const DiffArgs p, co
 #pragma unroll
             for (int e = 0; e < 8; ++e) d[e] = dy[e];
         }
-        // The products that follow take dO as a bf16 operand, and D from the same rounded values: what all v have in common cancels in G - D
-        // only so (130 x 130, d = 32, v = noise + 16: dQ 3.0e-3 from the 64-bit result, with D from before the rounding 4.7e-2; 0.1 - 0.2 us).  dlambda = -sum D_2 takes no
-        // difference and keeps the 32 bits.
+        // The products that follow take dO as a bf16 operand, and D is formed from the same rounded values: what all v have in common cancels
+        // in G - D only so (130 x 130, d = 32, v = noise + 16: dQ 3.0e-3 from the 64-bit result, with D from before the rounding 4.7e-2;
+        // costs 0.1 - 0.2 us).  dlambda = -sum D_2 takes no difference and keeps the 32 bits.
         const u32x4 db = pack8(d);
         float dr[8], d1 = 0.f, d2 = 0.f;
         unpack8(db, dr);
@@ -1361,8 +1368,8 @@ int launch_bwd(const DiffArgs& p, const BwdSpace& s, const ParamGrads& g, hipStr
         return BwdGrid{div_of(nb > 0 ? nb : 1), div_of(gr.chunk), gr.total, (int)gr.blocks};
     };
     const bool drop = p.drop.p > 0.f;
-    // d = 32: one launch for dQ and dK / dV, which fill the chip better together than one after the other (d = 32, 28 d flops counted:
-    // 4 heads x 2048 tokens 87 us against 130, 64 heads 371 against 368).  d = 64: dK / dV needs a register budget of its own.
+    // d = 32: one launch for dQ and dK / dV, which fill the chip better together than one after the other (2048 tokens, whole backward pass:
+    // 4 heads 76 us against 135, 16 heads 100 against 151, 64 heads 360 against 479).  d = 64: dK / dV needs a register budget of its own.
     if constexpr (D == 32) {
         const int nw = p.Lq > p.Lk ? waves_for(p.Lq) : waves_for(p.Lk);
         const BwdGrid gk = plan(p.Lk, nw), gq = plan(p.Lq, nw);

@@ -10,9 +10,9 @@
 //
 // What bounds it: HBM (4 bytes per element, ~1 flop).  One wave takes one token.  No table is read: a wave forms each pair's sine and
 // cosine once (half a dozen 64-bit instructions per pair) and hands them round through LDS.  Measured: 32749 tokens of 24 heads of 64, half
-// of each turned, 38.8 us (5.2 TB/s, a plain copy of that size takes 35 - 39); with a lane holding both halves of 8 pairs (32-byte
-// pieces of a row per load, each angle formed by every head's lanes) it was 52.7 us.  2848 tokens of 32 heads: 6 us, of which 3.5 are the
-// launch.  One token: 2 us in the kernel.
+// of each turned, 38.8 us (5.2 TB/s; 31 on inputs that the Infinity Cache partly holds, where a plain copy takes 28); with a lane holding
+// both halves of 8 pairs (32-byte pieces of a row per load, each angle formed by every head's lanes) it was 52.7 us.  2848 tokens of 32
+// heads: 6 us, of which 3.5 are the launch.  One token: 2.7 us in the kernel.
 #include "common.cuh"
 #include "kernels.h"
 #include "../../include/uniter_hip.h"

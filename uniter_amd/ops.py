@@ -906,7 +906,8 @@ def differential_attention(q, k, v, heads, lambdas, lambda_init, norm_weight=Non
     Packed rows: q [T, ..], k / v [Tk, ..], cu_seqlens int32 [examples + 1] on the device and max_len (a longest example's length, host
     int; what an example has beyond it is left out); cu_seqlens_k / max_len_k where the keys' differ (either alone: the other as the
     queries').  Rows of no example come back as zeros.
-    p_drop: dropout on the difference of the maps (callers pass 0 in evaluation).  Gradients flow to q, k, v, lambdas and norm_weight.
+    p_drop: dropout on the difference of the maps (callers pass 0 in evaluation); the draws are the host's, so a captured call repeats its own
+    at every replay.  Gradients flow to q, k, v, lambdas and norm_weight.
     Second and forward-mode derivatives and torch.jit.trace are refused.
     Both passes can be captured into a graph; as with any operator, release eager autograd graphs of the same leaves before capturing a
     backward pass."""
@@ -1016,8 +1017,8 @@ _TILE_192, _TILE_256 = 59, 58
 
 def _layer_wgrads(dys, xs_, dws, dbs, T, Ns, Ks, training):
     """The four weight gradients of a layer in one launch, on the widest deep-pipelined tile that fits: the base encoder's layer at 32 x 96
-    tokens 62 us on 192 x 192 (256 x 256: 77, 128 x 128: 112), the large one's at 2880 tokens 84 us on 256 x 256 (128 x 128: 184), base at 320
-    tokens 15.5 against 14.4 of the best small tile.  Rows that are not a multiple of 64 take the tuned tile (wgrad_group)."""
+    tokens 63 us on 192 x 192 (256 x 256: 77, 128 x 128: 112), the large one's at 2880 tokens 84 us on 256 x 256 (128 x 128: 184), base at 320
+    tokens 15.4 (128 x 128: 22).  Rows that are not a multiple of 64 take the tuned tile (wgrad_group)."""
     tile = next((c for c, e in ((_TILE_192, 192), (_TILE_256, 256)) if T % 64 == 0 and all(n % e == 0 for n in Ns + Ks)), None)
     if tile is None:
         return wgrad_group(dys, [0] * 4, xs_, [0] * 4, dws, dbs, T, Ns, Ks, training)
