@@ -318,6 +318,16 @@ def test_tile_indices_are_those_of_the_gemm_kernels():
     assert (ops._TILE_256, ops._TILE_192) == tuple(int(x) for x in found.groups())
 
 
+def test_a_mask_that_wants_a_gradient_is_refused():
+    x, learned = torch.zeros(2, 3, 128), torch.zeros(2, 3, requires_grad=True)
+    for m in (learned, 2 * learned[:, None, None, :]):
+        with pytest.raises(_lib.UniterHipError, match="detached"):
+            ops.key_mask(m, x)
+        with torch.no_grad():
+            assert ops.key_mask(m, x).shape == (2, 3)
+    assert ops.key_mask(learned.detach(), x).shape == (2, 3) and ops.key_mask(None, x) is None
+
+
 PROJECTIONS = ["query.weight", "key.weight", "value.weight", "query.bias", "key.bias", "value.bias"]
 
 

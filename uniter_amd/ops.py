@@ -931,6 +931,8 @@ def key_mask(attention_mask, hidden_states):
     """The additive key mask of dense hidden_states [B, L, H] as fp32 [B, L] (None stays None)."""
     if attention_mask is None:
         return None
+    if attention_mask.requires_grad and torch.is_grad_enabled():
+        raise _lib.UniterHipError("attention_mask has no gradient here: pass it detached")
     B, L = hidden_states.shape[0], hidden_states.shape[1]
     if attention_mask.numel() != B * L:
         raise _lib.UniterHipError("attention_mask must have B*L elements (got %d for B=%d L=%d)" % (attention_mask.numel(), B, L))
